@@ -45,7 +45,8 @@ enum spanqr_status {
     SPANQR_ERR_WORKSPACE = 3, /* workspace too small or not 256-byte aligned                                    */
     SPANQR_ERR_CUDA = 4,      /* a CUDA runtime call or kernel launch failed                                    */
     SPANQR_ERR_DEVICE = 5,    /* the device status word reports a failure (spanqr_read_status)                  */
-    SPANQR_ERR_TOO_LARGE = 6  /* the shape needs more scratch than spanqr_orth_noalloc_f32's fixed array holds     */
+    SPANQR_ERR_TOO_LARGE = 6, /* the shape needs more scratch than spanqr_orth_noalloc_f32's fixed array holds     */
+    SPANQR_ERR_OVERLAP = 7    /* an output overlaps another tensor of the call                                    */
 };
 
 /* version as MAJOR * 10000 + MINOR * 100 + PATCH */
@@ -234,6 +235,35 @@ int spanqr_peer_slab_open(const void* handle, void** ptr);
 int spanqr_peer_slab_close(void* ptr);
 int spanqr_peer_slab_free(void* ptr);
 int spanqr_peer_copy(void* dst, const void* src, size_t bytes, spanqr_stream_t stream);
+
+/* element types of the entry points below */
+enum spanqr_dtype { SPANQR_F32 = 0, SPANQR_F16 = 1, SPANQR_BF16 = 2 };
+
+/*
+ * The global L2 norm of a list of gradients and its clipping (no reference counterpart: these stand before orth in an
+ * optimizer step).  in[i], out[i] are device pointers to n[i] contiguous elements of type in_type[i], out_type[i]
+ * (host arrays of length count, read during the call only), each aligned to its element.  Lists of any length and
+ * empty tensors are fine.  The norm is
+ *     sqrt(sum of the squares of every element),
+ * summed in fp64 (fp32 inside a 32-byte vector, rescaled where squares would leave fp32's range) in a fixed order:
+ * deterministic, and a tensor listed twice counts twice.
+ *
+ * spanqr_grad_norm writes the sum of squares to *sumsq and the norm to *norm (device pointers; either may be NULL).
+ * spanqr_grad_clip writes out = in * min(1, max_norm / (norm + 1e-6)), the product in fp32 and rounded to out_type
+ *   (in_type, or SPANQR_F32); out[i] may equal in[i] when the types are equal (in place; a coefficient of one then
+ *   leaves the tensor untouched), any other overlap returns SPANQR_ERR_OVERLAP.  max_norm >= 0, infinity included.
+ *   sumsq: NULL, or a device pointer to the sum of squares to use instead of this list's own (summed over several
+ *   GPUs, say).  *norm (device, or NULL) receives the norm (infinity above fp32's largest
+ *   value; the coefficient comes from the fp64 norm).  A norm of infinity in fp64 gives the coefficient 0 and a NaN norm
+ *   makes every output NaN.
+ * The workspace (spanqr_grad_workspace_bytes(count)) needs no initialisation.
+ */
+int spanqr_grad_workspace_bytes(int count, size_t* bytes);
+int spanqr_grad_norm(const void* const* in, const int* in_type, const long long* n, int count, double* sumsq, float* norm,
+                     void* ws, size_t ws_bytes, spanqr_stream_t stream);
+int spanqr_grad_clip(const void* const* in, const int* in_type, void* const* out, const int* out_type, const long long* n,
+                     int count, double max_norm, const double* sumsq, float* norm, void* ws, size_t ws_bytes,
+                     spanqr_stream_t stream);
 
 #ifdef __cplusplus
 }

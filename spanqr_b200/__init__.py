@@ -3,14 +3,16 @@
     from spanqr_b200 import orth, orth_batched
     Q = orth(X)                  # X: fp32 CUDA [K, r] -> Q, Q^T Q = I, span(Q) = span(X)
     Qs = orth_batched([X1, X2])  # many layers at once; across GPUs under torch.distributed
+    grads, n = clip_grads(grads, 1.0)   # the list's global norm, and the list scaled to it (grad_norm: the norm alone)
 
 The compute runs in libspanqr.so (CUDA kernels behind the C ABI of include/spanqr.h); this package only binds it.
 """
 from .core import orth, zdust, workspace, TB, MAX_R, DUST_SEED
 from .batched import orth_batched, partition
+from .grads import grad_norm, clip_grads
 from ._lib import SpanqrError, workspace_bytes
 
-__all__ = ["orth", "orth_batched", "partition", "zdust", "workspace", "workspace_bytes", "SpanqrError",
+__all__ = ["orth", "orth_batched", "grad_norm", "clip_grads", "partition", "zdust", "workspace", "workspace_bytes", "SpanqrError",
            "register_qrbench", "TB", "MAX_R", "DUST_SEED"]
 
 

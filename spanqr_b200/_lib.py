@@ -9,6 +9,7 @@ LIB_PATH = _DIR / "libspanqr.so"
 
 # every entry point include/spanqr.h declares, with its argument types
 _P, _I, _LL, _F, _SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_size_t
+_D = ctypes.c_double
 SIGNATURES = {
     "spanqr_version": (_I, []),
     "spanqr_strerror": (ctypes.c_char_p, [_I]),
@@ -42,6 +43,9 @@ SIGNATURES = {
     "spanqr_peer_slab_close": (_I, [_P]),
     "spanqr_peer_slab_free": (_I, [_P]),
     "spanqr_peer_copy": (_I, [_P, _P, _SZ, _P]),
+    "spanqr_grad_workspace_bytes": (_I, [_I, ctypes.POINTER(_SZ)]),
+    "spanqr_grad_norm": (_I, [_P, _P, _P, _I, _P, _P, _P, _SZ, _P]),
+    "spanqr_grad_clip": (_I, [_P, _P, _P, _P, _P, _I, _D, _P, _P, _P, _SZ, _P]),
 }
 
 _lib = None

@@ -3,10 +3,13 @@
 // orth(X) (candidates/kcholqr.py:92-112, kcholqr_f with eps 5e-7, alpha 1e-7, tau 1e-8, ns 2) as a stream-ordered
 // sequence of kernels; no host synchronisation, no device allocation.  Between passes Y lives in Q (the row-block
 // kernels run in place), so the workspace holds only r x r matrices and the Gram partials.
+#include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <vector>
 
 #include "../../include/spanqr.h"
@@ -28,9 +31,11 @@ int cuda_fail(cudaError_t e) {
 }
 
 // ---- optional per-kernel timing (spanqr_timing_*) ----
-enum Kind { K_SETUP = 0, K_ABSMAX, K_GRAM, K_REDUCE, K_CHOL, K_TRSM_W, K_TRSM, K_NS, K_GRAM_ACC, K_COPY, K_BAND, K_PROJ, K_COUNT };
+enum Kind { K_SETUP = 0, K_ABSMAX, K_GRAM, K_REDUCE, K_CHOL, K_TRSM_W, K_TRSM, K_NS, K_GRAM_ACC, K_COPY, K_BAND, K_PROJ, K_GRAD_SUMSQ, K_GRAD_SCALE,
+            K_COUNT };
 const char* const KIND_NAMES[K_COUNT] = {"k_setup", "k_absmax", "k_gram_tc", "k_gram_reduce", "k_chol", "k_trsm_w", "k_trsm",
-                                         "k_ns_update", "k_gram_tc_acc", "k_scale_copy", "k_band_image", "k_project"};
+                                         "k_ns_update", "k_gram_tc_acc", "k_scale_copy", "k_band_image", "k_project",
+                                         "k_grad_sumsq", "k_grad_scale"};
 struct TimedLaunch {
     int kind;
     cudaEvent_t a, b;
@@ -214,6 +219,7 @@ const char* spanqr_strerror(int code) {
         case SPANQR_ERR_WORKSPACE: return "workspace too small or not 256-byte aligned";
         case SPANQR_ERR_CUDA: return "CUDA error";
         case SPANQR_ERR_DEVICE: return "device reported a failure";
+        case SPANQR_ERR_OVERLAP: return "an output overlaps another tensor of the call";
         case SPANQR_ERR_TOO_LARGE: return "shape needs more scratch than the no-allocation entry point's fixed 16 MiB array";
         default: return "unknown status";
     }
@@ -844,6 +850,126 @@ int spanqr_read_status(const void* ws, spanqr_stream_t stream, int* device_statu
     if (e != cudaSuccess) return cuda_fail(e);
     *device_status = h;
     return h ? SPANQR_ERR_DEVICE : SPANQR_OK;
+}
+
+}  // extern "C"
+
+// ---- gradient lists: global norm and clipping (no reference counterpart) ----
+namespace {
+int type_bytes(int t) { return t == SPANQR_F32 ? 4 : (t == SPANQR_F16 || t == SPANQR_BF16) ? 2 : 0; }
+
+// the non-empty tensors of a list; out and out_type null for the norm alone
+int grad_entries(const void* const* in, const int* in_type, void* const* out, const int* out_type, const long long* n,
+                 int count, std::vector<GradEntry>& es) {
+    if (count < 0 || (count > 0 && (!in || !in_type || !n))) return SPANQR_ERR_ARG;
+    es.reserve(count);
+    for (int i = 0; i < count; ++i) {
+        GradEntry e{in[i], out ? out[i] : nullptr, n[i], in_type[i], out ? out_type[i] : in_type[i]};
+        const int is = type_bytes(e.in_type), os = type_bytes(e.out_type);
+        if (n[i] < 0 || !is || !os || (e.out_type != e.in_type && e.out_type != SPANQR_F32)) return SPANQR_ERR_ARG;
+        if (n[i] == 0) continue;
+        if (!e.in || reinterpret_cast<uintptr_t>(e.in) % is) return SPANQR_ERR_ARG;
+        if (out && (!e.out || reinterpret_cast<uintptr_t>(e.out) % os)) return SPANQR_ERR_ARG;
+        es.push_back(e);
+    }
+    return SPANQR_OK;
+}
+
+// An output may be its own input (same address and type); any other overlap of an output with an input or another
+// output would be a race.
+int grad_overlap(const std::vector<GradEntry>& es) {
+    struct Span {
+        uintptr_t a, b;
+        bool out;
+    };
+    std::vector<Span> v;
+    v.reserve(2 * es.size());
+    for (const GradEntry& e : es) {
+        const uintptr_t i = reinterpret_cast<uintptr_t>(e.in), o = reinterpret_cast<uintptr_t>(e.out);
+        const bool same = i == o && e.in_type == e.out_type;
+        if (!same) v.push_back({i, i + (uintptr_t)e.n * type_bytes(e.in_type), false});
+        v.push_back({o, o + (uintptr_t)e.n * type_bytes(e.out_type), true});
+    }
+    std::sort(v.begin(), v.end(), [](const Span& x, const Span& y) { return x.a < y.a; });
+    uintptr_t end_in = 0, end_out = 0;   // furthest ends of the inputs and outputs that begin at or before this span
+    for (const Span& s : v) {
+        if (s.a < end_out || (s.out && s.a < end_in)) return SPANQR_ERR_OVERLAP;
+        uintptr_t& end = s.out ? end_out : end_in;
+        end = std::max(end, s.b);
+    }
+    return SPANQR_OK;
+}
+
+size_t grad_slots(int count, int nsm) { return (size_t)grad_launches(count) * GRAD_CTAS_PER_SM * nsm; }
+
+constexpr int MAX_SMS = 256;   // the workspace is sized without asking the device
+
+int check_grad_ws(const void* ws, size_t ws_bytes, int count) {
+    if (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0) return SPANQR_ERR_WORKSPACE;
+    return ws_bytes < grad_slots(count, MAX_SMS) * sizeof(double) ? SPANQR_ERR_WORKSPACE : SPANQR_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int spanqr_grad_workspace_bytes(int count, size_t* bytes) {
+    if (!bytes || count < 0) return SPANQR_ERR_ARG;
+    *bytes = std::max<size_t>(256, grad_slots(count, MAX_SMS) * sizeof(double));
+    return SPANQR_OK;
+}
+
+int spanqr_grad_norm(const void* const* in, const int* in_type, const long long* n, int count, double* sumsq, float* norm,
+                     void* ws, size_t ws_bytes, spanqr_stream_t stream) try {
+    std::vector<GradEntry> es;
+    int rc = grad_entries(in, in_type, nullptr, nullptr, n, count, es);
+    if (rc) return rc;
+    if ((!sumsq && !norm) || reinterpret_cast<uintptr_t>(sumsq) % 8 || reinterpret_cast<uintptr_t>(norm) % 4)
+        return SPANQR_ERR_ARG;
+    if ((rc = check_grad_ws(ws, ws_bytes, count))) return rc;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    double* part = static_cast<double*>(ws);
+    int nparts = 0;
+    cudaError_t e = cudaSuccess;
+    if (!es.empty())
+        e = timed(K_GRAD_SUMSQ, st, [&] { return launch_grad_sumsq(es.data(), (int)es.size(), part, &nparts, st); },
+                  grad_launches((int)es.size()));
+    if (e == cudaSuccess)
+        e = timed(K_GRAD_SUMSQ, st, [&] { return launch_grad_finish(part, nparts, sumsq, norm, st); });
+    return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
+} catch (const std::bad_alloc&) {
+    return SPANQR_ERR_ARG;
+}
+
+int spanqr_grad_clip(const void* const* in, const int* in_type, void* const* out, const int* out_type, const long long* n,
+                     int count, double max_norm, const double* sumsq, float* norm, void* ws, size_t ws_bytes,
+                     spanqr_stream_t stream) try {
+    std::vector<GradEntry> es;
+    if (count > 0 && (!out || !out_type)) return SPANQR_ERR_ARG;
+    int rc = grad_entries(in, in_type, out, out_type, n, count, es);
+    if (rc) return rc;
+    if (!(max_norm >= 0.0) || reinterpret_cast<uintptr_t>(sumsq) % 8 || reinterpret_cast<uintptr_t>(norm) % 4)
+        return SPANQR_ERR_ARG;
+    if ((rc = grad_overlap(es))) return rc;
+    if ((rc = check_grad_ws(ws, ws_bytes, count))) return rc;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    double* part = static_cast<double*>(ws);
+    int nparts = 0;
+    const int launches = grad_launches((int)es.size());
+    cudaError_t e = cudaSuccess;
+    if (!sumsq && !es.empty())
+        e = timed(K_GRAD_SUMSQ, st, [&] { return launch_grad_sumsq(es.data(), (int)es.size(), part, &nparts, st); },
+                  launches);
+    const double* sums = sumsq ? sumsq : part;
+    if (sumsq) nparts = 1;
+    if (e == cudaSuccess && es.empty()) {
+        if (norm) e = timed(K_GRAD_SUMSQ, st, [&] { return launch_grad_finish(sums, nparts, nullptr, norm, st); });
+    } else if (e == cudaSuccess) {
+        e = timed(K_GRAD_SCALE, st,
+                  [&] { return launch_grad_scale(es.data(), (int)es.size(), sums, nparts, max_norm, norm, st); }, launches);
+    }
+    return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
+} catch (const std::bad_alloc&) {
+    return SPANQR_ERR_ARG;
 }
 
 }  // extern "C"

@@ -145,6 +145,22 @@ cudaError_t launch_project(PtrArg p, int K, int n, long long ldq, int j, const c
 cudaError_t launch_scale_copy(const float* X, long long ldx, float* Q, long long ldq, int K, int w,
                               const uint32_t* maxbits, cudaStream_t st);
 
-
+// ---- gradient lists: global norm and clipping ----
+enum DType : int { DT_F32 = 0, DT_F16 = 1, DT_BF16 = 2 };   // SPANQR_F32, SPANQR_F16, SPANQR_BF16
+struct GradEntry {
+    const void* in;
+    void* out;           // the scaled values (launch_grad_scale only)
+    long long n;         // elements
+    int in_type, out_type;
+};
+constexpr int GRAD_CTAS_PER_SM = 4;
+int grad_launches(int count);   // launches for a list of `count` tensors
+// CTA sums of squares into part[0 .. *nparts), at most grad_launches(count) * GRAD_CTAS_PER_SM per SM
+cudaError_t launch_grad_sumsq(const GradEntry* e, int count, double* part, int* nparts, cudaStream_t st);
+// *sumsq = the slots' sum, *norm = its square root (either may be null)
+cudaError_t launch_grad_finish(const double* part, int nparts, double* sumsq, float* norm, cudaStream_t st);
+// out = in * min(1, max_norm / (n + 1e-6)) with n the root of the slots' sum, also to *norm when not null
+cudaError_t launch_grad_scale(const GradEntry* e, int count, const double* part, int nparts, double max_norm, float* norm,
+                              cudaStream_t st);
 
 }  // namespace spq

@@ -1,0 +1,266 @@
+"""grad_norm and clip_grads on the GPU against the formula in fp64.
+
+Tolerances.  The kernel sums a vector of at most 16 squares in fp32 (relative error below 16 * 2^-24, all terms
+positive) and the rest in fp64, so the norm is within 8 * 2^-24 of the exact one before its rounding to fp32 (2^-24):
+NORM_TOL = 9 * 2^-24.  A scaled value carries the norm's 8, the coefficient's rounding, the product's rounding (1 each)
+and, in 16 bits, the rounding of the result: half a step of the type."""
+import pytest
+import torch
+
+from spanqr_b200 import clip_grads, grad_norm, orth_batched
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+NORM_TOL = 9 * U
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def norm64(ts):
+    # scaled so that squares of fp32's largest values stay inside fp64 comfortably (they do: 2^256)
+    return float(sum((t.double().cpu() ** 2).sum() for t in ts) ** 0.5)
+
+
+def coef64(n, max_norm):
+    return min(1.0, max_norm / (n + 1e-6))
+
+
+def check_norm(got, want):
+    assert got.dtype == F32 and got.dim() == 0
+    assert abs(got.item() - want) <= NORM_TOL * want, (got.item(), want)
+
+
+def check_clipped(got, x, coef):
+    want = x.double().cpu() * coef
+    half = torch.finfo(got.dtype).eps / 2 if got.dtype != F32 else 0.0
+    tiny = torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps / 2    # half a subnormal step
+    err = (got.double().cpu() - want).abs()
+    tol = want.abs() * (half * (1 + 10 * U) + 10 * U) + tiny * 1.01
+    assert got.shape == x.shape and bool((err <= tol).all()), float((err - tol).max())
+
+
+def rand(shape, dtype=F32, seed=0, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype).cuda()
+
+
+def mixed(seed=0):
+    """odd sizes around the vector (8 or 16 elements) and chunk (8192 or 16384) borders, empty tensors and scalars"""
+    sizes = [(), (1,), (0,), (7,), (8,), (9,), (15, 3), (16,), (17,), (33, 5), (8191,), (8192,), (8193,), (16385,), (0, 4),
+             (3, 16384), (129, 257)]
+    return [rand(s, (F32, BF16, F16)[i % 3], seed + i, 10.0 ** (i % 5 - 3)) for i, s in enumerate(sizes)]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n", [1, 7, 8, 31, 8192, 8193, 100003, 3 << 20])
+def test_norm_and_clip_of_one_tensor(dtype, n):
+    x = rand((n,), dtype, n)
+    want = norm64([x])
+    check_norm(grad_norm([x]), want)
+    x0 = x.clone()
+    (y,), norm = clip_grads([x], 0.5)
+    assert y.dtype == dtype and torch.equal(x, x0)
+    check_norm(norm, want)
+    check_clipped(y, x, coef64(want, 0.5))
+
+
+def test_mixed_list_new_tensors_in_place_and_fp32_out():
+    ts = mixed()
+    want = norm64(ts)
+    check_norm(grad_norm(ts), want)
+    c = coef64(want, 1.0)
+    ys, norm = clip_grads(ts, 1.0)
+    check_norm(norm, want)
+    for y, x in zip(ys, ts):
+        assert y.dtype == x.dtype
+        check_clipped(y, x, c)
+    wide = [torch.full(t.shape, float("nan"), device="cuda") for t in ts]
+    res, _ = clip_grads(ts, 1.0, out=wide)
+    for y, x, o in zip(res, ts, wide):
+        assert y is o
+        check_clipped(y, x, c)
+    inplace = [t.clone() for t in ts]
+    res, _ = clip_grads(inplace, 1.0, out=inplace)
+    for a, b in zip(res, ys):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("count", [63, 64, 65, 900, 901, 2003])
+def test_long_lists(count):
+    big = rand((count * 37,), F32, count)
+    ts = [big[37 * i:37 * i + 1 + i % 37] for i in range(count)]
+    want = norm64(ts)
+    check_norm(grad_norm(ts), want)
+    ys, norm = clip_grads(ts, 0.1)
+    check_norm(norm, want)
+    c = coef64(want, 0.1)
+    check_clipped(torch.cat(ys), torch.cat(ts), c)
+
+
+@pytest.mark.parametrize("dtype,off_in,off_out", [(F32, 1, 0), (F32, 3, 5), (BF16, 1, 0), (BF16, 0, 3), (F16, 7, 7)])
+def test_misaligned_views(dtype, off_in, off_out):
+    n = 50021
+    src = rand((n + 64,), dtype, 5)
+    x = src[off_in:off_in + n]
+    guard = torch.full((n + 64,), 7.0, dtype=dtype, device="cuda")
+    o = guard[off_out:off_out + n]
+    want = norm64([x])
+    check_norm(grad_norm([x]), want)
+    clip_grads([x], 0.25, out=[o])
+    check_clipped(o, x, coef64(want, 0.25))
+    assert bool((guard[:off_out] == 7).all()) and bool((guard[off_out + n:] == 7).all())
+
+
+@pytest.mark.parametrize("scale", [1e-44, 1e-38, 1e-30, 1e-20, 1e-12, 1e15, 1e19, 1e30, 3e37])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_squares_outside_fp32(scale, dtype):
+    x = rand((40001,), dtype, 3, scale)
+    for ts in ([x], [x, rand((513,), dtype, 4, 1.0)]):
+        want = norm64(ts)
+        n = grad_norm(ts)
+        if want > torch.finfo(F32).max:      # 200 * 3e37 = 6e39: the norm's nearest fp32 value is infinity
+            assert n.item() == float("inf")
+        else:                                # a norm below fp32's normal range is rounded to a subnormal step
+            assert abs(n.item() - want) <= NORM_TOL * want + 2.0 ** -150, (n.item(), want)
+        ys, _ = clip_grads(ts, 1.0)          # the coefficient comes from the fp64 norm
+        for y, t in zip(ys, ts):
+            check_clipped(y, t, coef64(want, 1.0))
+
+
+def test_norm_of_many_equal_values_does_not_drift():
+    x = torch.full((1 << 26,), 0.1, device="cuda")
+    want = (float(x[0].item()) ** 2 * x.numel()) ** 0.5
+    check_norm(grad_norm([x]), want)
+
+
+def test_zero_empty_and_unclipped():
+    z = [torch.zeros(1000, device="cuda"), torch.zeros(0, device="cuda")]
+    assert grad_norm(z).item() == 0.0 and grad_norm([]).item() == 0.0
+    ys, n = clip_grads(z, 1.0)
+    assert n.item() == 0.0 and bool((ys[0] == 0).all()) and ys[1].numel() == 0
+    assert clip_grads([], 1.0)[1].item() == 0.0
+    x = rand((3000,), BF16, 1)
+    for m in (1e6, float("inf")):
+        (y,), _ = clip_grads([x], m)
+        assert torch.equal(x, y)
+        w = x.clone()
+        clip_grads([w], m, out=[w])
+        assert torch.equal(x, w)
+    (y,), _ = clip_grads([x], 0.0)
+    assert bool((y == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_infinite_and_nan_gradients(dtype):
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        x = rand((20000,), dtype, 2)
+        x[12345] = bad
+        n = grad_norm([x]).item()
+        (y,), norm = clip_grads([x], 1.0)
+        if bad != bad:
+            assert n != n and bool(y.isnan().all())
+        else:
+            assert n == float("inf") and bool(y[12345].isnan()) and int((y == 0).sum()) == 19999
+
+
+def test_strides():
+    base = rand((300, 200), F32, 8)
+    col, tr, ex = base[:, 3:50], base.t(), base[:1].expand(9, 200)
+    for t in (col, tr, ex):
+        want = norm64([t])
+        check_norm(grad_norm([t]), want)
+        (y,), _ = clip_grads([t], 1.0)
+        assert y.is_contiguous()
+        check_clipped(y, t, coef64(want, 1.0))
+    want = coef64(norm64([base]), 1.0) * base.double()
+    clip_grads([tr], 1.0, out=[tr])                      # dense: in place through its transposed view
+    assert float((base.double() - want).abs().max()) <= 10 * U * float(want.abs().max())
+    with pytest.raises(ValueError, match="contiguous"):
+        clip_grads([col], 1.0, out=[col])
+    with pytest.raises(ValueError, match="contiguous"):
+        clip_grads([rand((300, 47))], 1.0, out=[col])
+
+
+def test_refusals():
+    x, y = rand((64,)), rand((64,))
+    with pytest.raises(ValueError, match="overlap"):
+        clip_grads([x, x], 1.0, out=[x, x])
+    with pytest.raises(ValueError, match="overlap"):
+        clip_grads([x[:32], x[16:48]], 1.0, out=[x[:32], x[16:48]])
+    with pytest.raises(ValueError, match="overlap"):
+        clip_grads([x, y], 1.0, out=[y, x])
+    with pytest.raises(ValueError, match="2 tensors"):
+        clip_grads([x, y], 1.0, out=[x])
+    with pytest.raises(ValueError, match="shape"):
+        clip_grads([x], 1.0, out=[y.view(8, 8)])
+    with pytest.raises(TypeError, match="fp32"):
+        clip_grads([x], 1.0, out=[y.half()])
+    n = grad_norm([x, x])                                # listed twice: counts twice
+    check_norm(n, norm64([x, x]))
+
+
+def test_deterministic_and_version_counter():
+    ts = mixed(100)
+    a, na = clip_grads(ts, 1.0)
+    for _ in range(3):
+        b, nb = clip_grads(ts, 1.0)
+        assert torch.equal(na, nb) and all(torch.equal(p, q) for p, q in zip(a, b))
+    v = ts[3]._version
+    clip_grads(ts, 1.0, out=ts)
+    assert ts[3]._version > v
+
+
+def test_streams_and_captured_graphs():
+    """calls on two streams, and two graphs captured one after the other and replayed at the same time, keep apart"""
+    a, b = rand((5 << 20,), F32, 1), rand((5 << 20,), F32, 2, 3.0)
+    oa, ob = torch.empty_like(a), torch.empty_like(b)
+    wa, wb = norm64([a]), norm64([b])
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g1, stream=s1):
+        _, n1 = clip_grads([a], 1.0, out=[oa])
+    with torch.cuda.graph(g2, stream=s1):
+        _, n2 = clip_grads([b], 2.0, out=[ob])
+    torch.cuda.synchronize()
+    for _ in range(5):
+        oa.zero_(), ob.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(s1):
+            g1.replay()
+        with torch.cuda.stream(s2):
+            g2.replay()
+            n3 = grad_norm([a])
+        torch.cuda.synchronize()
+        check_norm(n1, wa), check_norm(n2, wb), check_norm(n3, wa)
+        check_clipped(oa, a, coef64(wa, 1.0)), check_clipped(ob, b, coef64(wb, 2.0))
+    a.mul_(2.0)                                          # a replay reads the tensors' present values
+    g1.replay()
+    torch.cuda.synchronize()
+    check_norm(n1, 2 * wa)
+
+
+def test_under_a_process_group():
+    import torch.distributed as dist
+    dist.init_process_group("nccl", init_method="tcp://127.0.0.1:29517", rank=0, world_size=1)
+    try:
+        ts = mixed(7)
+        want = norm64(ts)
+        check_norm(grad_norm(ts, group=dist.group.WORLD), want)
+        ys, n = clip_grads(ts, 1.0, group=dist.group.WORLD)
+        check_norm(n, want)
+        for y, x in zip(ys, ts):
+            check_clipped(y, x, coef64(want, 1.0))
+        assert grad_norm([], group=dist.group.WORLD).item() == 0.0
+    finally:
+        dist.destroy_process_group()
+
+
+def test_clipped_gradients_go_to_orth():
+    """bf16 layer gradients -> clipped fp32 -> orth_batched: the clipped step's basis is the gradients' own"""
+    gs = [rand((768, 128), BF16, 20 + i, 4.0) for i in range(3)]
+    wide = [torch.empty(g.shape, device="cuda") for g in gs]
+    fs, _ = clip_grads(gs, 1.0, out=wide)
+    for q, g in zip(orth_batched(fs), gs):
+        q, g = q.double(), g.double()
+        assert float((q.t() @ q - torch.eye(128, device="cuda")).abs().max()) <= 3e-7
+        assert float((g - q @ (q.t() @ g)).norm() / g.norm()) <= 1e-5

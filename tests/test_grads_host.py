@@ -1,0 +1,101 @@
+"""grad_norm and clip_grads without a GPU: the Python layer's refusals and the C ABI's argument checks, which come before
+any device work."""
+import ctypes
+from array import array
+
+import pytest
+import torch
+
+from spanqr_b200 import _lib, clip_grads, grad_norm
+from spanqr_b200.grads import _dense
+
+OK, ARG, WS, OVERLAP = 0, 2, 3, 7
+BASE = 1 << 40          # device addresses that no call below dereferences: each fails its checks first
+
+
+def test_refusals():
+    cpu = torch.zeros(4)
+    with pytest.raises(TypeError, match="list of tensors"):
+        grad_norm(cpu)
+    with pytest.raises(TypeError, match="tensors only"):
+        grad_norm([1.0])
+    with pytest.raises(TypeError, match="CUDA"):
+        grad_norm([cpu])
+    with pytest.raises(TypeError, match="float64"):
+        grad_norm([cpu.double()])
+    with pytest.raises(TypeError, match="CUDA"):
+        clip_grads([cpu], 1.0)
+    for bad in (-1.0, float("nan")):
+        with pytest.raises(ValueError, match="max_norm"):
+            clip_grads([], bad)
+
+
+@pytest.mark.parametrize("make,want", [
+    (lambda: torch.zeros(4, 6), True), (lambda: torch.zeros(4, 6).t(), True), (lambda: torch.zeros(4, 6)[:, :3], False),
+    (lambda: torch.zeros(4, 1, 6).permute(2, 1, 0), True), (lambda: torch.zeros(4, 1).expand(4, 3), False),
+    (lambda: torch.zeros(4, 6)[::2], False), (lambda: torch.zeros(()), True), (lambda: torch.zeros(7)[2:3], True)])
+def test_dense(make, want):
+    assert _dense(make()) is want
+
+
+def test_workspace_bytes():
+    n = ctypes.c_size_t(0)
+    L = _lib.lib()
+    assert L.spanqr_grad_workspace_bytes(-1, ctypes.byref(n)) == ARG
+    assert L.spanqr_grad_workspace_bytes(1, None) == ARG
+    last = 0
+    for count in (0, 1, 64, 65, 900, 901, 5000):
+        assert L.spanqr_grad_workspace_bytes(count, ctypes.byref(n)) == OK
+        assert n.value >= max(last, 256)
+        last = n.value
+
+
+def _at(a):
+    return a.buffer_info()[0]
+
+
+def _clip(ins, outs, kinds=None, okinds=None, sizes=None, max_norm=1.0, ws=BASE, ws_bytes=1 << 30, norm=BASE):
+    n = len(ins)
+    pi, po = array("Q", ins), array("Q", outs)
+    ki = array("i", kinds or [0] * n)
+    ko = array("i", okinds or list(ki))
+    sz = array("q", sizes or [64] * n)
+    return _lib.lib().spanqr_grad_clip(_at(pi), _at(ki), _at(po), _at(ko), _at(sz), n, max_norm, None, norm, ws, ws_bytes,
+                                       None)
+
+
+def test_clip_argument_checks_before_any_device_work():
+    a, b, c = BASE, BASE + 4096, BASE + 8192
+    assert _clip([a], [a], kinds=[3]) == ARG                       # no such type
+    assert _clip([a], [b], kinds=[0], okinds=[1]) == ARG           # fp32 to fp16
+    assert _clip([a], [b], kinds=[1], okinds=[2]) == ARG           # fp16 to bf16
+    assert _clip([a + 2], [b]) == ARG                              # fp32 off its alignment
+    assert _clip([a], [b + 1], kinds=[1]) == ARG
+    assert _clip([0], [b]) == ARG
+    assert _clip([a], [0]) == ARG
+    assert _clip([a], [b], sizes=[-1]) == ARG
+    assert _clip([a], [b], max_norm=-1.0) == ARG
+    assert _clip([a], [b], max_norm=float("nan")) == ARG
+    assert _clip([a], [b], norm=BASE + 2) == ARG
+    assert _clip([a], [b], ws=BASE + 16) == WS
+    assert _clip([a], [b], ws=None) == WS
+    assert _clip([a], [b], ws_bytes=256) == WS
+    # overlaps: 64 fp32 elements are 256 bytes
+    assert _clip([a, a], [a, a]) == OVERLAP                        # one tensor twice, in place
+    assert _clip([a, c], [b, b]) == OVERLAP                        # two inputs to one output
+    assert _clip([a], [a + 128]) == OVERLAP                        # shifted against its own input
+    assert _clip([a, b], [b, c]) == OVERLAP                        # an output on another input
+    assert _clip([a, b], [c, a]) == OVERLAP
+    assert _clip([a], [a], kinds=[1], okinds=[0]) == OVERLAP       # fp16 widened in place
+    # overlapping inputs alone are no race: the call gets as far as its workspace
+    assert _clip([a, a + 128], [b, c], ws=None) == WS
+
+
+def test_norm_argument_checks_before_any_device_work():
+    L = _lib.lib()
+    p, k, n = array("Q", [BASE]), array("i", [0]), array("q", [64])
+    assert L.spanqr_grad_norm(_at(p), _at(k), _at(n), 1, None, None, BASE, 1 << 30, None) == ARG     # no result wanted
+    assert L.spanqr_grad_norm(_at(p), _at(k), _at(n), -1, None, BASE, BASE, 1 << 30, None) == ARG
+    assert L.spanqr_grad_norm(None, _at(k), _at(n), 1, None, BASE, BASE, 1 << 30, None) == ARG
+    assert L.spanqr_grad_norm(_at(p), _at(k), _at(n), 1, BASE + 4, BASE, BASE, 1 << 30, None) == ARG  # fp64 off 8 bytes
+    assert L.spanqr_grad_norm(_at(p), _at(k), _at(n), 1, None, BASE, BASE, 64, None) == WS
