@@ -32,10 +32,10 @@ int cuda_fail(cudaError_t e) {
 
 // ---- optional per-kernel timing (spanqr_timing_*) ----
 enum Kind { K_SETUP = 0, K_ABSMAX, K_GRAM, K_REDUCE, K_CHOL, K_TRSM_W, K_TRSM, K_NS, K_GRAM_ACC, K_COPY, K_BAND, K_PROJ, K_GRAD_SUMSQ, K_GRAD_SCALE,
-            K_COUNT };
+            K_MM, K_MM_WGRAD, K_COUNT };
 const char* const KIND_NAMES[K_COUNT] = {"k_setup", "k_absmax", "k_gram_tc", "k_gram_reduce", "k_chol", "k_trsm_w", "k_trsm",
                                          "k_ns_update", "k_gram_tc_acc", "k_scale_copy", "k_band_image", "k_project",
-                                         "k_grad_sumsq", "k_grad_scale"};
+                                         "k_grad_sumsq", "k_grad_scale", "k_mm", "k_mm_wgrad"};
 struct TimedLaunch {
     int kind;
     cudaEvent_t a, b;
@@ -970,6 +970,91 @@ int spanqr_grad_clip(const void* const* in, const int* in_type, void* const* out
     return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
 } catch (const std::bad_alloc&) {
     return SPANQR_ERR_ARG;
+}
+
+}  // extern "C"
+
+// ---- products grouped by expert (no reference counterpart) ----
+namespace {
+// the kernels report a bounded wait that ran out here: a word of the library's device image, so that no call has to
+// bring or clear a status word of its own
+__device__ int g_mm_status;
+
+int* mm_status() {
+    void* p = nullptr;
+    return cudaGetSymbolAddress(&p, g_mm_status) == cudaSuccess ? static_cast<int*>(p) : nullptr;
+}
+
+constexpr int MM_WIDE = 64;   // rows per expert on average above which a pair of SMs works on a tile
+constexpr int MM_MAX_E = 1024, MM_MAX_T = 1 << 30, MM_MAX_DIM = 1 << 24;
+
+int check_mm(int type, int T, int E, int N, int K, const int* offsets) {
+    if (T < 0 || T > MM_MAX_T || E < 1 || E > MM_MAX_E || N < 1 || N > MM_MAX_DIM || K < 1 || K > MM_MAX_DIM)
+        return SPANQR_ERR_SHAPE;
+    if ((type != SPANQR_F16 && type != SPANQR_BF16) || !offsets || reinterpret_cast<uintptr_t>(offsets) % 4)
+        return SPANQR_ERR_ARG;
+    return SPANQR_OK;
+}
+// a row-major 16-bit operand that TMA can read: 16-byte aligned rows that do not overlap
+bool mm_rows(const void* p, long long ld, long long cols) { return p && a16(p) && ld >= cols && ld % 8 == 0 && ld < (1LL << 38); }
+}  // namespace
+
+extern "C" {
+
+int spanqr_mm_grouped(const void* x, long long ldx, const void* w, long long ldw, long long stride_w, int w_transposed,
+                      const int* offsets, void* y, long long ldy, int type, int T, int E, int N, int K, int zero_tail,
+                      spanqr_stream_t stream) {
+    const int rc = check_mm(type, T, E, N, K, offsets);
+    if (rc) return rc;
+    if (T == 0) return SPANQR_OK;
+    const long long wcols = w_transposed ? N : K, wrows = w_transposed ? K : N;
+    if (!mm_rows(x, ldx, K) || !mm_rows(w, ldw, wcols) || !y || reinterpret_cast<uintptr_t>(y) % 2 || ldy < N)
+        return SPANQR_ERR_ARG;
+    if (stride_w % 8 || (E > 1 && stride_w < (wrows - 1) * ldw + wcols) || stride_w >= (1LL << 38)) return SPANQR_ERR_ARG;
+    const MmOperand ox{x, K, T, ldx, 0, 0, false};
+    const MmOperand ow{w, wcols, wrows, ldw, E, E > 1 ? stride_w : wrows * ldw, w_transposed != 0};
+    MmArgs a{offsets, E, T, N, K, static_cast<uint16_t*>(y), ldy, (N + 127) / 128, type == SPANQR_BF16, zero_tail != 0,
+             mm_status()};
+    if (!a.status) return cuda_fail(cudaGetLastError());
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const cudaError_t e = timed(K_MM, st, [&] {
+        return T > MM_WIDE * (long long)E ? launch_mm_wide(ox, ow, a, st)
+                                          : launch_mm_narrow(ox, ow, a, T <= 16LL * E ? 16 : T <= 32LL * E ? 32 : 64, st);
+    });
+    return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
+}
+
+int spanqr_mm_grouped_wgrad(const void* dy, long long lddy, const void* x, long long ldx, const int* offsets, void* dw,
+                            int type, int out_type, int T, int E, int N, int K, spanqr_stream_t stream) {
+    const int rc = check_mm(type, T, E, N, K, offsets);
+    if (rc) return rc;
+    const int os = type_bytes(out_type);
+    if ((out_type != type && out_type != SPANQR_F32) || !dw || reinterpret_cast<uintptr_t>(dw) % os) return SPANQR_ERR_ARG;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (T == 0) {
+        const cudaError_t e = cudaMemsetAsync(dw, 0, (size_t)E * N * K * os, st);
+        return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
+    }
+    if (!mm_rows(dy, lddy, N) || !mm_rows(x, ldx, K)) return SPANQR_ERR_ARG;
+    const MmOperand ody{dy, N, T, lddy, 0, 0, true}, ox{x, K, T, ldx, 0, 0, true};
+    const MmWgradArgs a{offsets, E, T, N, K, dw, type == SPANQR_BF16, out_type == SPANQR_F32, mm_status()};
+    if (!a.status) return cuda_fail(cudaGetLastError());
+    const cudaError_t e = timed(K_MM_WGRAD, st, [&] { return launch_mm_wgrad(ody, ox, a, st); });
+    return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
+}
+
+int spanqr_mm_read_status(spanqr_stream_t stream, int* device_status) {
+    if (!device_status) return SPANQR_ERR_ARG;
+    int* p = mm_status();
+    if (!p) return cuda_fail(cudaGetLastError());
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    int h = 0;
+    cudaError_t e = cudaMemcpyAsync(&h, p, sizeof(int), cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, sizeof(int), st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e != cudaSuccess) return cuda_fail(e);
+    *device_status = h;
+    return h ? SPANQR_ERR_DEVICE : SPANQR_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,496 @@
+// Products grouped by expert on pairs of SMs (no reference counterpart): the forward product for many rows per expert,
+// and the weight gradient.
+//
+//   k_mm_wide   y[t] = w[e(t)] x[t]           D = W X^T: 256 features x up to 256 of one expert's rows
+//   k_mm_wgrad  dw[e] = sum_t dy[t] x[t]^T    D = dy^T x: 256 features x up to 256 columns of x, over e's rows
+//
+// One tcgen05.mma.cta_group::2 works on both SMs of a pair (a cluster of two CTAs): each CTA holds the accumulators of
+// 128 of the 256 features, its own half of A and half of B, so a 64-element stage costs each SM 32 KB of shared memory
+// and of L2 traffic for 512 cycles of products; a 128 x 256 tile on one SM would need 48 KB.  Six stages in flight, two
+// accumulators of 256 TMEM columns: the epilogue of one tile overlaps the products of the next.  The grid is one pair
+// per two SMs, each pair taking tiles in turn; the pipeline runs on from tile to tile.
+//
+// Barriers.  full[s] (used in the first CTA of the pair, the leader, whose thread issues the products): both CTAs' copies
+// of stage s; empty[s] and tfull[b] (both CTAs): signalled by the products' commit to both; tempty[b] (leader): the
+// sixteen epilogue warps have read accumulator b.
+#include "mm.cuh"
+
+namespace spq {
+namespace {
+
+using namespace mm;
+
+constexpr int THREADS = 320;       // warps 0-7: epilogue (TMEM lanes 32 (w % 4) .., columns by w / 4), 8: copies, 9: products
+constexpr int STAGES = 6;
+constexpr int HALF = FT * BK * 2;  // one operand half: 128 x 64 elements, 16 KB
+constexpr int STAGE = 2 * HALF;
+constexpr int NT = 256;            // columns of a tile
+constexpr int BARS = STAGES * STAGE;
+constexpr int MAPS = BARS + 256;
+constexpr int FIXED = MAPS + 16 + 1024;
+constexpr int DRAIN = 4;           // wgrad: stages (of 64 rows) summed in TMEM before they are added in registers
+
+// ---- cta_group::2 forms ----
+__device__ __forceinline__ void mma2_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        :
+        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// arrive on `bar` of both CTAs when every product this thread issued before has completed
+__device__ __forceinline__ void commit2(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            tc::smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_alloc2(uint32_t* dst_smem, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(dst_smem)),
+                 "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc2(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// copies into this CTA's shared memory whose bytes count on a barrier of either CTA of the pair (`bar`: a cluster address)
+__device__ __forceinline__ void tma2_load_3d(uint32_t smem_dst, const void* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+        "[%1, {%2, %3, %4}], [%5];" ::"r"(smem_dst),
+        "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma2_load_2d(uint32_t smem_dst, const void* map, int c0, int c1, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+        "[%1, {%2, %3}], [%4];" ::"r"(smem_dst),
+        "l"(map), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// the pair's shared state, set up before any role begins
+struct Pair {
+    char* sm;
+    uint64_t *full, *empty, *tfull, *tempty;
+    volatile int* err;
+    int *start, *pre;
+    uint32_t tmem;
+    int rank;
+    uint32_t full0, tempty0;   // cluster addresses of the leader's barriers
+};
+
+__device__ __forceinline__ Pair set_up(char* dyn, const int* offsets, int E, int T, int rows_per_tile, int full_arrivals) {
+    Pair p;
+    p.sm = dyn + ((1024u - (tc::smem_u32(dyn) & 1023u)) & 1023u);
+    p.full = reinterpret_cast<uint64_t*>(p.sm + BARS);
+    p.empty = p.full + STAGES;
+    p.tfull = p.empty + STAGES;
+    p.tempty = p.tfull + 2;
+    uint32_t* const slot = reinterpret_cast<uint32_t*>(p.sm + MAPS);
+    p.err = reinterpret_cast<int*>(p.sm + MAPS + 4);
+    p.start = reinterpret_cast<int*>(p.sm + MAPS + 16);
+    p.pre = p.start + E + 1;
+    p.rank = (int)cluster_rank();
+    const int warp = threadIdx.x >> 5;
+    if (warp == 0) map_groups(offsets, E, T, rows_per_tile, p.start, p.pre);
+    if (warp == 9) tmem_alloc2(slot, 2 * NT);
+    if (threadIdx.x == 256) {
+        for (int s = 0; s < STAGES; ++s) {
+            tc::mbar_init(&p.full[s], full_arrivals);
+            tc::mbar_init(&p.empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            tc::mbar_init(&p.tfull[b], 1);
+            tc::mbar_init(&p.tempty[b], 16);
+        }
+        tc::mbar_init(p.tempty + 2, 1);   // wgrad: the copies of a ragged last stage
+        tc::mbar_fence_init();
+        *p.err = 0;
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    cluster_sync_all();
+    tc::fence_after_sync();
+    p.tmem = *slot;
+    p.full0 = mapa(tc::smem_u32(p.full), 0);
+    p.tempty0 = mapa(tc::smem_u32(p.tempty), 0);
+    return p;
+}
+
+// no CTA of the pair leaves while the other may still signal its barriers or read its operands
+__device__ __forceinline__ void tear_down(const Pair& p, int* status) {
+    __syncwarp();
+    tc::fence_before_sync();
+    cluster_sync_all();
+    if ((threadIdx.x >> 5) == 9) tmem_dealloc2(p.tmem, 2 * NT);
+    if (threadIdx.x == 0 && *p.err) atomicOr(status, MM_TIMEOUT);
+}
+
+// the wait for stage i to be free (true), or a limit that ran out
+__device__ __forceinline__ bool stage_free(const Pair& p, int i) {
+    if (i < STAGES) return true;
+    if (!*p.err && tc::mbar_wait(&p.empty[i % STAGES], (uint32_t)((i / STAGES - 1) & 1))) return true;
+    *p.err = 1;
+    return false;
+}
+// the end of the copies, after i stages: the products have released the last ones (so no signal is on its way to a
+// barrier of a CTA that is gone), or, after a limit ran out, the leader has seen both CTAs' copies arrive
+__device__ __forceinline__ void finish_copies(const Pair& p, int i) {
+    const bool failed = *p.err;
+    if (failed && p.rank != 0) return;
+    for (int j = max(0, i - STAGES); j < i; ++j)
+        if (!tc::mbar_wait(failed ? &p.full[j % STAGES] : &p.empty[j % STAGES], (uint32_t)((j / STAGES) & 1))) *p.err = 1;
+}
+
+__device__ __forceinline__ int up32(int n) { return (n + 31) & ~31; }
+
+template <bool W_MN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    k_mm_wide(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, const MmArgs a) {
+    extern __shared__ char dyn[];
+    const Pair p = set_up(dyn, a.offsets, a.E, a.T, NT, 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ntn = a.ntn, tiles = p.pre[a.E] * ntn, pairs = (int)gridDim.x / 2;
+    const int kb = (a.K + BK - 1) / BK;
+    struct Tile {
+        int e, n0, t0, t1, cols;   // cols: the tile's rows of x, up to a multiple of 32
+    };
+    auto tile_at = [&](int i) {
+        const int u = i / ntn;
+        Tile t;
+        t.n0 = (i - u * ntn) * 2 * FT;
+        t.e = group_of(p.pre, a.E, u);
+        t.t0 = p.start[t.e] + (u - p.pre[t.e]) * NT;
+        t.t1 = min(p.start[t.e + 1], t.t0 + NT);
+        t.cols = up32(t.t1 - t.t0);
+        return t;
+    };
+
+    if (warp == 8) {
+        if (lane == 0) {
+            prefetch_map(&tw);
+            prefetch_map(&tx);
+            int i = 0;
+            bool ok = true;
+            for (int t = (int)blockIdx.x / 2; ok && t < tiles; t += pairs) {
+                const Tile d = tile_at(t);
+                const int n = d.n0 + p.rank * FT, r = d.t0 + p.rank * (d.cols / 2);
+                for (int k = 0; k < kb; ++k, ++i) {
+                    if (!(ok = stage_free(p, i))) break;
+                    const int s = i % STAGES;
+                    const uint32_t as = tc::smem_u32(p.sm) + s * STAGE, bar = p.full0 + s * 8;
+                    if (p.rank == 0) tc::mbar_expect_tx(&p.full[s], 2 * STAGE);
+                    if (W_MN) {
+                        tma2_load_3d(as, &tw, n, k * BK, d.e, bar);
+                        tma2_load_3d(as + BOX_MN, &tw, n + 64, k * BK, d.e, bar);
+                    } else {
+                        tma2_load_3d(as, &tw, k * BK, n, d.e, bar);
+                    }
+                    tma2_load_2d(as + HALF, &tx, k * BK, r, bar);
+                }
+            }
+            finish_copies(p, i);
+        }
+    } else if (warp == 9) {
+        if (lane == 0 && p.rank == 0) {
+            int i = 0, j = 0;
+            for (int t = (int)blockIdx.x / 2; t < tiles && !*p.err; t += pairs, ++j) {
+                const Tile d = tile_at(t);
+                const int b = j & 1;
+                const uint32_t acc = p.tmem + b * NT, id = idesc_f16(2 * FT, d.cols, a.bf16, W_MN, false);
+                if (j >= 2 && !tc::mbar_wait(&p.tempty[b], (uint32_t)((j / 2 - 1) & 1))) *p.err = 1;
+                tc::fence_after_sync();
+                for (int k = 0; k < kb; ++k, ++i) {
+                    const int s = i % STAGES;
+                    if (*p.err || !tc::mbar_wait(&p.full[s], (uint32_t)((i / STAGES) & 1))) {
+                        *p.err = 1;
+                        break;
+                    }
+                    tc::fence_after_sync();
+                    const uint32_t as = tc::smem_u32(p.sm) + s * STAGE, bs = as + HALF;
+#pragma unroll
+                    for (int q = 0; q < BK / 16; ++q)
+                        mma2_f16(acc, sdesc<W_MN>(as + q * kstep<W_MN>()), sdesc<false>(bs + q * kstep<false>()), id,
+                                 k > 0 || q > 0);
+                    commit2(&p.empty[s]);
+                }
+                commit2(&p.tfull[b]);
+            }
+        }
+    } else {
+        // TMEM lane = feature, column = row of y: neighbouring lanes exchange values so that each stores two features of
+        // one row
+        const bool pairs32 = a.ldy % 2 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 3) == 0;
+        const int q = warp & 3, half = warp >> 2, odd = lane & 1;
+        if (a.zero_tail) {   // rows behind the last expert
+            for (long long t = p.start[a.E] + (long long)blockIdx.x; t < a.T; t += gridDim.x)
+                for (int n = threadIdx.x; n < a.N; n += 256) a.y[t * a.ldy + n] = 0;
+        }
+        int j = 0;
+        for (int t = (int)blockIdx.x / 2; t < tiles; t += pairs, ++j) {
+            const Tile d = tile_at(t);
+            const int b = j & 1;
+            const bool ok = !*p.err && tc::mbar_wait(&p.tfull[b], (uint32_t)((j / 2) & 1));
+            if (!__all_sync(~0u, ok)) {
+                *p.err = 1;
+                break;
+            }
+            tc::fence_after_sync();
+            const int n = d.n0 + p.rank * FT + q * 32 + lane;
+            for (int c0 = half * 16; c0 < d.cols; c0 += 32) {
+                float v[16];
+                tc::tmem_ld16(p.tmem + b * NT + ((uint32_t)(q * 32) << 16) + c0, v);
+                tc::tmem_wait_ld();
+                uint16_t* y = a.y + (long long)(d.t0 + c0) * a.ldy + n;
+                if (pairs32) {
+                    y -= odd;
+#pragma unroll
+                    for (int c = 0; c < 16; c += 2) {
+                        const float got = __shfl_xor_sync(~0u, odd ? v[c] : v[c + 1], 1);
+                        const int r = d.t0 + c0 + c + odd;
+                        if (r < d.t1) {
+                            uint16_t* const o = y + (long long)(c + odd) * a.ldy;
+                            if (n - odd + 1 < a.N)
+                                *reinterpret_cast<uint32_t*>(o) = odd ? pack16(got, v[c + 1], a.bf16) : pack16(v[c], got, a.bf16);
+                            else if (n - odd < a.N)
+                                *o = to16(odd ? got : v[c], a.bf16);
+                        }
+                    }
+                } else if (n < a.N) {
+#pragma unroll
+                    for (int c = 0; c < 16; ++c)
+                        if (d.t0 + c0 + c < d.t1) y[(long long)c * a.ldy] = to16(v[c], a.bf16);
+                }
+                __syncwarp();
+            }
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive_cluster(p.tempty0 + b * 8);
+        }
+    }
+    tear_down(p, a.status);
+}
+
+// The sums of products of 16-bit values are rounded toward zero by the tensor core at every addition to its fp32
+// accumulator; over thousands of rows that bias would pass what fp32 results may be off.  So the accumulator is taken
+// after every DRAIN stages (256 rows) and added to fp32 sums in registers, rounded to nearest, while the products go on
+// in the other accumulator.
+template <typename OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    k_mm_wgrad(const __grid_constant__ CUtensorMap tdy, const __grid_constant__ CUtensorMap tx, const MmWgradArgs a) {
+    extern __shared__ char dyn[];
+    const Pair p = set_up(dyn, a.offsets, a.E, a.T, 1 << 30, 2);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ntn = (a.N + 2 * FT - 1) / (2 * FT), ntk = (a.K + NT - 1) / NT, per = ntn * ntk;
+    const long long tiles = (long long)a.E * per;
+    const int pairs = (int)gridDim.x / 2;
+    struct Tile {
+        int e, n0, k0, cols, r0, rows, nb;   // cols: the tile's columns of x up to a multiple of 32; nb: stages of 64 rows
+    };
+    auto tile_at = [&](long long i) {
+        Tile t;
+        t.e = (int)(i / per);
+        const int l = (int)(i - (long long)t.e * per);
+        t.n0 = l / ntk * 2 * FT;
+        t.k0 = l % ntk * NT;
+        t.cols = min(NT, up32(a.K - t.k0));
+        t.r0 = p.start[t.e];
+        t.rows = p.start[t.e + 1] - t.r0;
+        t.nb = (t.rows + BK - 1) / BK;
+        return t;
+    };
+
+    if (warp == 8) {
+        uint64_t* const ragged = p.tempty + 2;
+        int i = 0, nragged = 0;
+        bool ok = true;
+        for (long long t = blockIdx.x / 2; ok && t < tiles; t += pairs) {
+            const Tile d = tile_at(t);
+            const int n = d.n0 + p.rank * FT, k = d.k0 + p.rank * (d.cols / 2);
+            for (int c = 0; c < d.nb; ++c, ++i) {
+                ok = stage_free(p, i);   // every lane: the warp leaves together
+                if (!__all_sync(~0u, ok)) {
+                    ok = false;
+                    break;
+                }
+                const int s = i % STAGES, left = d.rows - c * BK, row = d.r0 + c * BK;
+                const uint32_t as = tc::smem_u32(p.sm) + s * STAGE;
+                if (left >= BK || left % 16 == 0) {
+                    if (lane == 0) {
+                        const uint32_t bar = p.full0 + s * 8;
+                        if (p.rank == 0) tc::mbar_expect_tx(&p.full[s], 2 * STAGE);
+                        else arrive_cluster(bar);
+                        tma2_load_2d(as, &tdy, n, row, bar);
+                        tma2_load_2d(as + BOX_MN, &tdy, n + 64, row, bar);
+                        tma2_load_2d(as + HALF, &tx, k, row, bar);
+                        tma2_load_2d(as + HALF + BOX_MN, &tx, k + 64, row, bar);
+                    }
+                } else {
+                    // the expert's last rows, not a multiple of one product's 16: the rows behind them (another expert's)
+                    // are zeroed in both operands before the products may read the stage
+                    if (lane == 0) {
+                        const uint32_t bar = tc::smem_u32(ragged);
+                        tc::mbar_expect_tx(ragged, STAGE);
+                        mm::tma_load_2d(as, &tdy, n, row, bar);
+                        mm::tma_load_2d(as + BOX_MN, &tdy, n + 64, row, bar);
+                        mm::tma_load_2d(as + HALF, &tx, k, row, bar);
+                        mm::tma_load_2d(as + HALF + BOX_MN, &tx, k + 64, row, bar);
+                    }
+                    __syncwarp();
+                    ok = tc::mbar_wait(ragged, (uint32_t)(nragged++ & 1));
+                    if (!__all_sync(~0u, ok)) {
+                        *p.err = 1;
+                        ok = false;
+                        break;
+                    }
+                    char* const st = p.sm + s * STAGE;
+                    const int upto = (left + 15) & ~15;   // box lane / 8, 16 bytes (lane % 8) of each row
+                    for (int r = left; r < upto; ++r)
+                        *reinterpret_cast<int4*>(st + (lane >> 3) * BOX_MN + r * 128 + (lane & 7) * 16) = make_int4(0, 0, 0, 0);
+                    tc::fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) arrive_cluster(p.full0 + s * 8);
+                }
+            }
+        }
+        if (lane == 0) finish_copies(p, i);
+    } else if (warp == 9) {
+        if (lane == 0 && p.rank == 0) {
+            int i = 0, j = 0;   // stages and accumulators over all tiles
+            for (long long t = blockIdx.x / 2; t < tiles && !*p.err; t += pairs) {
+                const Tile d = tile_at(t);
+                const uint32_t id = idesc_f16(2 * FT, d.cols, a.bf16, true, true);
+                for (int c = 0; c < d.nb; ++c, ++i) {
+                    const int s = i % STAGES, b = j & 1;
+                    if (c % DRAIN == 0) {
+                        if (j >= 2 && !tc::mbar_wait(&p.tempty[b], (uint32_t)((j / 2 - 1) & 1))) *p.err = 1;
+                        tc::fence_after_sync();
+                    }
+                    if (*p.err || !tc::mbar_wait(&p.full[s], (uint32_t)((i / STAGES) & 1))) {
+                        *p.err = 1;
+                        break;
+                    }
+                    tc::fence_after_sync();
+                    const uint32_t as = tc::smem_u32(p.sm) + s * STAGE, bs = as + HALF, acc = p.tmem + b * NT;
+                    const int steps = min(BK, d.rows - c * BK + 15) / 16;
+                    for (int q = 0; q < steps; ++q)
+                        mma2_f16(acc, sdesc<true>(as + q * kstep<true>()), sdesc<true>(bs + q * kstep<true>()), id,
+                                 c % DRAIN > 0 || q > 0);
+                    commit2(&p.empty[s]);
+                    if (c % DRAIN == DRAIN - 1 || c == d.nb - 1) {
+                        commit2(&p.tfull[b]);
+                        ++j;
+                    }
+                }
+            }
+        }
+    } else {
+        const int q = warp & 3, half = warp >> 2;
+        int j = 0;
+        bool ok = true;
+        for (long long t = blockIdx.x / 2; ok && t < tiles; t += pairs) {
+            const Tile d = tile_at(t);
+            float sum[NT / 2];
+#pragma unroll
+            for (int c = 0; c < NT / 2; ++c) sum[c] = 0.f;
+            for (int c = 0; c < d.nb; c += DRAIN, ++j) {
+                const int b = j & 1;
+                ok = !*p.err && tc::mbar_wait(&p.tfull[b], (uint32_t)((j / 2) & 1));
+                if (!__all_sync(~0u, ok)) {
+                    *p.err = 1;
+                    ok = false;
+                    break;
+                }
+                tc::fence_after_sync();
+                const uint32_t at = p.tmem + b * NT + half * (NT / 2) + ((uint32_t)(q * 32) << 16);
+#pragma unroll
+                for (int c0 = 0; c0 < NT / 2; c0 += 16) {
+                    if (half * (NT / 2) + c0 < d.cols) {
+                        float v[16];
+                        tc::tmem_ld16(at + c0, v);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) sum[c0 + x] += v[x];
+                    }
+                }
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) arrive_cluster(p.tempty0 + b * 8);
+            }
+            if (!ok) break;
+            const int n = d.n0 + p.rank * FT + q * 32 + lane, k = d.k0 + half * (NT / 2);
+            OUT* const row = static_cast<OUT*>(a.dw) + ((long long)d.e * a.N + n) * a.K + k;
+            constexpr int PER = 32 / sizeof(OUT);
+            const bool whole = (reinterpret_cast<uintptr_t>(row) & 31) == 0;
+            const int K = n < a.N ? a.K : 0;   // a lane without a feature stores nothing
+#pragma unroll
+            for (int c = 0; c < NT / 2; c += PER) {
+                if (whole && k + c + PER <= K) {
+                    float w[8];
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        if constexpr (sizeof(OUT) == 4) w[x] = sum[c + x];
+                        else w[x] = __uint_as_float(pack16(sum[c + 2 * x], sum[c + 2 * x + 1], a.bf16));
+                    }
+                    tc::st8(reinterpret_cast<float*>(row + c), w);
+                } else {
+#pragma unroll
+                    for (int x = 0; x < PER; ++x) {
+                        if (k + c + x < K) {
+                            if constexpr (sizeof(OUT) == 4) row[c + x] = sum[c + x];
+                            else row[c + x] = to16(sum[c + x], a.bf16);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+        }
+    }
+    tear_down(p, a.status);
+}
+
+template <typename K, typename... A>
+cudaError_t go(K kernel, long long tiles, int E, cudaStream_t st, const A&... args) {
+    int nsm = 0;
+    cudaError_t e = sm_count(&nsm);
+    const int smem = FIXED + 2 * (E + 1) * (int)sizeof(int);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const long long pairs = tiles < nsm / 2 ? tiles : nsm / 2;
+    kernel<<<(unsigned)(2 * pairs), THREADS, smem, st>>>(args...);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_mm_wide(const MmOperand& x, const MmOperand& w, const MmArgs& args, cudaStream_t st) {
+    MmArgs a = args;
+    a.ntn = (a.N + 2 * FT - 1) / (2 * FT);
+    alignas(64) CUtensorMap tw, tx;
+    cudaError_t e = encode_mm(&tx, x, a.bf16, BK, FT);
+    if (e == cudaSuccess) e = w.mn ? encode_mm(&tw, w, a.bf16, 64, BK) : encode_mm(&tw, w, a.bf16, BK, FT);
+    if (e != cudaSuccess) return e;
+    const long long tiles = ((long long)(a.T / NT) + (a.T < a.E ? a.T : a.E)) * a.ntn;   // the most the offsets could give
+    if (tiles > (1LL << 30)) return cudaErrorInvalidValue;
+    return w.mn ? go(k_mm_wide<true>, tiles, a.E, st, tw, tx, a) : go(k_mm_wide<false>, tiles, a.E, st, tw, tx, a);
+}
+
+cudaError_t launch_mm_wgrad(const MmOperand& dy, const MmOperand& x, const MmWgradArgs& a, cudaStream_t st) {
+    alignas(64) CUtensorMap tdy, tx;
+    cudaError_t e = encode_mm(&tdy, dy, a.bf16, 64, BK);
+    if (e == cudaSuccess) e = encode_mm(&tx, x, a.bf16, 64, BK);
+    if (e != cudaSuccess) return e;
+    const long long tiles = (long long)a.E * ((a.N + 2 * FT - 1) / (2 * FT)) * ((a.K + NT - 1) / NT);
+    return a.out32 ? go(k_mm_wgrad<float>, tiles, a.E, st, tdy, tx, a) : go(k_mm_wgrad<uint16_t>, tiles, a.E, st, tdy, tx, a);
+}
+
+}  // namespace spq

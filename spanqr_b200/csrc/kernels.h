@@ -163,4 +163,41 @@ cudaError_t launch_grad_finish(const double* part, int nparts, double* sumsq, fl
 cudaError_t launch_grad_scale(const GradEntry* e, int count, const double* part, int nparts, double max_norm, float* norm,
                               cudaStream_t st);
 
+// ---- products grouped by expert ----
+// A 16-bit operand: `rows` rows of `cols` contiguous elements, `ld` elements apart (a multiple of 8), in `planes` planes
+// `plane` elements apart (0 planes: a plain matrix), 16-byte aligned.  mn: the contracted dimension runs along the rows.
+struct MmOperand {
+    const void* p;
+    long long cols, rows, ld;
+    int planes;
+    long long plane;
+    bool mn;
+};
+struct MmArgs {
+    const int* offsets;   // [E] ends of the experts' rows (device)
+    int E, T, N, K;       // experts, rows, features, contracted elements
+    uint16_t* y;          // [T, N], ld ldy
+    long long ldy;
+    int ntn;              // feature tiles of 128
+    bool bf16;            // bf16, else fp16
+    bool zero_tail;       // zero the rows behind the last expert (else they are left as they are)
+    int* status;          // a bounded wait that runs out ORs MM_TIMEOUT
+};
+constexpr int MM_TIMEOUT = 0x100;
+// tensor map of 16-bit tiles of box_cols x box_rows in the 128-byte-swizzled layout; elements outside read as zeros
+cudaError_t encode_mm(CUtensorMap* m, const MmOperand& o, bool bf16, int box_cols, int box_rows);
+// y[t] = w[e(t)] x[t] for few rows per expert: row tiles of tn (16, 32 or 64)
+cudaError_t launch_mm_narrow(const MmOperand& x, const MmOperand& w, const MmArgs& a, int tn, cudaStream_t st);
+// the same for many rows per expert: tiles of 256 features x up to 256 rows on pairs of SMs (a.ntn is set there)
+cudaError_t launch_mm_wide(const MmOperand& x, const MmOperand& w, const MmArgs& a, cudaStream_t st);
+struct MmWgradArgs {
+    const int* offsets;
+    int E, T, N, K;
+    void* dw;       // [E, N, K], fp32 (out32) or the operands' type
+    bool bf16, out32;
+    int* status;
+};
+// dw[e] = sum over e's rows of dy[t] x[t]^T
+cudaError_t launch_mm_wgrad(const MmOperand& dy, const MmOperand& x, const MmWgradArgs& a, cudaStream_t st);
+
 }  // namespace spq

@@ -1,0 +1,151 @@
+// What the products grouped by expert share: 16-bit tcgen05 products, TMA loads, and the map from offsets to tiles.
+//
+// Operand tiles hold 64 elements of the contracted dimension.  K-major (the contracted dimension contiguous in memory):
+// R rows of 128 bytes, one TMA box, 8-row atoms of 1024 bytes with the 16-byte chunks of row m at chunk ^ (m % 8).
+// MN-major (the other dimension contiguous): boxes of 64 columns x 64 contracted rows (8 KB), the same swizzle; one
+// product of 16 contracted rows then starts 2048 bytes after the last.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kernels.h"
+#include "tc.cuh"
+
+namespace spq {
+namespace mm {
+
+constexpr int BK = 64;                 // contracted elements per pipeline stage
+constexpr int FT = 128;                // features (rows of TMEM) per CTA
+constexpr int BOX_MN = 64 * 128;       // bytes of one MN-major box
+
+// ---- products: D[tmem] (+)= A[smem] * B[smem]^T, 16-bit operands of one type, fp32 accumulation ----
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+        :
+        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+        : "memory");
+}
+
+// instruction descriptor: D fp32, A and B both bf16 or both fp16, each K-major or MN-major, M x N
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool bf16, bool a_mn, bool b_mn) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((a_mn ? 1u : 0u) << 15) |
+           ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// shared-memory descriptor of an MN-major 128-byte-swizzled tile: 64-column boxes 8 KB apart (leading byte offset),
+// groups of 8 contracted rows 1024 bytes apart (stride byte offset)
+__device__ __forceinline__ uint64_t sdesc_mn128(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(BOX_MN >> 4) << 16) | ((uint64_t)64u << 32) |
+           ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+}
+template <bool MN>
+__device__ __forceinline__ uint64_t sdesc(uint32_t saddr) {
+    return MN ? sdesc_mn128(saddr) : tc::sdesc_k128(saddr);
+}
+// bytes from one product's operand start to the next one's (16 contracted elements)
+template <bool MN>
+__device__ __forceinline__ constexpr uint32_t kstep() { return MN ? 2048u : 32u; }
+
+__device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const void* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(smem_dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const void* map, int c0, int c1, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(smem_dst), "l"(map), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void prefetch_map(const void* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+// the address in CTA `rank` of this cluster of a shared-memory address of this CTA
+__device__ __forceinline__ uint32_t mapa(uint32_t saddr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+// ---- 16-bit results ----
+__device__ __forceinline__ uint16_t to16(float x, bool bf16) {
+    return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));
+}
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
+    if (bf16) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&b);
+    }
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// ---- offsets -> tiles ----
+// start[e], start[e + 1]: the rows of expert e; pre[e]: tiles of `rows` rows before it (both E + 1 long, in shared
+// memory).  offsets[e] is the end of expert e's rows; ends are clamped to [previous end, T], so that no offsets make a
+// kernel leave its tensors.  Run by one whole warp.
+__device__ __forceinline__ void map_groups(const int* __restrict__ offsets, int E, int T, int rows, int* start, int* pre) {
+    const int lane = threadIdx.x & 31;
+    int end = 0, tiles = 0;
+    int next = lane < E ? offsets[lane] : 0;
+    for (int e0 = 0; e0 < E; e0 += 32) {
+        int v = min(max(next, 0), T);
+        if (e0 + 32 + lane < E) next = offsets[e0 + 32 + lane];
+        else next = 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(~0u, v, o);
+            if (lane >= o) v = max(v, u);
+        }
+        v = max(v, end);
+        int before = __shfl_up_sync(~0u, v, 1);
+        if (lane == 0) before = end;
+        int s = (v - before + rows - 1) / rows;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(~0u, s, o);
+            if (lane >= o) s += u;
+        }
+        if (e0 + lane < E) {
+            start[e0 + lane + 1] = v;
+            pre[e0 + lane + 1] = tiles + s;
+        }
+        end = __shfl_sync(~0u, v, 31);
+        tiles += __shfl_sync(~0u, s, 31);
+    }
+    if (lane == 0) start[0] = pre[0] = 0;
+}
+
+// the expert that holds row tile u < pre[E]
+__device__ __forceinline__ int group_of(const int* pre, int E, int u) {
+    int lo = 0, hi = E - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid + 1] > u) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+
+}  // namespace mm
+}  // namespace spq

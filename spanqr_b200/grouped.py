@@ -1,0 +1,219 @@
+"""Matrix products grouped by expert: rows sorted by expert, a ragged number of them each (no reference counterpart; the
+layers whose gradients clip_grads and orth_batched then take).
+
+    from spanqr_b200 import mm_grouped, mm_grouped_wgrad
+    y = mm_grouped(x, w, offsets)                 # y[t] = w[e(t)] @ x[t], differentiable in x and w
+    dw = mm_grouped_wgrad(dy, x, offsets)         # dw[e] = sum over e's rows of dy[t] x[t]^T, fp32: orth's input type
+
+x is [T, K] with the rows of expert e at offsets[e - 1] .. offsets[e] (offsets: int32 on the GPU, the cumulative sum of
+the rows per expert), w is [E, N, K], bf16 or fp16.  Everything runs on libspanqr's kernels on the current stream of x's
+device; the offsets are only read on the device, so nothing synchronises with the host.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .grads import DTYPES
+
+MAX_EXPERTS = 1024
+
+
+def _up8(n):
+    return -(-n // 8) * 8
+
+
+def _row_stride(t, rows, cols):
+    """the row stride of t as an operand the copy engine can read (16-byte aligned rows of contiguous elements), or None.
+    rows, cols: the dimensions of t that run over rows and along them."""
+    if t.shape[cols] > 1 and t.stride(cols) != 1 or t.data_ptr() % 16:
+        return None
+    if t.shape[rows] == 1:
+        return _up8(t.shape[cols])   # a single row's stride is free
+    ld = t.stride(rows)
+    return ld if ld % 8 == 0 and ld >= t.shape[cols] else None
+
+
+def _padded(t):
+    """a copy of t with its last dimension contiguous and every row on 16 bytes"""
+    buf = torch.empty((*t.shape[:-1], _up8(t.shape[-1])), dtype=t.dtype, device=t.device)
+    v = buf[..., :t.shape[-1]]
+    v.copy_(t)
+    return v
+
+
+def _rows(x):
+    """x [T, K] (or a padded copy) and its row stride"""
+    ld = _row_stride(x, 0, 1)
+    if ld is None:
+        x = _padded(x)
+        ld = _row_stride(x, 0, 1)
+    return x, ld
+
+
+def _weights(w):
+    """w [E, N, K] (or a padded copy), its row stride, its expert stride and whether it is stored [E, K, N]"""
+    E, N, K = w.shape
+    for transposed, (rows, cols) in ((False, (1, 2)), (True, (2, 1))):
+        ld = _row_stride(w, rows, cols)
+        if ld is None:
+            continue
+        need = (w.shape[rows] - 1) * ld + w.shape[cols]
+        if E == 1:
+            return w, ld, _up8(need), transposed
+        if w.stride(0) % 8 == 0 and w.stride(0) >= need:
+            return w, ld, w.stride(0), transposed
+    return _weights(_padded(w))
+
+
+def _span(t):
+    a = t.data_ptr()
+    if t.numel() == 0:
+        return a, a
+    return a, a + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _no_overlap(out, **others):
+    a, b = _span(out)
+    for name, t in others.items():
+        c, d = _span(t)
+        if a < d and c < b:
+            raise ValueError(f"out overlaps {name}")
+
+
+def _check_rows(x, name):
+    if not torch.is_tensor(x) or x.dim() != 2:
+        raise ValueError(f"{name} must be a 2-D tensor")
+    if x.dtype not in (torch.bfloat16, torch.float16) or not x.is_cuda:
+        raise TypeError(f"{name} must be a bf16 or fp16 CUDA tensor (got {x.dtype} on {x.device})")
+    if x.shape[1] < 1:
+        raise ValueError(f"{name} has no columns")
+
+
+def _check_offsets(offsets, x, E=None):
+    if not torch.is_tensor(offsets) or offsets.dim() != 1:
+        raise ValueError("offsets must be a 1-D tensor: the end of each expert's rows")
+    if offsets.dtype != torch.int32 or offsets.device != x.device:
+        raise TypeError(f"offsets must be int32 on {x.device} (got {offsets.dtype} on {offsets.device})")
+    n = offsets.shape[0]
+    if E is not None and n != E:
+        raise ValueError(f"offsets must have one end per expert: {E} (got {n})")
+    if not 1 <= n <= MAX_EXPERTS:
+        raise ValueError(f"1 to {MAX_EXPERTS} experts (got {n})")
+    return offsets if offsets.stride(0) == 1 or n == 1 else offsets.contiguous()
+
+
+def _mm(x, w, offsets, out=None):
+    T, K = x.shape
+    E, N, _ = w.shape
+    y = torch.empty((T, N), dtype=x.dtype, device=x.device) if out is None else out
+    if T == 0:
+        return y
+    x, ldx = _rows(x)
+    w, ldw, plane, transposed = _weights(w)
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.lib().spanqr_mm_grouped(x.data_ptr(), ldx, w.data_ptr(), ldw, plane, int(transposed),
+                                                offsets.data_ptr(), y.data_ptr(), y.stride(0) if T > 1 else N,
+                                                DTYPES[x.dtype], T, E, N, K, int(out is None),
+                                                torch.cuda.current_stream(x.device).cuda_stream),
+                   f"mm_grouped({T}x{K}, {E} experts of {N}x{K})")
+    return y
+
+
+def _wgrad(dy, x, offsets, dtype, out=None):
+    T, N = dy.shape
+    K, E = x.shape[1], offsets.shape[0]
+    dw = torch.empty((E, N, K), dtype=dtype, device=x.device) if out is None else out
+    dy, lddy = _rows(dy) if T else (dy, N)
+    x, ldx = _rows(x) if T else (x, K)
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.lib().spanqr_mm_grouped_wgrad(dy.data_ptr(), lddy, x.data_ptr(), ldx, offsets.data_ptr(),
+                                                      dw.data_ptr(), DTYPES[x.dtype], DTYPES[dw.dtype], T, E, N, K,
+                                                      torch.cuda.current_stream(x.device).cuda_stream),
+                   f"mm_grouped_wgrad({T} rows, {E} experts of {N}x{K})")
+    return dw
+
+
+class _MmGrouped(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, offsets):
+        ctx.save_for_backward(x, w, offsets)
+        return _mm(x, w, offsets)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w, offsets = ctx.saved_tensors
+        dx = _mm(dy, w.transpose(1, 2), offsets) if ctx.needs_input_grad[0] else None
+        dw = _wgrad(dy, x, offsets, w.dtype) if ctx.needs_input_grad[1] else None
+        return dx, dw, None
+
+
+def mm_grouped(x, w, offsets, *, out=None):
+    """y [T, N] with y[t] = w[e(t)] @ x[t] for the expert e(t) whose rows hold t: x [T, K] and w [E, N, K] of one type
+    (bf16 or fp16), offsets int32 [E], the end of each expert's rows.  Experts may be empty; w may be stored [E, N, K] or
+    [E, K, N] (pass its transposed view).  Rows from offsets[-1] on belong to no expert: they are zero in a new y and
+    left as they are in `out`, a [T, N] tensor of x's type with contiguous rows that overlaps neither input.  The products
+    are summed in fp32 and rounded once.
+
+    Operands whose rows do not start on 16 bytes (K not a multiple of 8, odd strides or addresses), or that are contiguous
+    along neither dimension, are copied first.  Ends that decrease or lie outside [0, T] are clamped to the nearest that
+    do not, on the device.
+
+    Differentiable once in x and w (without `out`): dx is this product with the transposed weights, dw is
+    mm_grouped_wgrad in w's type; rows behind the last expert get a zero gradient and give none."""
+    _check_rows(x, "x")
+    if not torch.is_tensor(w) or w.dim() != 3 or w.shape[2] != x.shape[1]:
+        raise ValueError(f"w must be a 3-D tensor [E, N, {x.shape[1]}]")
+    if w.dtype != x.dtype or w.device != x.device:
+        raise TypeError(f"w must be {x.dtype} on {x.device}, as x (got {w.dtype} on {w.device})")
+    if w.shape[1] < 1:
+        raise ValueError("w has no rows")
+    offsets = _check_offsets(offsets, x, w.shape[0])
+    grad = torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
+    if out is None:
+        return _MmGrouped.apply(x, w, offsets) if grad else _mm(x, w, offsets)
+    if grad:
+        raise RuntimeError("mm_grouped with out= is not differentiable: leave out away, or use torch.no_grad()")
+    if not torch.is_tensor(out) or out.shape != (x.shape[0], w.shape[1]):
+        raise ValueError(f"out must have shape {(x.shape[0], w.shape[1])}")
+    if out.dtype != x.dtype or out.device != x.device:
+        raise TypeError(f"out must be {x.dtype} on {x.device} (got {out.dtype} on {out.device})")
+    if out.shape[1] > 1 and out.stride(1) != 1 or out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+        raise ValueError("out must have contiguous rows that do not overlap")
+    _no_overlap(out, x=x, w=w, offsets=offsets)
+    _mm(x, w, offsets, out)
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+    return out
+
+
+def mm_grouped_wgrad(dy, x, offsets, *, out=None, dtype=None):
+    """dw [E, N, K] with dw[e] = sum over expert e's rows t of dy[t] x[t]^T: the weight gradient of mm_grouped.  dy [T, N]
+    and x [T, K] of one type (bf16 or fp16), offsets int32 [E] as there; an expert without rows gets zeros, and rows from
+    offsets[-1] on count nowhere.  dtype is fp32 (the default: what clip_grads and orth_batched take) or the inputs' type;
+    `out`, a contiguous [E, N, K] tensor of either type that overlaps neither input, is overwritten.  Summed in fp32 (sums
+    of 256 rows by the tensor cores, those rounded to nearest) and rounded once.  Not differentiable."""
+    _check_rows(dy, "dy")
+    _check_rows(x, "x")
+    if dy.shape[0] != x.shape[0]:
+        raise ValueError(f"dy and x must have as many rows (got {dy.shape[0]} and {x.shape[0]})")
+    if dy.dtype != x.dtype or dy.device != x.device:
+        raise TypeError(f"dy must be {x.dtype} on {x.device}, as x (got {dy.dtype} on {dy.device})")
+    offsets = _check_offsets(offsets, x)
+    shape = (offsets.shape[0], dy.shape[1], x.shape[1])
+    if out is None:
+        dtype = torch.float32 if dtype is None else dtype
+        if dtype not in (torch.float32, x.dtype):
+            raise TypeError(f"dtype must be fp32 or {x.dtype} (got {dtype})")
+        return _wgrad(dy.detach(), x.detach(), offsets, dtype)
+    if dtype is not None:
+        raise ValueError("give dtype or out, not both")
+    if not torch.is_tensor(out) or out.shape != shape or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous with shape {shape}")
+    if out.dtype not in (torch.float32, x.dtype) or out.device != x.device:
+        raise TypeError(f"out must be fp32 or {x.dtype} on {x.device} (got {out.dtype} on {out.device})")
+    _no_overlap(out, dy=dy, x=x, offsets=offsets)
+    _wgrad(dy.detach(), x.detach(), offsets, None, out)
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+    return out
