@@ -28,7 +28,9 @@ constexpr int NT = 256;            // columns of a tile
 constexpr int BARS = STAGES * STAGE;
 constexpr int MAPS = BARS + 256;
 constexpr int FIXED = MAPS + 16 + 1024;
-constexpr int DRAIN = 4;           // wgrad: stages (of 64 rows) summed in TMEM before they are added in registers
+// wgrad: stages (of 64 rows) summed in TMEM before they are added in registers
+template <typename OUT>
+constexpr int DRAIN = sizeof(OUT) == 4 ? 8 : 32;
 
 // ---- cta_group::2 forms ----
 __device__ __forceinline__ void mma2_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -77,24 +79,44 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// the bounded wait on a barrier that the other CTA arrives on
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, uint64_t limit_ns = 2000000000ull) {
+    const uint64_t t0 = tc::globaltimer();
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(tc::smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (tc::globaltimer() - t0 > limit_ns) return false;
+    }
+}
+
 // the pair's shared state, set up before any role begins
 struct Pair {
     char* sm;
     uint64_t *full, *empty, *tfull, *tempty;
+    uint64_t *ragged, *zeroed;   // wgrad: this CTA's copies of a ragged stage; (leader) the other CTA's part of stage s is zeroed
     volatile int* err;
     int *start, *pre;
     uint32_t tmem;
     int rank;
-    uint32_t full0, tempty0;   // cluster addresses of the leader's barriers
+    uint32_t full0, tempty0, zeroed0;   // cluster addresses of the leader's barriers
 };
 
-__device__ __forceinline__ Pair set_up(char* dyn, const int* offsets, int E, int T, int rows_per_tile, int full_arrivals) {
+__device__ __forceinline__ Pair set_up(char* dyn, const int* offsets, int E, int T, int rows_per_tile) {
     Pair p;
     p.sm = dyn + ((1024u - (tc::smem_u32(dyn) & 1023u)) & 1023u);
     p.full = reinterpret_cast<uint64_t*>(p.sm + BARS);
     p.empty = p.full + STAGES;
     p.tfull = p.empty + STAGES;
     p.tempty = p.tfull + 2;
+    p.ragged = p.tempty + 2;
+    p.zeroed = p.ragged + 1;
     uint32_t* const slot = reinterpret_cast<uint32_t*>(p.sm + MAPS);
     p.err = reinterpret_cast<int*>(p.sm + MAPS + 4);
     p.start = reinterpret_cast<int*>(p.sm + MAPS + 16);
@@ -105,14 +127,15 @@ __device__ __forceinline__ Pair set_up(char* dyn, const int* offsets, int E, int
     if (warp == 9) tmem_alloc2(slot, 2 * NT);
     if (threadIdx.x == 256) {
         for (int s = 0; s < STAGES; ++s) {
-            tc::mbar_init(&p.full[s], full_arrivals);
+            tc::mbar_init(&p.full[s], 1);
             tc::mbar_init(&p.empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
             tc::mbar_init(&p.tfull[b], 1);
             tc::mbar_init(&p.tempty[b], 16);
         }
-        tc::mbar_init(p.tempty + 2, 1);   // wgrad: the copies of a ragged last stage
+        tc::mbar_init(p.ragged, 1);
+        for (int s = 0; s < STAGES; ++s) tc::mbar_init(&p.zeroed[s], 1);
         tc::mbar_fence_init();
         *p.err = 0;
     }
@@ -123,6 +146,7 @@ __device__ __forceinline__ Pair set_up(char* dyn, const int* offsets, int E, int
     p.tmem = *slot;
     p.full0 = mapa(tc::smem_u32(p.full), 0);
     p.tempty0 = mapa(tc::smem_u32(p.tempty), 0);
+    p.zeroed0 = mapa(tc::smem_u32(p.zeroed), 0);
     return p;
 }
 
@@ -157,7 +181,7 @@ template <bool W_MN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     k_mm_wide(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, const MmArgs a) {
     extern __shared__ char dyn[];
-    const Pair p = set_up(dyn, a.offsets, a.E, a.T, NT, 1);
+    const Pair p = set_up(dyn, a.offsets, a.E, a.T, NT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int ntn = a.ntn, tiles = p.pre[a.E] * ntn, pairs = (int)gridDim.x / 2;
     const int kb = (a.K + BK - 1) / BK;
@@ -201,29 +225,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             finish_copies(p, i);
         }
     } else if (warp == 9) {
-        if (lane == 0 && p.rank == 0) {
-            int i = 0, j = 0;
+        // the whole warp runs the loop (its state stays in uniform registers, which the products' operands need), one
+        // thread issues
+        if (p.rank == 0) {
+            const bool one = elect();
+            const uint64_t a0 = sdesc<W_MN>(tc::smem_u32(p.sm)), b0 = sdesc<false>(tc::smem_u32(p.sm) + HALF);
+            int s = 0, j = 0;
+            uint32_t phase = 0;
             for (int t = (int)blockIdx.x / 2; t < tiles && !*p.err; t += pairs, ++j) {
                 const Tile d = tile_at(t);
                 const int b = j & 1;
                 const uint32_t acc = p.tmem + b * NT, id = idesc_f16(2 * FT, d.cols, a.bf16, W_MN, false);
                 if (j >= 2 && !tc::mbar_wait(&p.tempty[b], (uint32_t)((j / 2 - 1) & 1))) *p.err = 1;
                 tc::fence_after_sync();
-                for (int k = 0; k < kb; ++k, ++i) {
-                    const int s = i % STAGES;
-                    if (*p.err || !tc::mbar_wait(&p.full[s], (uint32_t)((i / STAGES) & 1))) {
+                for (int k = 0; k < kb; ++k) {
+                    if (*p.err || !tc::mbar_wait(&p.full[s], phase)) {
                         *p.err = 1;
                         break;
                     }
                     tc::fence_after_sync();
-                    const uint32_t as = tc::smem_u32(p.sm) + s * STAGE, bs = as + HALF;
+                    if (one) {
 #pragma unroll
-                    for (int q = 0; q < BK / 16; ++q)
-                        mma2_f16(acc, sdesc<W_MN>(as + q * kstep<W_MN>()), sdesc<false>(bs + q * kstep<false>()), id,
-                                 k > 0 || q > 0);
-                    commit2(&p.empty[s]);
+                        for (int q = 0; q < BK / 16; ++q)
+                            mma2_f16(acc, a0 + ((s * STAGE + q * kstep<W_MN>()) >> 4), b0 + ((s * STAGE + q * kstep<false>()) >> 4),
+                                     id, k > 0 || q > 0);
+                        commit2(&p.empty[s]);
+                    }
+                    if (++s == STAGES) s = 0, phase ^= 1;
                 }
-                commit2(&p.tfull[b]);
+                if (one) commit2(&p.tfull[b]);
             }
         }
     } else {
@@ -280,15 +310,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tear_down(p, a.status);
 }
 
-// The sums of products of 16-bit values are rounded toward zero by the tensor core at every addition to its fp32
-// accumulator; over thousands of rows that bias would pass what fp32 results may be off.  So the accumulator is taken
-// after every DRAIN stages (256 rows) and added to fp32 sums in registers, rounded to nearest, while the products go on
-// in the other accumulator.
+// The tensor core rounds toward zero each time it adds 16 products to its fp32 accumulator: over n additions of terms of
+// random sign the sum comes out about n * 3e-8 of itself too small.  So the accumulator is taken every DRAIN stages and
+// added to fp32 sums in registers, rounded to nearest, while the products go on in the other accumulator.  For fp32
+// results every 512 rows (measured 4e-7 off in all at 5000 rows, as a sum in fp32 is); for 16-bit results, whose own
+// rounding is 2^-9 or 2^-12, every 2048, which keeps the bias from growing with the length.  The reads of TMEM
+// take tensor-core time: 16384 rows, 8 experts of 5120x2048 in bf16: 285 us with a drain every 256 rows, 258 every 512, 252 every 4096.
 template <typename OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     k_mm_wgrad(const __grid_constant__ CUtensorMap tdy, const __grid_constant__ CUtensorMap tx, const MmWgradArgs a) {
     extern __shared__ char dyn[];
-    const Pair p = set_up(dyn, a.offsets, a.E, a.T, 1 << 30, 2);
+    const Pair p = set_up(dyn, a.offsets, a.E, a.T, 1 << 30);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int ntn = (a.N + 2 * FT - 1) / (2 * FT), ntk = (a.K + NT - 1) / NT, per = ntn * ntk;
     const long long tiles = (long long)a.E * per;
@@ -310,8 +342,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     };
 
     if (warp == 8) {
-        uint64_t* const ragged = p.tempty + 2;
-        int i = 0, nragged = 0;
+        int i = 0;
+        uint32_t ragged_phase = 0, zeroed_phases = 0;   // (bit s: that of zeroed[s])
         bool ok = true;
         for (long long t = blockIdx.x / 2; ok && t < tiles; t += pairs) {
             const Tile d = tile_at(t);
@@ -328,7 +360,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     if (lane == 0) {
                         const uint32_t bar = p.full0 + s * 8;
                         if (p.rank == 0) tc::mbar_expect_tx(&p.full[s], 2 * STAGE);
-                        else arrive_cluster(bar);
                         tma2_load_2d(as, &tdy, n, row, bar);
                         tma2_load_2d(as + BOX_MN, &tdy, n + 64, row, bar);
                         tma2_load_2d(as + HALF, &tx, k, row, bar);
@@ -338,15 +369,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     // the expert's last rows, not a multiple of one product's 16: the rows behind them (another expert's)
                     // are zeroed in both operands before the products may read the stage
                     if (lane == 0) {
-                        const uint32_t bar = tc::smem_u32(ragged);
-                        tc::mbar_expect_tx(ragged, STAGE);
+                        const uint32_t bar = tc::smem_u32(p.ragged);
+                        tc::mbar_expect_tx(p.ragged, STAGE);
                         mm::tma_load_2d(as, &tdy, n, row, bar);
                         mm::tma_load_2d(as + BOX_MN, &tdy, n + 64, row, bar);
                         mm::tma_load_2d(as + HALF, &tx, k, row, bar);
                         mm::tma_load_2d(as + HALF + BOX_MN, &tx, k + 64, row, bar);
                     }
                     __syncwarp();
-                    ok = tc::mbar_wait(ragged, (uint32_t)(nragged++ & 1));
+                    ok = tc::mbar_wait(p.ragged, ragged_phase);
+                    ragged_phase ^= 1;
                     if (!__all_sync(~0u, ok)) {
                         *p.err = 1;
                         ok = false;
@@ -358,38 +390,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                         *reinterpret_cast<int4*>(st + (lane >> 3) * BOX_MN + r * 128 + (lane & 7) * 16) = make_int4(0, 0, 0, 0);
                     tc::fence_async_smem();
                     __syncwarp();
-                    if (lane == 0) arrive_cluster(p.full0 + s * 8);
+                    // the leader hands the stage over when both halves are zeroed (an arrival of the second CTA on full[s]
+                    // for every stage cost more than the products).  One barrier per stage: the other CTA may be several
+                    // ragged stages ahead, but not past a stage that the leader has not handed over
+                    if (p.rank != 0) {
+                        if (lane == 0) arrive_cluster(p.zeroed0 + s * 8);
+                    } else {
+                        ok = wait_cluster(&p.zeroed[s], (zeroed_phases >> s) & 1);
+                        zeroed_phases ^= 1u << s;
+                        if (!__all_sync(~0u, ok)) {
+                            *p.err = 1;
+                            ok = false;
+                            break;
+                        }
+                        if (lane == 0) tc::mbar_arrive(&p.full[s]);
+                    }
                 }
             }
         }
         if (lane == 0) finish_copies(p, i);
     } else if (warp == 9) {
-        if (lane == 0 && p.rank == 0) {
-            int i = 0, j = 0;   // stages and accumulators over all tiles
+        if (p.rank == 0) {
+            const bool one = elect();
+            const uint64_t a0 = sdesc<true>(tc::smem_u32(p.sm)), b0 = sdesc<true>(tc::smem_u32(p.sm) + HALF);
+            int s = 0, j = 0;   // stage, accumulators over all tiles
+            uint32_t phase = 0;
             for (long long t = blockIdx.x / 2; t < tiles && !*p.err; t += pairs) {
                 const Tile d = tile_at(t);
                 const uint32_t id = idesc_f16(2 * FT, d.cols, a.bf16, true, true);
-                for (int c = 0; c < d.nb; ++c, ++i) {
-                    const int s = i % STAGES, b = j & 1;
-                    if (c % DRAIN == 0) {
-                        if (j >= 2 && !tc::mbar_wait(&p.tempty[b], (uint32_t)((j / 2 - 1) & 1))) *p.err = 1;
-                        tc::fence_after_sync();
-                    }
-                    if (*p.err || !tc::mbar_wait(&p.full[s], (uint32_t)((i / STAGES) & 1))) {
-                        *p.err = 1;
-                        break;
-                    }
+                for (int c0 = 0; c0 < d.nb; c0 += DRAIN<OUT>, ++j) {
+                    const int b = j & 1, c1 = min(c0 + DRAIN<OUT>, d.nb);
+                    const uint32_t acc = p.tmem + b * NT;
+                    if (j >= 2 && !tc::mbar_wait(&p.tempty[b], (uint32_t)((j / 2 - 1) & 1))) *p.err = 1;
                     tc::fence_after_sync();
-                    const uint32_t as = tc::smem_u32(p.sm) + s * STAGE, bs = as + HALF, acc = p.tmem + b * NT;
-                    const int steps = min(BK, d.rows - c * BK + 15) / 16;
-                    for (int q = 0; q < steps; ++q)
-                        mma2_f16(acc, sdesc<true>(as + q * kstep<true>()), sdesc<true>(bs + q * kstep<true>()), id,
-                                 c % DRAIN > 0 || q > 0);
-                    commit2(&p.empty[s]);
-                    if (c % DRAIN == DRAIN - 1 || c == d.nb - 1) {
-                        commit2(&p.tfull[b]);
-                        ++j;
+                    for (int c = c0; c < c1; ++c) {
+                        if (*p.err || !tc::mbar_wait(&p.full[s], phase)) {
+                            *p.err = 1;
+                            break;
+                        }
+                        tc::fence_after_sync();
+                        const int left = d.rows - c * BK;
+                        if (one) {
+#pragma unroll
+                            for (int q = 0; q < BK / 16; ++q)
+                                if (q * 16 < left)
+                                    mma2_f16(acc, a0 + ((s * STAGE + q * kstep<true>()) >> 4), b0 + ((s * STAGE + q * kstep<true>()) >> 4),
+                                             id, c > c0 || q > 0);
+                            commit2(&p.empty[s]);
+                        }
+                        if (++s == STAGES) s = 0, phase ^= 1;
                     }
+                    if (one) commit2(&p.tfull[b]);
                 }
             }
         }
@@ -402,7 +453,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             float sum[NT / 2];
 #pragma unroll
             for (int c = 0; c < NT / 2; ++c) sum[c] = 0.f;
-            for (int c = 0; c < d.nb; c += DRAIN, ++j) {
+            for (int c = 0; c < d.nb; c += DRAIN<OUT>, ++j) {
                 const int b = j & 1;
                 ok = !*p.err && tc::mbar_wait(&p.tfull[b], (uint32_t)((j / 2) & 1));
                 if (!__all_sync(~0u, ok)) {

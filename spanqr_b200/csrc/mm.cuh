@@ -51,6 +51,17 @@ __device__ __forceinline__ uint64_t sdesc(uint32_t saddr) {
 template <bool MN>
 __device__ __forceinline__ constexpr uint32_t kstep() { return MN ? 2048u : 32u; }
 
+// one thread of a whole warp, the same each time
+__device__ __forceinline__ bool elect() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
+}
+
 __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const void* map, int c0, int c1, int c2, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"

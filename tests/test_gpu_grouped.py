@@ -84,6 +84,18 @@ def test_wgrad_exact(T, E, N, K, dtype, out):
     assert torch.equal(mm_grouped_wgrad(dy, x, off, dtype=out), exact_wgrad(dy, x, off).to(out))
 
 
+@pytest.mark.parametrize("T,E,N,K", [(6000, 300, 64, 64), (12000, 600, 40, 72), (20000, 1024, 64, 256), (9000, 150, 300, 520)])
+def test_many_small_ragged_experts(T, E, N, K):
+    """one CTA pair after another takes experts whose few rows end inside a product's 16: its two CTAs run apart by
+    several such tiles"""
+    dy, x, w = ints((T, N), 1, BF16), ints((T, K), 2, BF16), ints((E, N, K), 3, BF16)
+    g = torch.Generator().manual_seed(T)
+    off = offsets(torch.bincount(torch.randint(0, E, (T,), generator=g), minlength=E).tolist())
+    for _ in range(3):
+        assert torch.equal(mm_grouped_wgrad(dy, x, off), exact_wgrad(dy, x, off).to(F32))
+    assert torch.equal(mm_grouped(x, w, off), exact_mm(x, w, off).to(BF16))
+
+
 @pytest.mark.parametrize("T,E,N,K", [(24, 8, 512, 2048), (700, 16, 384, 1024), (3000, 4, 640, 4096), (5000, 3, 256, 17408)])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 def test_product_gaussian(T, E, N, K, dtype):
