@@ -20,7 +20,11 @@ namespace {
 
 using namespace mm;
 
-constexpr int THREADS = 320;       // warps 0-7: epilogue (TMEM lanes 32 (w % 4) .., columns by w / 4), 8: copies, 9: products
+// warps 0-7: epilogue (TMEM lanes 32 (w % 4) .., columns by w / 4), 8 and 9: copies of A and of B, 10: products.  The issue
+// of the copies is on the critical path (a stage lasts 512 cycles): one warp for both operands held the weight gradient
+// to 1340 TFLOP/s where two give 1500 (16384 rows, 8 experts of 5120x2048, bf16).
+constexpr int THREADS = 352;
+constexpr int COPY_A = 8, COPY_B = 9, PRODUCTS = 10;
 constexpr int STAGES = 6;
 constexpr int HALF = FT * BK * 2;  // one operand half: 128 x 64 elements, 16 KB
 constexpr int STAGE = 2 * HALF;
@@ -124,7 +128,7 @@ __device__ __forceinline__ Pair set_up(char* dyn, const int* offsets, int E, int
     p.rank = (int)cluster_rank();
     const int warp = threadIdx.x >> 5;
     if (warp == 0) map_groups(offsets, E, T, rows_per_tile, p.start, p.pre);
-    if (warp == 9) tmem_alloc2(slot, 2 * NT);
+    if (warp == PRODUCTS) tmem_alloc2(slot, 2 * NT);
     if (threadIdx.x == 256) {
         for (int s = 0; s < STAGES; ++s) {
             tc::mbar_init(&p.full[s], 1);
@@ -155,24 +159,37 @@ __device__ __forceinline__ void tear_down(const Pair& p, int* status) {
     __syncwarp();
     tc::fence_before_sync();
     cluster_sync_all();
-    if ((threadIdx.x >> 5) == 9) tmem_dealloc2(p.tmem, 2 * NT);
+    if ((threadIdx.x >> 5) == PRODUCTS) tmem_dealloc2(p.tmem, 2 * NT);
     if (threadIdx.x == 0 && *p.err) atomicOr(status, MM_TIMEOUT);
 }
 
-// the wait for stage i to be free (true), or a limit that ran out
-__device__ __forceinline__ bool stage_free(const Pair& p, int i) {
-    if (i < STAGES) return true;
-    if (!*p.err && tc::mbar_wait(&p.empty[i % STAGES], (uint32_t)((i / STAGES - 1) & 1))) return true;
+// a role's place in the ring of stages
+struct Ring {
+    int s = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++s == STAGES) {
+            s = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+// the wait for the ring's stage to be free (a barrier's first wait, for the phase before its first, returns at once)
+__device__ __forceinline__ bool stage_free(const Pair& p, const Ring& r) {
+    if (!*p.err && tc::mbar_wait(&p.empty[r.s], r.phase ^ 1)) return true;
     *p.err = 1;
     return false;
 }
-// the end of the copies, after i stages: the products have released the last ones (so no signal is on its way to a
-// barrier of a CTA that is gone), or, after a limit ran out, the leader has seen both CTAs' copies arrive
-__device__ __forceinline__ void finish_copies(const Pair& p, int i) {
-    const bool failed = *p.err;
-    if (failed && p.rank != 0) return;
-    for (int j = max(0, i - STAGES); j < i; ++j)
-        if (!tc::mbar_wait(failed ? &p.full[j % STAGES] : &p.empty[j % STAGES], (uint32_t)((j / STAGES) & 1))) *p.err = 1;
+// the end of the copies: the products have released every stage (so no signal is on its way to a barrier of a CTA that
+// is gone), or, after a limit ran out, the leader has seen both CTAs' copies arrive
+__device__ __forceinline__ void finish_copies(const Pair& p, Ring r) {
+    if (!*p.err) {
+        for (int n = 0; n < STAGES; ++n, r.next())
+            if (!tc::mbar_wait(&p.empty[r.s], r.phase ^ 1)) *p.err = 1;
+    } else if (p.rank == 0) {
+        for (int s = 0; s < STAGES; ++s) tc::mbar_wait(&p.full[s], s < r.s ? r.phase : r.phase ^ 1);
+    }
 }
 
 __device__ __forceinline__ int up32(int n) { return (n + 31) & ~31; }
@@ -199,39 +216,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         return t;
     };
 
-    if (warp == 8) {
-        if (lane == 0) {
-            prefetch_map(&tw);
-            prefetch_map(&tx);
-            int i = 0;
-            bool ok = true;
-            for (int t = (int)blockIdx.x / 2; ok && t < tiles; t += pairs) {
-                const Tile d = tile_at(t);
-                const int n = d.n0 + p.rank * FT, r = d.t0 + p.rank * (d.cols / 2);
-                for (int k = 0; k < kb; ++k, ++i) {
-                    if (!(ok = stage_free(p, i))) break;
-                    const int s = i % STAGES;
-                    const uint32_t as = tc::smem_u32(p.sm) + s * STAGE, bar = p.full0 + s * 8;
-                    if (p.rank == 0) tc::mbar_expect_tx(&p.full[s], 2 * STAGE);
+    // the copy and product warps run their loops whole (their state stays in uniform registers, which TMA and tcgen05
+    // operands need); one thread issues
+    if (warp == COPY_A) {
+        const bool one = elect();
+        Ring r;
+        bool ok = true;
+        for (int t = (int)blockIdx.x / 2; ok && t < tiles; t += pairs) {
+            const Tile d = tile_at(t);
+            const int n = d.n0 + p.rank * FT;
+            for (int k = 0; k < kb; ++k, r.next()) {
+                if (!(ok = __all_sync(~0u, stage_free(p, r)))) break;
+                if (one) {
+                    const uint32_t as = tc::smem_u32(p.sm) + r.s * STAGE, bar = p.full0 + r.s * 8;
+                    if (p.rank == 0) tc::mbar_expect_tx(&p.full[r.s], 2 * STAGE);
                     if (W_MN) {
                         tma2_load_3d(as, &tw, n, k * BK, d.e, bar);
                         tma2_load_3d(as + BOX_MN, &tw, n + 64, k * BK, d.e, bar);
                     } else {
                         tma2_load_3d(as, &tw, k * BK, n, d.e, bar);
                     }
-                    tma2_load_2d(as + HALF, &tx, k * BK, r, bar);
                 }
+                __syncwarp();
             }
-            finish_copies(p, i);
         }
-    } else if (warp == 9) {
-        // the whole warp runs the loop (its state stays in uniform registers, which the products' operands need), one
-        // thread issues
+        finish_copies(p, r);
+    } else if (warp == COPY_B) {
+        const bool one = elect();
+        Ring r;
+        bool ok = true;
+        for (int t = (int)blockIdx.x / 2; ok && t < tiles; t += pairs) {
+            const Tile d = tile_at(t);
+            const int row = d.t0 + p.rank * (d.cols / 2);
+            for (int k = 0; k < kb; ++k, r.next()) {
+                if (!(ok = __all_sync(~0u, stage_free(p, r)))) break;
+                if (one)
+                    tma2_load_2d(tc::smem_u32(p.sm) + r.s * STAGE + HALF, &tx, k * BK, row, p.full0 + r.s * 8);
+                __syncwarp();
+            }
+        }
+    } else if (warp == PRODUCTS) {
         if (p.rank == 0) {
             const bool one = elect();
             const uint64_t a0 = sdesc<W_MN>(tc::smem_u32(p.sm)), b0 = sdesc<false>(tc::smem_u32(p.sm) + HALF);
-            int s = 0, j = 0;
-            uint32_t phase = 0;
+            Ring r;
+            int j = 0;
             for (int t = (int)blockIdx.x / 2; t < tiles && !*p.err; t += pairs, ++j) {
                 const Tile d = tile_at(t);
                 const int b = j & 1;
@@ -239,7 +268,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 if (j >= 2 && !tc::mbar_wait(&p.tempty[b], (uint32_t)((j / 2 - 1) & 1))) *p.err = 1;
                 tc::fence_after_sync();
                 for (int k = 0; k < kb; ++k) {
-                    if (*p.err || !tc::mbar_wait(&p.full[s], phase)) {
+                    if (*p.err || !tc::mbar_wait(&p.full[r.s], r.phase)) {
                         *p.err = 1;
                         break;
                     }
@@ -247,11 +276,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     if (one) {
 #pragma unroll
                         for (int q = 0; q < BK / 16; ++q)
-                            mma2_f16(acc, a0 + ((s * STAGE + q * kstep<W_MN>()) >> 4), b0 + ((s * STAGE + q * kstep<false>()) >> 4),
+                            mma2_f16(acc, a0 + ((r.s * STAGE + q * kstep<W_MN>()) >> 4), b0 + ((r.s * STAGE + q * kstep<false>()) >> 4),
                                      id, k > 0 || q > 0);
-                        commit2(&p.empty[s]);
+                        commit2(&p.empty[r.s]);
                     }
-                    if (++s == STAGES) s = 0, phase ^= 1;
+                    r.next();
                 }
                 if (one) commit2(&p.tfull[b]);
             }
@@ -310,6 +339,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tear_down(p, a.status);
 }
 
+// whether a stage with `left` rows of its expert ends inside one product's 16
+__device__ __forceinline__ bool ragged(int left) { return left < BK && left % 16 != 0; }
+
 // The tensor core rounds toward zero each time it adds 16 products to its fp32 accumulator: over n additions of terms of
 // random sign the sum comes out about n * 3e-8 of itself too small.  So the accumulator is taken every DRAIN stages and
 // added to fp32 sums in registers, rounded to nearest, while the products go on in the other accumulator.  For fp32
@@ -341,80 +373,89 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         return t;
     };
 
-    if (warp == 8) {
-        int i = 0;
+    if (warp == COPY_A) {
+        const bool one = elect();
+        Ring r;
         uint32_t ragged_phase = 0, zeroed_phases = 0;   // (bit s: that of zeroed[s])
         bool ok = true;
         for (long long t = blockIdx.x / 2; ok && t < tiles; t += pairs) {
             const Tile d = tile_at(t);
             const int n = d.n0 + p.rank * FT, k = d.k0 + p.rank * (d.cols / 2);
-            for (int c = 0; c < d.nb; ++c, ++i) {
-                ok = stage_free(p, i);   // every lane: the warp leaves together
-                if (!__all_sync(~0u, ok)) {
-                    ok = false;
-                    break;
-                }
-                const int s = i % STAGES, left = d.rows - c * BK, row = d.r0 + c * BK;
-                const uint32_t as = tc::smem_u32(p.sm) + s * STAGE;
-                if (left >= BK || left % 16 == 0) {
-                    if (lane == 0) {
-                        const uint32_t bar = p.full0 + s * 8;
-                        if (p.rank == 0) tc::mbar_expect_tx(&p.full[s], 2 * STAGE);
+            for (int c = 0; c < d.nb; ++c, r.next()) {
+                if (!(ok = __all_sync(~0u, stage_free(p, r)))) break;
+                const int left = d.rows - c * BK, row = d.r0 + c * BK;
+                const uint32_t as = tc::smem_u32(p.sm) + r.s * STAGE;
+                if (!ragged(left)) {
+                    if (one) {
+                        const uint32_t bar = p.full0 + r.s * 8;
+                        if (p.rank == 0) tc::mbar_expect_tx(&p.full[r.s], 2 * STAGE);
                         tma2_load_2d(as, &tdy, n, row, bar);
                         tma2_load_2d(as + BOX_MN, &tdy, n + 64, row, bar);
-                        tma2_load_2d(as + HALF, &tx, k, row, bar);
-                        tma2_load_2d(as + HALF + BOX_MN, &tx, k + 64, row, bar);
-                    }
-                } else {
-                    // the expert's last rows, not a multiple of one product's 16: the rows behind them (another expert's)
-                    // are zeroed in both operands before the products may read the stage
-                    if (lane == 0) {
-                        const uint32_t bar = tc::smem_u32(p.ragged);
-                        tc::mbar_expect_tx(p.ragged, STAGE);
-                        mm::tma_load_2d(as, &tdy, n, row, bar);
-                        mm::tma_load_2d(as + BOX_MN, &tdy, n + 64, row, bar);
-                        mm::tma_load_2d(as + HALF, &tx, k, row, bar);
-                        mm::tma_load_2d(as + HALF + BOX_MN, &tx, k + 64, row, bar);
                     }
                     __syncwarp();
-                    ok = tc::mbar_wait(p.ragged, ragged_phase);
-                    ragged_phase ^= 1;
-                    if (!__all_sync(~0u, ok)) {
-                        *p.err = 1;
-                        ok = false;
-                        break;
-                    }
-                    char* const st = p.sm + s * STAGE;
-                    const int upto = (left + 15) & ~15;   // box lane / 8, 16 bytes (lane % 8) of each row
-                    for (int r = left; r < upto; ++r)
-                        *reinterpret_cast<int4*>(st + (lane >> 3) * BOX_MN + r * 128 + (lane & 7) * 16) = make_int4(0, 0, 0, 0);
+                    continue;
+                }
+                // the expert's last rows, not a multiple of one product's 16: the rows behind them (another expert's) are
+                // zeroed in both operands before the products may read the stage
+                if (one) {
+                    const uint32_t bar = tc::smem_u32(p.ragged);
+                    tc::mbar_expect_tx(p.ragged, STAGE);
+                    mm::tma_load_2d(as, &tdy, n, row, bar);
+                    mm::tma_load_2d(as + BOX_MN, &tdy, n + 64, row, bar);
+                    mm::tma_load_2d(as + HALF, &tx, k, row, bar);
+                    mm::tma_load_2d(as + HALF + BOX_MN, &tx, k + 64, row, bar);
+                }
+                __syncwarp();
+                ok = __all_sync(~0u, tc::mbar_wait(p.ragged, ragged_phase));
+                ragged_phase ^= 1;
+                if (ok) {
+                    char* const st = p.sm + r.s * STAGE;   // box lane / 8, 16 bytes (lane % 8) of each row
+                    for (int x = left; x < ((left + 15) & ~15); ++x)
+                        *reinterpret_cast<int4*>(st + (lane >> 3) * BOX_MN + x * 128 + (lane & 7) * 16) = make_int4(0, 0, 0, 0);
                     tc::fence_async_smem();
                     __syncwarp();
                     // the leader hands the stage over when both halves are zeroed (an arrival of the second CTA on full[s]
                     // for every stage cost more than the products).  One barrier per stage: the other CTA may be several
                     // ragged stages ahead, but not past a stage that the leader has not handed over
                     if (p.rank != 0) {
-                        if (lane == 0) arrive_cluster(p.zeroed0 + s * 8);
+                        if (one) arrive_cluster(p.zeroed0 + r.s * 8);
                     } else {
-                        ok = wait_cluster(&p.zeroed[s], (zeroed_phases >> s) & 1);
-                        zeroed_phases ^= 1u << s;
-                        if (!__all_sync(~0u, ok)) {
-                            *p.err = 1;
-                            ok = false;
-                            break;
-                        }
-                        if (lane == 0) tc::mbar_arrive(&p.full[s]);
+                        ok = __all_sync(~0u, wait_cluster(&p.zeroed[r.s], (zeroed_phases >> r.s) & 1));
+                        zeroed_phases ^= 1u << r.s;
+                        if (ok && one) tc::mbar_arrive(&p.full[r.s]);
                     }
                 }
+                if (!ok) {
+                    *p.err = 1;
+                    break;
+                }
+                __syncwarp();
             }
         }
-        if (lane == 0) finish_copies(p, i);
-    } else if (warp == 9) {
+        finish_copies(p, r);
+    } else if (warp == COPY_B) {
+        const bool one = elect();
+        Ring r;
+        bool ok = true;
+        for (long long t = blockIdx.x / 2; ok && t < tiles; t += pairs) {
+            const Tile d = tile_at(t);
+            const int k = d.k0 + p.rank * (d.cols / 2);
+            for (int c = 0; c < d.nb; ++c, r.next()) {
+                if (!(ok = __all_sync(~0u, stage_free(p, r)))) break;
+                if (one && !ragged(d.rows - c * BK)) {
+                    const uint32_t bs = tc::smem_u32(p.sm) + r.s * STAGE + HALF, bar = p.full0 + r.s * 8;
+                    tma2_load_2d(bs, &tx, k, d.r0 + c * BK, bar);
+                    tma2_load_2d(bs + BOX_MN, &tx, k + 64, d.r0 + c * BK, bar);
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == PRODUCTS) {
         if (p.rank == 0) {
             const bool one = elect();
             const uint64_t a0 = sdesc<true>(tc::smem_u32(p.sm)), b0 = sdesc<true>(tc::smem_u32(p.sm) + HALF);
-            int s = 0, j = 0;   // stage, accumulators over all tiles
-            uint32_t phase = 0;
+            Ring r;
+            int j = 0;   // accumulators over all tiles
             for (long long t = blockIdx.x / 2; t < tiles && !*p.err; t += pairs) {
                 const Tile d = tile_at(t);
                 const uint32_t id = idesc_f16(2 * FT, d.cols, a.bf16, true, true);
@@ -424,7 +465,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     if (j >= 2 && !tc::mbar_wait(&p.tempty[b], (uint32_t)((j / 2 - 1) & 1))) *p.err = 1;
                     tc::fence_after_sync();
                     for (int c = c0; c < c1; ++c) {
-                        if (*p.err || !tc::mbar_wait(&p.full[s], phase)) {
+                        if (*p.err || !tc::mbar_wait(&p.full[r.s], r.phase)) {
                             *p.err = 1;
                             break;
                         }
@@ -434,11 +475,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 #pragma unroll
                             for (int q = 0; q < BK / 16; ++q)
                                 if (q * 16 < left)
-                                    mma2_f16(acc, a0 + ((s * STAGE + q * kstep<true>()) >> 4), b0 + ((s * STAGE + q * kstep<true>()) >> 4),
+                                    mma2_f16(acc, a0 + ((r.s * STAGE + q * kstep<true>()) >> 4), b0 + ((r.s * STAGE + q * kstep<true>()) >> 4),
                                              id, c > c0 || q > 0);
-                            commit2(&p.empty[s]);
+                            commit2(&p.empty[r.s]);
                         }
-                        if (++s == STAGES) s = 0, phase ^= 1;
+                        r.next();
                     }
                     if (one) commit2(&p.tfull[b]);
                 }
