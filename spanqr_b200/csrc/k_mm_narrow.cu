@@ -199,8 +199,8 @@ cudaError_t launch(const CUtensorMap& tw, const CUtensorMap& tx, const MmArgs& a
 template <int TN>
 cudaError_t run(const MmOperand& x, const MmOperand& w, MmArgs a, cudaStream_t st) {
     alignas(64) CUtensorMap tw, tx;
-    cudaError_t e = encode_mm(&tx, x, a.bf16, BK, TN);
-    if (e == cudaSuccess) e = w.mn ? encode_mm(&tw, w, a.bf16, 64, BK) : encode_mm(&tw, w, a.bf16, BK, FT);
+    cudaError_t e = encode_mm(&tx, x, a.type(), BK, TN);
+    if (e == cudaSuccess) e = w.mn ? encode_mm(&tw, w, a.type(), 64, BK) : encode_mm(&tw, w, a.type(), BK, FT);
     int nsm = 0;
     if (e == cudaSuccess) e = sm_count(&nsm);
     if (e != cudaSuccess) return e;

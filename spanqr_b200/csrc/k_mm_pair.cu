@@ -6,7 +6,7 @@
 //
 // One tcgen05.mma.cta_group::2 works on both SMs of a pair (a cluster of two CTAs): each CTA holds the accumulators of
 // 128 of the 256 features, its own half of A and half of B, so a 64-element stage costs each SM 32 KB of shared memory
-// and of L2 traffic for 512 cycles of products; a 128 x 256 tile on one SM would need 48 KB.  Six stages in flight, two
+// and of L2 traffic for 512 cycles of products; a 128 x 256 tile on one SM would need 48 KB.  Five stages in flight, two
 // accumulators of 256 TMEM columns: the epilogue of one tile overlaps the products of the next.  The grid is one pair
 // per two SMs, each pair taking tiles in turn; the pipeline runs on from tile to tile.
 //
@@ -25,11 +25,12 @@ using namespace mm;
 // to 1340 TFLOP/s where two give 1500 (16384 rows, 8 experts of 5120x2048, bf16).
 constexpr int THREADS = 352;
 constexpr int COPY_A = 8, COPY_B = 9, PRODUCTS = 10;
-constexpr int STAGES = 6;
+constexpr int STAGES = 5;           // (four cost up to 7 %, six gave no more)
 constexpr int HALF = FT * BK * 2;  // one operand half: 128 x 64 elements, 16 KB
 constexpr int STAGE = 2 * HALF;
 constexpr int NT = 256;            // columns of a tile
-constexpr int BARS = STAGES * STAGE;
+constexpr int STAGING = STAGES * STAGE;       // wgrad: 32 rows x 128 bytes of results per epilogue warp
+constexpr int BARS = STAGING + 8 * 4096;
 constexpr int MAPS = BARS + 256;
 constexpr int FIXED = MAPS + 16 + 1024;
 // wgrad: stages (of 64 rows) summed in TMEM before they are added in registers
@@ -79,6 +80,15 @@ __device__ __forceinline__ void tma2_load_2d(uint32_t smem_dst, const void* map,
         "l"(map), "r"(c0), "r"(c1), "r"(bar)
         : "memory");
 }
+// a tile of 32 rows x 128 bytes to global memory, one bulk group each
+__device__ __forceinline__ void tma_store_3d(const void* map, int c0, int c1, int c2, uint32_t smem_src) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(c0),
+                 "r"(c1), "r"(c2), "r"(smem_src)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -339,6 +349,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tear_down(p, a.status);
 }
 
+__device__ __forceinline__ void st_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// a warp's staged results to rows of dw that do not start on 16 bytes
+template <typename OUT>
+__device__ __forceinline__ void store_rows(const char* stage, OUT* row, int ld, int rows, int cols) {
+#pragma unroll 1
+    for (int x = 0; x < rows; ++x, row += ld)
+#pragma unroll 1
+        for (int y = threadIdx.x & 31; y < cols; y += 32) {
+            const int at = y * (int)sizeof(OUT);
+            row[y] = *reinterpret_cast<const OUT*>(stage + x * 128 + (((at >> 4) ^ (x & 7)) << 4) + (at & 15));
+        }
+    __syncwarp();
+}
+
 // whether a stage with `left` rows of its expert ends inside one product's 16
 __device__ __forceinline__ bool ragged(int left) { return left < BK && left % 16 != 0; }
 
@@ -348,9 +375,10 @@ __device__ __forceinline__ bool ragged(int left) { return left < BK && left % 16
 // results every 512 rows (measured 4e-7 off in all at 5000 rows, as a sum in fp32 is); for 16-bit results, whose own
 // rounding is 2^-9 or 2^-12, every 2048, which keeps the bias from growing with the length.  The reads of TMEM
 // take tensor-core time: 16384 rows, 8 experts of 5120x2048 in bf16: 285 us with a drain every 256 rows, 258 every 512, 252 every 4096.
-template <typename OUT>
+template <typename OUT, bool TMA_OUT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
-    k_mm_wgrad(const __grid_constant__ CUtensorMap tdy, const __grid_constant__ CUtensorMap tx, const MmWgradArgs a) {
+    k_mm_wgrad(const __grid_constant__ CUtensorMap tdy, const __grid_constant__ CUtensorMap tx,
+               const __grid_constant__ CUtensorMap tdw, const MmWgradArgs a) {
     extern __shared__ char dyn[];
     const Pair p = set_up(dyn, a.offsets, a.E, a.T, 1 << 30);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -486,7 +514,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             }
         }
     } else {
+        constexpr int COLS = 128 / sizeof(OUT);
         const int q = warp & 3, half = warp >> 2;
+        const bool one = elect();
+        char* const stage = p.sm + STAGING + warp * 4096;
         int j = 0;
         bool ok = true;
         for (long long t = blockIdx.x / 2; ok && t < tiles; t += pairs) {
@@ -519,33 +550,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 if (lane == 0) arrive_cluster(p.tempty0 + b * 8);
             }
             if (!ok) break;
-            const int n = d.n0 + p.rank * FT + q * 32 + lane, k = d.k0 + half * (NT / 2);
-            OUT* const row = static_cast<OUT*>(a.dw) + ((long long)d.e * a.N + n) * a.K + k;
-            constexpr int PER = 32 / sizeof(OUT);
-            const bool whole = (reinterpret_cast<uintptr_t>(row) & 31) == 0;
-            const int K = n < a.N ? a.K : 0;   // a lane without a feature stores nothing
+            // 32 rows x 128 bytes at a time through shared memory (in the swizzled layout, so that the lanes' rows meet no
+            // bank twice), then one TMA store: lanes that write their own rows to memory touch 32 lines per instruction,
+            // which took longer than the products (16 experts of 2048x5120 in fp32: 328 us so)
+            const int n = d.n0 + p.rank * FT + q * 32, k = d.k0 + half * (NT / 2);
+            const uint32_t mine = tc::smem_u32(stage) + lane * 128;
 #pragma unroll
-            for (int c = 0; c < NT / 2; c += PER) {
-                if (whole && k + c + PER <= K) {
-                    float w[8];
+            for (int c = 0; c < NT / 2; c += COLS) {
+                if (n < a.N && k + c < a.K) {
+                    if (one) bulk_wait_read();
+                    __syncwarp();
 #pragma unroll
                     for (int x = 0; x < 8; ++x) {
-                        if constexpr (sizeof(OUT) == 4) w[x] = sum[c + x];
-                        else w[x] = __uint_as_float(pack16(sum[c + 2 * x], sum[c + 2 * x + 1], a.bf16));
-                    }
-                    tc::st8(reinterpret_cast<float*>(row + c), w);
-                } else {
-#pragma unroll
-                    for (int x = 0; x < PER; ++x) {
-                        if (k + c + x < K) {
-                            if constexpr (sizeof(OUT) == 4) row[c + x] = sum[c + x];
-                            else row[c + x] = to16(sum[c + x], a.bf16);
+                        const uint32_t at = mine + ((x ^ (lane & 7)) << 4);
+                        if constexpr (sizeof(OUT) == 4) {
+                            const float* v = sum + c + 4 * x;
+                            st_shared16(at, __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                        } else {
+                            const float* v = sum + c + 8 * x;
+                            st_shared16(at, pack16(v[0], v[1], a.bf16), pack16(v[2], v[3], a.bf16), pack16(v[4], v[5], a.bf16),
+                                        pack16(v[6], v[7], a.bf16));
                         }
+                    }
+                    if (TMA_OUT) {
+                        tc::fence_async_smem();
+                        __syncwarp();
+                        if (one) tma_store_3d(&tdw, k + c, n, d.e, tc::smem_u32(stage));
+                    } else {
+                        __syncwarp();
+                        store_rows(stage, static_cast<OUT*>(a.dw) + ((long long)d.e * a.N + n) * a.K + k + c, a.K,
+                                   min(32, a.N - n), min(COLS, a.K - k - c));
                     }
                 }
             }
-            __syncwarp();
         }
+        if (one) bulk_wait();   // the last results have left shared memory before it goes
     }
     tear_down(p, a.status);
 }
@@ -568,8 +607,8 @@ cudaError_t launch_mm_wide(const MmOperand& x, const MmOperand& w, const MmArgs&
     MmArgs a = args;
     a.ntn = (a.N + 2 * FT - 1) / (2 * FT);
     alignas(64) CUtensorMap tw, tx;
-    cudaError_t e = encode_mm(&tx, x, a.bf16, BK, FT);
-    if (e == cudaSuccess) e = w.mn ? encode_mm(&tw, w, a.bf16, 64, BK) : encode_mm(&tw, w, a.bf16, BK, FT);
+    cudaError_t e = encode_mm(&tx, x, a.type(), BK, FT);
+    if (e == cudaSuccess) e = w.mn ? encode_mm(&tw, w, a.type(), 64, BK) : encode_mm(&tw, w, a.type(), BK, FT);
     if (e != cudaSuccess) return e;
     const long long tiles = ((long long)(a.T / NT) + (a.T < a.E ? a.T : a.E)) * a.ntn;   // the most the offsets could give
     if (tiles > (1LL << 30)) return cudaErrorInvalidValue;
@@ -577,12 +616,21 @@ cudaError_t launch_mm_wide(const MmOperand& x, const MmOperand& w, const MmArgs&
 }
 
 cudaError_t launch_mm_wgrad(const MmOperand& dy, const MmOperand& x, const MmWgradArgs& a, cudaStream_t st) {
-    alignas(64) CUtensorMap tdy, tx;
-    cudaError_t e = encode_mm(&tdy, dy, a.bf16, 64, BK);
-    if (e == cudaSuccess) e = encode_mm(&tx, x, a.bf16, 64, BK);
+    const int size = a.out32 ? 4 : 2;
+    const bool rows16 = reinterpret_cast<uintptr_t>(a.dw) % 16 == 0 && (long long)a.K * size % 16 == 0;
+    alignas(64) CUtensorMap tdy, tx, tdw{};
+    cudaError_t e = encode_mm(&tdy, dy, a.type(), 64, BK);
+    if (e == cudaSuccess) e = encode_mm(&tx, x, a.type(), 64, BK);
+    if (e == cudaSuccess && rows16)
+        e = encode_mm(&tdw, MmOperand{a.dw, a.K, a.N, a.K, a.E, (long long)a.N * a.K, false}, a.out32 ? DT_F32 : a.type(),
+                      128 / size, 32);
     if (e != cudaSuccess) return e;
     const long long tiles = (long long)a.E * ((a.N + 2 * FT - 1) / (2 * FT)) * ((a.K + NT - 1) / NT);
-    return a.out32 ? go(k_mm_wgrad<float>, tiles, a.E, st, tdy, tx, a) : go(k_mm_wgrad<uint16_t>, tiles, a.E, st, tdy, tx, a);
+    if (rows16)
+        return a.out32 ? go(k_mm_wgrad<float, true>, tiles, a.E, st, tdy, tx, tdw, a)
+                       : go(k_mm_wgrad<uint16_t, true>, tiles, a.E, st, tdy, tx, tdw, a);
+    return a.out32 ? go(k_mm_wgrad<float, false>, tiles, a.E, st, tdy, tx, tdw, a)
+                   : go(k_mm_wgrad<uint16_t, false>, tiles, a.E, st, tdy, tx, tdw, a);
 }
 
 }  // namespace spq

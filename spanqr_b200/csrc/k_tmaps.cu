@@ -40,14 +40,16 @@ cudaError_t encode_rows(CUtensorMap* m, const void* base, int rows, int cols, lo
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-cudaError_t encode_mm(CUtensorMap* m, const MmOperand& o, bool bf16, int box_cols, int box_rows) {
+cudaError_t encode_mm(CUtensorMap* m, const MmOperand& o, DType type, int box_cols, int box_rows) {
     cudaError_t e = encoder();
     if (e != cudaSuccess) return e;
     const cuuint64_t dims[3] = {(cuuint64_t)o.cols, (cuuint64_t)o.rows, (cuuint64_t)o.planes};
-    const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)o.plane * 2};
+    const cuuint64_t size = type == DT_F32 ? 4 : 2, strides[2] = {(cuuint64_t)o.ld * size, (cuuint64_t)o.plane * size};
     const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
     const cuuint32_t es[3] = {1, 1, 1};
-    const CUresult r = g_encode(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+    const CUresult r = g_encode(m, type == DT_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : type == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                                 o.planes > 0 ? 3 : 2, const_cast<void*>(o.p), dims, strides, box, es,
                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

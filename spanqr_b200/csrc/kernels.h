@@ -164,8 +164,8 @@ cudaError_t launch_grad_scale(const GradEntry* e, int count, const double* part,
                               cudaStream_t st);
 
 // ---- products grouped by expert ----
-// A 16-bit operand: `rows` rows of `cols` contiguous elements, `ld` elements apart (a multiple of 8), in `planes` planes
-// `plane` elements apart (0 planes: a plain matrix), 16-byte aligned.  mn: the contracted dimension runs along the rows.
+// An operand: `rows` rows of `cols` contiguous elements, `ld` elements apart, in `planes` planes `plane` elements apart (0
+// planes: a plain matrix), every row 16-byte aligned.  mn: the contracted dimension runs along the rows.
 struct MmOperand {
     const void* p;
     long long cols, rows, ld;
@@ -180,12 +180,14 @@ struct MmArgs {
     long long ldy;
     int ntn;              // feature tiles of 128
     bool bf16;            // bf16, else fp16
+    DType type() const { return bf16 ? DT_BF16 : DT_F16; }
     bool zero_tail;       // zero the rows behind the last expert (else they are left as they are)
     int* status;          // a bounded wait that runs out ORs MM_TIMEOUT
 };
 constexpr int MM_TIMEOUT = 0x100;
-// tensor map of 16-bit tiles of box_cols x box_rows in the 128-byte-swizzled layout; elements outside read as zeros
-cudaError_t encode_mm(CUtensorMap* m, const MmOperand& o, bool bf16, int box_cols, int box_rows);
+// tensor map of tiles of box_cols x box_rows (128 bytes wide) in the 128-byte-swizzled layout; elements outside read as
+// zeros and are not written
+cudaError_t encode_mm(CUtensorMap* m, const MmOperand& o, DType type, int box_cols, int box_rows);
 // y[t] = w[e(t)] x[t] for few rows per expert: row tiles of tn (16, 32 or 64)
 cudaError_t launch_mm_narrow(const MmOperand& x, const MmOperand& w, const MmArgs& a, int tn, cudaStream_t st);
 // the same for many rows per expert: tiles of 256 features x up to 256 rows on pairs of SMs (a.ntn is set there)
@@ -196,6 +198,7 @@ struct MmWgradArgs {
     void* dw;       // [E, N, K], fp32 (out32) or the operands' type
     bool bf16, out32;
     int* status;
+    DType type() const { return bf16 ? DT_BF16 : DT_F16; }
 };
 // dw[e] = sum over e's rows of dy[t] x[t]^T
 cudaError_t launch_mm_wgrad(const MmOperand& dy, const MmOperand& x, const MmWgradArgs& a, cudaStream_t st);
