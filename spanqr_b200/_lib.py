@@ -4,6 +4,8 @@ import ctypes
 import threading
 from pathlib import Path
 
+import torch
+
 _DIR = Path(__file__).resolve().parent
 LIB_PATH = _DIR / "libspanqr.so"
 
@@ -90,6 +92,19 @@ def strerror(code):
 def check(code, what):
     if code != 0:
         raise SpanqrError(code, what)
+
+
+def launch(index, fn, what, *args):
+    """fn(*args, stream) on CUDA device `index` and its current stream; what() names the call in an error.  Entering the
+    device and asking for the stream object cost more than the rest of a small call, so the device is entered only where it
+    is not the current one and the stream's handle is read directly."""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        raise SpanqrError(rc, what())
 
 
 def workspace_bytes(K, r, batch=1):

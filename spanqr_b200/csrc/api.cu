@@ -986,7 +986,7 @@ int* mm_status() {
 }
 
 constexpr int MM_WIDE = 64;   // rows per expert on average above which a pair of SMs works on a tile
-constexpr int MM_MAX_E = 1024, MM_MAX_T = 1 << 30, MM_MAX_DIM = 1 << 24;
+constexpr int MM_MAX_T = 1 << 30, MM_MAX_DIM = 1 << 24;
 
 int check_mm(int type, int T, int E, int N, int K, const int* offsets) {
     if (T < 0 || T > MM_MAX_T || E < 1 || E > MM_MAX_E || N < 1 || N > MM_MAX_DIM || K < 1 || K > MM_MAX_DIM)

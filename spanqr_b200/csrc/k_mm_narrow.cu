@@ -181,7 +181,9 @@ __global__ void __launch_bounds__(THREADS, 2) k_mm_narrow(const __grid_constant_
 template <int TN, bool W_MN>
 cudaError_t launch(const CUtensorMap& tw, const CUtensorMap& tx, const MmArgs& a, int tiles, int S, cudaStream_t st) {
     const int smem = Cfg<TN>::FIXED + 2 * (a.E + 1) * (int)sizeof(int);
-    cudaError_t e = cudaFuncSetAttribute(k_mm_narrow<TN, W_MN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static SmemOnce once;
+    cudaError_t e = once.allow(reinterpret_cast<const void*>(k_mm_narrow<TN, W_MN>),
+                               Cfg<TN>::FIXED + 2 * (MM_MAX_E + 1) * (int)sizeof(int));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)tiles * S);

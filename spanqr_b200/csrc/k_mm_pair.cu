@@ -589,12 +589,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tear_down(p, a.status);
 }
 
-template <typename K, typename... A>
-cudaError_t go(K kernel, long long tiles, int E, cudaStream_t st, const A&... args) {
+template <auto kernel, typename... A>
+cudaError_t go(long long tiles, int E, cudaStream_t st, const A&... args) {
     int nsm = 0;
     cudaError_t e = sm_count(&nsm);
     const int smem = FIXED + 2 * (E + 1) * (int)sizeof(int);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static SmemOnce once;   // of this kernel
+    if (e == cudaSuccess) e = once.allow(reinterpret_cast<const void*>(kernel), FIXED + 2 * (MM_MAX_E + 1) * (int)sizeof(int));
     if (e != cudaSuccess) return e;
     const long long pairs = tiles < nsm / 2 ? tiles : nsm / 2;
     kernel<<<(unsigned)(2 * pairs), THREADS, smem, st>>>(args...);
@@ -612,7 +613,7 @@ cudaError_t launch_mm_wide(const MmOperand& x, const MmOperand& w, const MmArgs&
     if (e != cudaSuccess) return e;
     const long long tiles = ((long long)(a.T / NT) + (a.T < a.E ? a.T : a.E)) * a.ntn;   // the most the offsets could give
     if (tiles > (1LL << 30)) return cudaErrorInvalidValue;
-    return w.mn ? go(k_mm_wide<true>, tiles, a.E, st, tw, tx, a) : go(k_mm_wide<false>, tiles, a.E, st, tw, tx, a);
+    return w.mn ? go<k_mm_wide<true>>(tiles, a.E, st, tw, tx, a) : go<k_mm_wide<false>>(tiles, a.E, st, tw, tx, a);
 }
 
 cudaError_t launch_mm_wgrad(const MmOperand& dy, const MmOperand& x, const MmWgradArgs& a, cudaStream_t st) {
@@ -627,10 +628,10 @@ cudaError_t launch_mm_wgrad(const MmOperand& dy, const MmOperand& x, const MmWgr
     if (e != cudaSuccess) return e;
     const long long tiles = (long long)a.E * ((a.N + 2 * FT - 1) / (2 * FT)) * ((a.K + NT - 1) / NT);
     if (rows16)
-        return a.out32 ? go(k_mm_wgrad<float, true>, tiles, a.E, st, tdy, tx, tdw, a)
-                       : go(k_mm_wgrad<uint16_t, true>, tiles, a.E, st, tdy, tx, tdw, a);
-    return a.out32 ? go(k_mm_wgrad<float, false>, tiles, a.E, st, tdy, tx, tdw, a)
-                   : go(k_mm_wgrad<uint16_t, false>, tiles, a.E, st, tdy, tx, tdw, a);
+        return a.out32 ? go<k_mm_wgrad<float, true>>(tiles, a.E, st, tdy, tx, tdw, a)
+                       : go<k_mm_wgrad<uint16_t, true>>(tiles, a.E, st, tdy, tx, tdw, a);
+    return a.out32 ? go<k_mm_wgrad<float, false>>(tiles, a.E, st, tdy, tx, tdw, a)
+                   : go<k_mm_wgrad<uint16_t, false>>(tiles, a.E, st, tdy, tx, tdw, a);
 }
 
 }  // namespace spq

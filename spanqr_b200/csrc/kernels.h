@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace spq {
@@ -185,6 +187,23 @@ struct MmArgs {
     int* status;          // a bounded wait that runs out ORs MM_TIMEOUT
 };
 constexpr int MM_TIMEOUT = 0x100;
+constexpr int MM_MAX_E = 1024;
+// raises one kernel's dynamic shared memory limit, once per device
+class SmemOnce {
+    std::atomic<unsigned long long> done{0};
+
+public:
+    cudaError_t allow(const void* kernel, int bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+        if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+        return e;
+    }
+};
 // tensor map of tiles of box_cols x box_rows (128 bytes wide) in the 128-byte-swizzled layout; elements outside read as
 // zeros and are not written
 cudaError_t encode_mm(CUtensorMap* m, const MmOperand& o, DType type, int box_cols, int box_rows);

@@ -10,7 +10,7 @@ Both run on libspanqr's kernels on the current stream of the tensors' device, wi
 workspace comes from torch's allocator per call, so calls on different streams and captured graphs never share one.
 """
 from array import array
-from operator import attrgetter, methodcaller
+from operator import attrgetter
 
 import torch
 import torch.distributed as dist
@@ -19,7 +19,8 @@ from . import _lib
 
 # SPANQR_F32, SPANQR_F16, SPANQR_BF16
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_dtype, _contiguous = attrgetter("dtype"), methodcaller("is_contiguous")
+_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
+_contiguous = torch.Tensor.is_contiguous
 _ptr, _numel, _device = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
 
 
@@ -34,67 +35,68 @@ def _dense(t):
 
 
 def _check(tensors, name):
-    """the list as a list, and its device (None when empty)"""
+    """the list as a list, its types and its device's index (None when empty)"""
     if torch.is_tensor(tensors):
         raise TypeError(f"{name} must be a list of tensors (got one tensor)")
     ts = list(tensors)
     if not all(map(torch.is_tensor, ts)):
         raise TypeError(f"{name} must hold tensors only")
-    bad = set(map(_dtype, ts)) - DTYPES.keys()
-    if bad:
-        raise TypeError(f"{name} must be fp32, fp16 or bf16 (got {', '.join(map(str, bad))})")
+    kinds = set(map(_dtype, ts))
+    if not kinds <= DTYPES.keys():
+        raise TypeError(f"{name} must be fp32, fp16 or bf16 (got {', '.join(map(str, kinds - DTYPES.keys()))})")
     devs = set(map(_device, ts))
     if -1 in devs:
         raise TypeError(f"{name} must be CUDA tensors")
     if len(devs) > 1:
         raise ValueError(f"{name} must be on one device (got cuda:{', cuda:'.join(map(str, sorted(devs)))})")
-    return ts, (torch.device("cuda", devs.pop()) if devs else None)
-
-
-def _types(ts):
-    kinds = set(map(_dtype, ts))
-    if len(kinds) == 1:
-        return array("i", [DTYPES[kinds.pop()]]) * len(ts)
-    return array("i", [DTYPES[d] for d in map(_dtype, ts)])
+    types = array("i", [DTYPES[kinds.pop()]]) * len(ts) if len(kinds) == 1 else array("i", map(DTYPES.get, map(_dtype, ts)))
+    return ts, types, devs.pop() if devs else None
 
 
 def _at(a):
     return a.buffer_info()[0]
 
 
+_WS_BYTES = {}
+
+
 def _workspace(dev, count):
-    n = _lib.ctypes.c_size_t(0)
-    _lib.check(_lib.lib().spanqr_grad_workspace_bytes(count, _lib.ctypes.byref(n)), f"grad_workspace_bytes({count})")
-    return torch.empty(n.value, dtype=torch.uint8, device=dev)
+    bytes_ = _WS_BYTES.get(count)
+    if bytes_ is None:
+        n = _lib.ctypes.c_size_t(0)
+        _lib.check(_lib.lib().spanqr_grad_workspace_bytes(count, _lib.ctypes.byref(n)), f"grad_workspace_bytes({count})")
+        bytes_ = _WS_BYTES[count] = n.value
+    return torch.empty(bytes_, dtype=torch.uint8, device=dev)
 
 
-def _run_norm(ts, dev, sumsq, norm, stream):
+def _run_norm(ts, types, dev, sumsq, norm):
     """the norm's kernels for contiguous tensors ts; sumsq and norm are tensors or None"""
     ws = _workspace(dev, len(ts))
-    ptrs, kinds, sizes = array("Q", map(_ptr, ts)), _types(ts), array("q", map(_numel, ts))
-    _lib.check(_lib.lib().spanqr_grad_norm(_at(ptrs), _at(kinds), _at(sizes), len(ts),
-                                           None if sumsq is None else sumsq.data_ptr(),
-                                           None if norm is None else norm.data_ptr(), ws.data_ptr(), ws.numel(),
-                                           stream), f"grad_norm({len(ts)} tensors)")
+    ptrs, sizes = array("Q", map(_ptr, ts)), array("q", map(_numel, ts))
+    _lib.launch(dev, _lib.lib().spanqr_grad_norm, lambda: f"grad_norm({len(ts)} tensors)", _at(ptrs), _at(types),
+                _at(sizes), len(ts), None if sumsq is None else sumsq.data_ptr(), None if norm is None else norm.data_ptr(),
+                ws.data_ptr(), ws.numel())
 
 
-def _run_clip(ins, outs, dev, max_norm, sumsq, norm, stream):
+def _run_clip(ins, in_types, outs, out_types, dev, max_norm, sumsq, norm):
     ws = _workspace(dev, len(ins))
     pi, po, sizes = array("Q", map(_ptr, ins)), array("Q", map(_ptr, outs)), array("q", map(_numel, ins))
-    ki, ko = _types(ins), _types(outs)
-    rc = _lib.lib().spanqr_grad_clip(_at(pi), _at(ki), _at(po), _at(ko), _at(sizes), len(ins), max_norm,
-                                     None if sumsq is None else sumsq.data_ptr(), norm.data_ptr(), ws.data_ptr(),
-                                     ws.numel(), stream)
-    if rc == 7:   # SPANQR_ERR_OVERLAP
-        raise ValueError("clip_grads: an output overlaps another tensor of the call (the same tensor listed twice?)")
-    _lib.check(rc, f"clip_grads({len(ins)} tensors)")
+    try:
+        _lib.launch(dev, _lib.lib().spanqr_grad_clip, lambda: f"clip_grads({len(ins)} tensors)", _at(pi), _at(in_types),
+                    _at(po), _at(out_types), _at(sizes), len(ins), max_norm, None if sumsq is None else sumsq.data_ptr(),
+                    norm.data_ptr(), ws.data_ptr(), ws.numel())
+    except _lib.SpanqrError as e:
+        if e.code != 7:   # SPANQR_ERR_OVERLAP
+            raise
+        raise ValueError("clip_grads: an output overlaps another tensor of the call (one tensor listed twice?)") from None
 
 
-def _group_sumsq(ts, dev, group, stream):
+def _group_sumsq(ts, types, dev, group):
     """the list's sum of squares (fp64), summed over the group's ranks"""
-    sumsq = torch.empty((), dtype=torch.float64, device=dev)
-    _run_norm(ts, dev, sumsq, None, stream)
-    dist.all_reduce(sumsq, group=group)
+    with torch.cuda.device(dev):
+        sumsq = torch.empty((), dtype=torch.float64, device=dev)
+        _run_norm(ts, types, dev, sumsq, None)
+        dist.all_reduce(sumsq, group=group)
     return sumsq
 
 
@@ -105,17 +107,17 @@ def grad_norm(tensors, *, group=None):
     of the sum of squares; every rank of the group must call, with an empty list if it holds nothing.  Without it the
     norm is of this process's list alone.  Deterministic; large and small values do not overflow or vanish in their
     squares.  Not differentiable."""
-    ts, dev = _check(tensors, "tensors")
+    ts, types, dev = _check(tensors, "tensors")
     if dev is None:
-        dev = torch.device("cuda", torch.cuda.current_device())
-    ts = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in ts]
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        if group is None:
-            _run_norm(ts, dev, None, norm, stream)
-        else:
-            _run_clip([], [], dev, 0.0, _group_sumsq(ts, dev, group, stream), norm, stream)   # its square root
+        dev = torch.cuda.current_device()
+    if not all(map(_contiguous, ts)):
+        ts = [t if _dense(t) else t.contiguous() for t in ts]
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    if group is None:
+        _run_norm(ts, types, dev, None, norm)
+    else:   # an empty list's clipping gives the sum's square root
+        none = array("i")
+        _run_clip([], none, [], none, dev, 0.0, _group_sumsq(ts, types, dev, group), norm)
     return norm
 
 
@@ -132,39 +134,40 @@ def clip_grads(tensors, max_norm, *, out=None, group=None):
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must be a number >= 0 (got {max_norm})")
-    ts, dev = _check(tensors, "tensors")
+    ts, types, dev = _check(tensors, "tensors")
     if out is None:
         ins = ts if all(map(_contiguous, ts)) else [t.contiguous() for t in ts]
-        res = outs = [torch.empty_like(t, memory_format=torch.contiguous_format, requires_grad=False) for t in ins]
+        res, out_types = [torch.empty_like(t, requires_grad=False) for t in ins], types
     else:
-        res, odev = _check(out, "out")
-        outs = res
+        res, out_types, odev = _check(out, "out")
         if len(res) != len(ts):
             raise ValueError(f"out must hold {len(ts)} tensors (got {len(res)})")
         if odev != dev:
-            raise ValueError(f"out must be on the tensors' device (got {odev} and {dev})")
-        ins = []
-        for i, (t, o) in enumerate(zip(ts, outs)):
-            if t is not o:
-                if o.shape != t.shape:
-                    raise ValueError(f"out[{i}] has shape {tuple(o.shape)}, its input {tuple(t.shape)}")
+            raise ValueError(f"out must be on the tensors' device (got cuda:{odev} and cuda:{dev})")
+        if list(map(_shape, ts)) != list(map(_shape, res)):
+            i = next(i for i, (t, o) in enumerate(zip(ts, res)) if t.shape != o.shape)
+            raise ValueError(f"out[{i}] has shape {tuple(res[i].shape)}, its input {tuple(ts[i].shape)}")
+        if out_types != types:
+            for i, (t, o) in enumerate(zip(ts, res)):
                 if o.dtype != t.dtype and o.dtype != torch.float32:
                     raise TypeError(f"out[{i}] must be {t.dtype} or fp32 (got {o.dtype})")
-            if not (t.is_contiguous() and o.is_contiguous()):
-                if t.stride() == o.stride() and _dense(t):
-                    pass
-                elif not o.is_contiguous():
-                    raise ValueError(f"out[{i}] must be contiguous, or dense with its input's strides")
-                else:
-                    t = t.contiguous()
-            ins.append(t)
+        ins = ts
+        if not (all(map(_contiguous, ts)) and all(map(_contiguous, res))):
+            ins = [_like_output(i, t, o) for i, (t, o) in enumerate(zip(ts, res))]
     if dev is None:
-        dev = torch.device("cuda", torch.cuda.current_device())
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        sumsq = None if group is None else _group_sumsq(ins, dev, group, stream)
-        _run_clip(ins, outs, dev, max_norm, sumsq, norm, stream)
+        dev = torch.cuda.current_device()
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    sumsq = None if group is None else _group_sumsq(ins, types, dev, group)
+    _run_clip(ins, types, res, out_types, dev, max_norm, sumsq, norm)
     if out is not None and res:
         torch.autograd.graph.increment_version([o for o in res if not o.is_inference()])
     return res, norm
+
+
+def _like_output(i, t, o):
+    """t, or a contiguous copy of it, with its elements in o's order in memory"""
+    if t.stride() == o.stride() and _dense(t):
+        return t
+    if not o.is_contiguous():
+        raise ValueError(f"out[{i}] must be contiguous, or dense with its input's strides")
+    return t.contiguous()

@@ -22,15 +22,14 @@ def _up8(n):
     return -(-n // 8) * 8
 
 
-def _row_stride(t, rows, cols):
-    """the row stride of t as an operand the copy engine can read (16-byte aligned rows of contiguous elements), or None.
-    rows, cols: the dimensions of t that run over rows and along them."""
-    if t.shape[cols] > 1 and t.stride(cols) != 1 or t.data_ptr() % 16:
+def _row_stride(ptr, rows, cols, ld, step):
+    """the row stride of an operand the copy engine can read (16-byte aligned rows of contiguous elements), or None: `rows`
+    rows `ld` elements apart, of `cols` elements `step` apart"""
+    if step != 1 and cols > 1 or ptr % 16:
         return None
-    if t.shape[rows] == 1:
-        return _up8(t.shape[cols])   # a single row's stride is free
-    ld = t.stride(rows)
-    return ld if ld % 8 == 0 and ld >= t.shape[cols] else None
+    if rows == 1:
+        return _up8(cols)   # a single row's stride is free
+    return ld if ld % 8 == 0 and ld >= cols else None
 
 
 def _padded(t):
@@ -43,26 +42,27 @@ def _padded(t):
 
 def _rows(x):
     """x [T, K] (or a padded copy) and its row stride"""
-    ld = _row_stride(x, 0, 1)
+    T, K = x.shape
+    ld = _row_stride(x.data_ptr(), T, K, *x.stride())
     if ld is None:
-        x = _padded(x)
-        ld = _row_stride(x, 0, 1)
+        x, ld = _padded(x), _up8(K)
     return x, ld
 
 
 def _weights(w):
     """w [E, N, K] (or a padded copy), its row stride, its expert stride and whether it is stored [E, K, N]"""
     E, N, K = w.shape
-    for transposed, (rows, cols) in ((False, (1, 2)), (True, (2, 1))):
-        ld = _row_stride(w, rows, cols)
-        if ld is None:
-            continue
-        need = (w.shape[rows] - 1) * ld + w.shape[cols]
-        if E == 1:
-            return w, ld, _up8(need), transposed
-        if w.stride(0) % 8 == 0 and w.stride(0) >= need:
-            return w, ld, w.stride(0), transposed
-    return _weights(_padded(w))
+    se, sn, sk = w.stride()
+    ptr = w.data_ptr()
+    for transposed, rows, cols, ld, step in ((False, N, K, sn, sk), (True, K, N, sk, sn)):
+        ld = _row_stride(ptr, rows, cols, ld, step)
+        if ld is not None:
+            need = (rows - 1) * ld + cols
+            if E == 1:
+                return w, ld, _up8(need), transposed
+            if se % 8 == 0 and se >= need:
+                return w, ld, se, transposed
+    return _padded(w), _up8(K), N * _up8(K), False
 
 
 def _span(t):
@@ -105,31 +105,26 @@ def _check_offsets(offsets, x, E=None):
 def _mm(x, w, offsets, out=None):
     T, K = x.shape
     E, N, _ = w.shape
-    y = torch.empty((T, N), dtype=x.dtype, device=x.device) if out is None else out
+    y = x.new_empty((T, N)) if out is None else out
     if T == 0:
         return y
     x, ldx = _rows(x)
     w, ldw, plane, transposed = _weights(w)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().spanqr_mm_grouped(x.data_ptr(), ldx, w.data_ptr(), ldw, plane, int(transposed),
-                                                offsets.data_ptr(), y.data_ptr(), y.stride(0) if T > 1 else N,
-                                                DTYPES[x.dtype], T, E, N, K, int(out is None),
-                                                torch.cuda.current_stream(x.device).cuda_stream),
-                   f"mm_grouped({T}x{K}, {E} experts of {N}x{K})")
+    _lib.launch(x.get_device(), _lib.lib().spanqr_mm_grouped, lambda: f"mm_grouped({T}x{K}, {E} experts of {N}x{K})",
+                x.data_ptr(), ldx, w.data_ptr(), ldw, plane, transposed, offsets.data_ptr(), y.data_ptr(),
+                y.stride(0) if T > 1 else N, DTYPES[x.dtype], T, E, N, K, out is None)
     return y
 
 
 def _wgrad(dy, x, offsets, dtype, out=None):
     T, N = dy.shape
     K, E = x.shape[1], offsets.shape[0]
-    dw = torch.empty((E, N, K), dtype=dtype, device=x.device) if out is None else out
+    dw = x.new_empty((E, N, K), dtype=dtype) if out is None else out
     dy, lddy = _rows(dy) if T else (dy, N)
     x, ldx = _rows(x) if T else (x, K)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.lib().spanqr_mm_grouped_wgrad(dy.data_ptr(), lddy, x.data_ptr(), ldx, offsets.data_ptr(),
-                                                      dw.data_ptr(), DTYPES[x.dtype], DTYPES[dw.dtype], T, E, N, K,
-                                                      torch.cuda.current_stream(x.device).cuda_stream),
-                   f"mm_grouped_wgrad({T} rows, {E} experts of {N}x{K})")
+    _lib.launch(x.get_device(), _lib.lib().spanqr_mm_grouped_wgrad,
+                lambda: f"mm_grouped_wgrad({T} rows, {E} experts of {N}x{K})", dy.data_ptr(), lddy, x.data_ptr(), ldx,
+                offsets.data_ptr(), dw.data_ptr(), DTYPES[x.dtype], DTYPES[dw.dtype], T, E, N, K)
     return dw
 
 
