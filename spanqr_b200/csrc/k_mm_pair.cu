@@ -296,10 +296,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             }
         }
     } else {
-        // TMEM lane = feature, column = row of y: neighbouring lanes exchange values so that each stores two features of
-        // one row
-        const bool pairs32 = a.ldy % 2 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 3) == 0;
-        const int q = warp & 3, half = warp >> 2, odd = lane & 1;
+        const bool v16 = a.ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
+        const int q = warp & 3, half = warp >> 2;
+        const uint32_t stage = tc::smem_u32(p.sm) + STAGING + warp * Y_STAGE;
         if (a.zero_tail) {   // rows behind the last expert
             for (long long t = p.start[a.E] + (long long)blockIdx.x; t < a.T; t += gridDim.x)
                 for (int n = threadIdx.x; n < a.N; n += 256) a.y[t * a.ldy + n] = 0;
@@ -314,33 +313,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                 break;
             }
             tc::fence_after_sync();
-            const int n = d.n0 + p.rank * FT + q * 32 + lane;
-            for (int c0 = half * 16; c0 < d.cols; c0 += 32) {
-                float v[16];
-                tc::tmem_ld16(p.tmem + b * NT + ((uint32_t)(q * 32) << 16) + c0, v);
-                tc::tmem_wait_ld();
-                uint16_t* y = a.y + (long long)(d.t0 + c0) * a.ldy + n;
-                if (pairs32) {
-                    y -= odd;
-#pragma unroll
-                    for (int c = 0; c < 16; c += 2) {
-                        const float got = __shfl_xor_sync(~0u, odd ? v[c] : v[c + 1], 1);
-                        const int r = d.t0 + c0 + c + odd;
-                        if (r < d.t1) {
-                            uint16_t* const o = y + (long long)(c + odd) * a.ldy;
-                            if (n - odd + 1 < a.N)
-                                *reinterpret_cast<uint32_t*>(o) = odd ? pack16(got, v[c + 1], a.bf16) : pack16(v[c], got, a.bf16);
-                            else if (n - odd < a.N)
-                                *o = to16(odd ? got : v[c], a.bf16);
-                        }
-                    }
-                } else if (n < a.N) {
-#pragma unroll
-                    for (int c = 0; c < 16; ++c)
-                        if (d.t0 + c0 + c < d.t1) y[(long long)c * a.ldy] = to16(v[c], a.bf16);
-                }
-                __syncwarp();
-            }
+            const int n = d.n0 + p.rank * FT + q * 32;
+            if (n < a.N)
+                for (int c = half * 32; c < d.cols; c += 64)
+                    store_y32(p.tmem + b * NT + c + ((uint32_t)(q * 32) << 16), stage, a.y + (long long)(d.t0 + c) * a.ldy + n,
+                              a.ldy, d.t1 - d.t0 - c, a.N - n, a.bf16, v16);
             tc::fence_before_sync();
             __syncwarp();
             if (lane == 0) arrive_cluster(p.tempty0 + b * 8);

@@ -111,6 +111,67 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// ---- accumulators (TMEM lanes = features, columns = rows of y) to row-major 16-bit rows of y ----
+// 16 lanes x 32 columns as four fragments of 16 x 8: v[4 i + {0, 1}] of thread t is lane t / 4, columns 8 i + 2 (t % 4) + {0,
+// 1}; v[4 i + {2, 3}] the same 8 lanes on
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+// four 8 x 8 matrices of 16-bit values, each transposed: lane 8 i + r gives the address of row r of matrix i as stored
+__device__ __forceinline__ void stmatrix4t(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+                 "r"(d)
+                 : "memory");
+}
+constexpr int Y_PITCH = 80;            // bytes from one staged row of y to the next: 32 features and 16 bytes against conflicts
+constexpr int Y_STAGE = 32 * Y_PITCH;  // per warp
+
+// This warp's 32 features x 32 rows of y: TMEM at `taddr` (this warp's lanes, the first column) through `stage` to y + r *
+// ldy, rows r < rows and features f < features.  v16: every row of y and the first feature are on 16 bytes.
+__device__ __forceinline__ void store_y32(uint32_t taddr, uint32_t stage, uint16_t* y, long long ldy, int rows, int features,
+                                          bool bf16, bool v16) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();   // the previous block has been read
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float v[16];
+        tmem_ld_frag(taddr + ((uint32_t)(16 * h) << 16), v);
+        tc::tmem_wait_ld();
+        const uint32_t at = stage + ((lane >> 4) * 8 + (lane & 7)) * Y_PITCH + h * 32 + ((lane >> 3) & 1) * 16;
+#pragma unroll
+        for (int i = 0; i < 4; i += 2)
+            stmatrix4t(at + i * 8 * Y_PITCH, pack16(v[4 * i], v[4 * i + 1], bf16), pack16(v[4 * i + 2], v[4 * i + 3], bf16),
+                       pack16(v[4 * i + 4], v[4 * i + 5], bf16), pack16(v[4 * i + 6], v[4 * i + 7], bf16));
+    }
+    __syncwarp();
+    const int f = (lane & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
+        uint32_t w[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                     : "r"(stage + r * Y_PITCH + f * 2));
+        if (r >= rows) continue;
+        uint16_t* const o = y + r * ldy + f;
+        if (v16 && f + 8 <= features) {
+            *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+                if (f + x < features) o[x] = (uint16_t)(w[x >> 1] >> (16 * (x & 1)));
+        }
+    }
+}
+
 // ---- offsets -> tiles ----
 // start[e], start[e + 1]: the rows of expert e; pre[e]: tiles of `rows` rows before it (both E + 1 long, in shared
 // memory).  offsets[e] is the end of expert e's rows; ends are clamped to [previous end, T], so that no offsets make a
