@@ -278,14 +278,16 @@ int spanqr_grad_clip(const void* const* in, const int* in_type, void* const* out
  *   from offsets[E - 1] on are zeroed (zero_tail != 0) or left as they are.
  * spanqr_mm_grouped_wgrad: dw[e] = sum over e's rows of dy[t] x[t]^T, dw [E, N, K] contiguous, of out_type SPANQR_F32 or
  *   `type`; zeros for an expert without rows.  Sums of 256 rows are taken by the tensor cores, their sums in fp32.
- * Both are deterministic, need no workspace and read no host memory after they return.
+ * Both are deterministic.  Their workspaces (the _workspace_bytes of the same sizes, often 0, then ws may be NULL; 256-byte
+ * aligned) need no initialisation; calls in flight at the same time need different ones.
  * spanqr_mm_read_status: the word in which these kernels report, on the current device, a bounded device wait that ran
  *   out (0: none since the last read; else SPANQR_ERR_DEVICE, and results since then must not be used).  Clears it and
  *   synchronises `stream`.
  */
+int spanqr_mm_grouped_workspace_bytes(int T, int E, int N, int K, size_t* bytes);
 int spanqr_mm_grouped(const void* x, long long ldx, const void* w, long long ldw, long long stride_w, int w_transposed,
                       const int* offsets, void* y, long long ldy, int type, int T, int E, int N, int K, int zero_tail,
-                      spanqr_stream_t stream);
+                      void* ws, size_t ws_bytes, spanqr_stream_t stream);
 int spanqr_mm_grouped_wgrad(const void* dy, long long lddy, const void* x, long long ldx, const int* offsets, void* dw,
                             int type, int out_type, int T, int E, int N, int K, spanqr_stream_t stream);
 int spanqr_mm_read_status(spanqr_stream_t stream, int* device_status);

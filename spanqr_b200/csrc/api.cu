@@ -985,12 +985,15 @@ int* mm_status() {
     return cudaGetSymbolAddress(&p, g_mm_status) == cudaSuccess ? static_cast<int*>(p) : nullptr;
 }
 
-constexpr int MM_WIDE = 64;   // rows per expert on average above which a pair of SMs works on a tile
 constexpr int MM_MAX_T = 1 << 30, MM_MAX_DIM = 1 << 24;
 
+int check_mm_sizes(int T, int E, int N, int K) {
+    const bool ok = T >= 0 && T <= MM_MAX_T && E >= 1 && E <= MM_MAX_E && N >= 1 && N <= MM_MAX_DIM && K >= 1 && K <= MM_MAX_DIM;
+    return ok ? SPANQR_OK : SPANQR_ERR_SHAPE;
+}
 int check_mm(int type, int T, int E, int N, int K, const int* offsets) {
-    if (T < 0 || T > MM_MAX_T || E < 1 || E > MM_MAX_E || N < 1 || N > MM_MAX_DIM || K < 1 || K > MM_MAX_DIM)
-        return SPANQR_ERR_SHAPE;
+    const int rc = check_mm_sizes(T, E, N, K);
+    if (rc) return rc;
     if ((type != SPANQR_F16 && type != SPANQR_BF16) || !offsets || reinterpret_cast<uintptr_t>(offsets) % 4)
         return SPANQR_ERR_ARG;
     return SPANQR_OK;
@@ -1001,9 +1004,18 @@ bool mm_rows(const void* p, long long ld, long long cols) { return p && a16(p) &
 
 extern "C" {
 
+int spanqr_mm_grouped_workspace_bytes(int T, int E, int N, int K, size_t* bytes) {
+    int rc = check_mm_sizes(T, E, N, K);
+    if (rc) return rc;
+    if (!bytes) return SPANQR_ERR_ARG;
+    // the largest that a device of any number of SMs needs (a plan on more pairs splits no less)
+    *bytes = T > 0 ? mm_plan(T, E, N, K, MAX_SMS).ws : 0;
+    return SPANQR_OK;
+}
+
 int spanqr_mm_grouped(const void* x, long long ldx, const void* w, long long ldw, long long stride_w, int w_transposed,
                       const int* offsets, void* y, long long ldy, int type, int T, int E, int N, int K, int zero_tail,
-                      spanqr_stream_t stream) {
+                      void* ws, size_t ws_bytes, spanqr_stream_t stream) {
     const int rc = check_mm(type, T, E, N, K, offsets);
     if (rc) return rc;
     if (T == 0) return SPANQR_OK;
@@ -1013,14 +1025,16 @@ int spanqr_mm_grouped(const void* x, long long ldx, const void* w, long long ldw
     if (stride_w % 8 || (E > 1 && stride_w < (wrows - 1) * ldw + wcols) || stride_w >= (1LL << 38)) return SPANQR_ERR_ARG;
     const MmOperand ox{x, K, T, ldx, 0, 0, false};
     const MmOperand ow{w, wcols, wrows, ldw, E, E > 1 ? stride_w : wrows * ldw, w_transposed != 0};
-    MmArgs a{offsets, E, T, N, K, static_cast<uint16_t*>(y), ldy, (N + 127) / 128, type == SPANQR_BF16, zero_tail != 0,
-             mm_status()};
+    int nsm = 0;
+    cudaError_t e = sm_count(&nsm);
+    if (e != cudaSuccess) return cuda_fail(e);
+    const MmPlan plan = mm_plan(T, E, N, K, nsm);
+    if (plan.ws && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0 || ws_bytes < plan.ws)) return SPANQR_ERR_WORKSPACE;
+    const MmArgs a{offsets, E, T, N, K, static_cast<uint16_t*>(y), ldy, (N + 255) / 256, plan.ws ? static_cast<float*>(ws) : nullptr,
+                   type == SPANQR_BF16, zero_tail != 0, mm_status()};
     if (!a.status) return cuda_fail(cudaGetLastError());
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    const cudaError_t e = timed(K_MM, st, [&] {
-        return T > MM_WIDE * (long long)E ? launch_mm_wide(ox, ow, a, st)
-                                          : launch_mm_narrow(ox, ow, a, T <= 16LL * E ? 16 : T <= 32LL * E ? 32 : 64, st);
-    });
+    e = timed(K_MM, st, [&] { return launch_mm(ox, ow, a, plan, st); }, plan.split ? 2 : 1);
     return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
 }
 

@@ -1,0 +1,280 @@
+// dw[e] = sum over expert e's rows of dy[t] x[t]^T (no reference counterpart): D = dy^T x in tiles of 256 features x 256
+// columns of x, on pairs of SMs (mm_pair.cuh).  Both operands are read as they lie, row by row (MN-major), in stages of 64
+// rows.
+#include "mm_pair.cuh"
+
+namespace spq {
+namespace {
+
+using namespace mm;
+
+constexpr int NT = 256;
+using C = PairCfg<NT, 5, 8 * 4096>;   // five stages (four cost up to 7 %, six gave no more); 32 rows x 128 bytes of results per warp
+// stages (of 64 rows) summed in TMEM before they are added in registers
+template <typename OUT>
+constexpr int DRAIN = sizeof(OUT) == 4 ? 8 : 32;
+
+__device__ __forceinline__ void st_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// a warp's staged results to rows of dw that do not start on 16 bytes
+template <typename OUT>
+__device__ __forceinline__ void store_rows(const char* stage, OUT* row, int ld, int rows, int cols) {
+#pragma unroll 1
+    for (int x = 0; x < rows; ++x, row += ld)
+#pragma unroll 1
+        for (int y = threadIdx.x & 31; y < cols; y += 32) {
+            const int at = y * (int)sizeof(OUT);
+            row[y] = *reinterpret_cast<const OUT*>(stage + x * 128 + (((at >> 4) ^ (x & 7)) << 4) + (at & 15));
+        }
+    __syncwarp();
+}
+
+// whether a stage with `left` rows of its expert ends inside one product's 16
+__device__ __forceinline__ bool ragged(int left) { return left < BK && left % 16 != 0; }
+
+// The tensor core rounds toward zero each time it adds 16 products to its fp32 accumulator: over n additions of terms of
+// random sign the sum comes out about n * 3e-8 of itself too small.  So the accumulator is taken every DRAIN stages and
+// added to fp32 sums in registers, rounded to nearest, while the products go on in the other accumulator.  For fp32
+// results every 512 rows (measured 4e-7 off in all at 5000 rows, as a sum in fp32 is); for 16-bit results, whose own
+// rounding is 2^-9 or 2^-12, every 2048, which keeps the bias from growing with the length.  The reads of TMEM
+// take tensor-core time: 16384 rows, 8 experts of 5120x2048 in bf16: 285 us with a drain every 256 rows, 258 every 512, 252 every 4096.
+template <typename OUT, bool TMA_OUT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    k_mm_wgrad(const __grid_constant__ CUtensorMap tdy, const __grid_constant__ CUtensorMap tx,
+               const __grid_constant__ CUtensorMap tdw, const MmWgradArgs a) {
+    extern __shared__ char dyn[];
+    const Pair p = set_up<C>(dyn, a.offsets, a.E, a.T, 1 << 30);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int ntn = (a.N + 2 * FT - 1) / (2 * FT), ntk = (a.K + NT - 1) / NT, per = ntn * ntk;
+    const long long tiles = (long long)a.E * per;
+    const int pairs = (int)gridDim.x / 2;
+    struct Tile {
+        int e, n0, k0, cols, r0, rows, nb;   // cols: the tile's columns of x up to a multiple of 32; nb: stages of 64 rows
+    };
+    auto tile_at = [&](long long i) {
+        Tile t;
+        t.e = (int)(i / per);
+        const int l = (int)(i - (long long)t.e * per);
+        t.n0 = l / ntk * 2 * FT;
+        t.k0 = l % ntk * NT;
+        t.cols = min(NT, up32(a.K - t.k0));
+        t.r0 = p.start[t.e];
+        t.rows = p.start[t.e + 1] - t.r0;
+        t.nb = (t.rows + BK - 1) / BK;
+        return t;
+    };
+
+    if (warp == COPY_A) {
+        const bool one = elect();
+        Ring<C> r;
+        uint32_t ragged_phase = 0, zeroed_phases = 0;   // (bit s: that of zeroed[s])
+        bool ok = true;
+        for (long long t = blockIdx.x / 2; ok && t < tiles; t += pairs) {
+            const Tile d = tile_at(t);
+            const int n = d.n0 + p.rank * FT, k = d.k0 + p.rank * (d.cols / 2);
+            for (int c = 0; c < d.nb; ++c, r.next()) {
+                if (!(ok = __all_sync(~0u, stage_free(p, r)))) break;
+                const int left = d.rows - c * BK, row = d.r0 + c * BK;
+                const uint32_t as = tc::smem_u32(p.sm) + r.s * C::STAGE;
+                if (!ragged(left)) {
+                    if (one) {
+                        const uint32_t bar = p.full0 + r.s * 8;
+                        if (p.rank == 0) tc::mbar_expect_tx(&p.full[r.s], 2 * C::STAGE);
+                        tma2_load_2d(as, &tdy, n, row, bar);
+                        tma2_load_2d(as + BOX_MN, &tdy, n + 64, row, bar);
+                    }
+                    __syncwarp();
+                    continue;
+                }
+                // the expert's last rows, not a multiple of one product's 16: the rows behind them (another expert's) are
+                // zeroed in both operands before the products may read the stage
+                if (one) {
+                    const uint32_t bar = tc::smem_u32(p.ragged);
+                    tc::mbar_expect_tx(p.ragged, C::STAGE);
+                    mm::tma_load_2d(as, &tdy, n, row, bar);
+                    mm::tma_load_2d(as + BOX_MN, &tdy, n + 64, row, bar);
+                    mm::tma_load_2d(as + A_BYTES, &tx, k, row, bar);
+                    mm::tma_load_2d(as + A_BYTES + BOX_MN, &tx, k + 64, row, bar);
+                }
+                __syncwarp();
+                ok = __all_sync(~0u, tc::mbar_wait(p.ragged, ragged_phase));
+                ragged_phase ^= 1;
+                if (ok) {
+                    char* const st = p.sm + r.s * C::STAGE;   // box lane / 8, 16 bytes (lane % 8) of each row
+                    for (int x = left; x < ((left + 15) & ~15); ++x)
+                        *reinterpret_cast<int4*>(st + (lane >> 3) * BOX_MN + x * 128 + (lane & 7) * 16) = make_int4(0, 0, 0, 0);
+                    tc::fence_async_smem();
+                    __syncwarp();
+                    // the leader hands the stage over when both halves are zeroed (an arrival of the second CTA on full[s]
+                    // for every stage cost more than the products).  One barrier per stage: the other CTA may be several
+                    // ragged stages ahead, but not past a stage that the leader has not handed over
+                    if (p.rank != 0) {
+                        if (one) arrive_cluster(p.zeroed0 + r.s * 8);
+                    } else {
+                        ok = __all_sync(~0u, wait_cluster(&p.zeroed[r.s], (zeroed_phases >> r.s) & 1));
+                        zeroed_phases ^= 1u << r.s;
+                        if (ok && one) tc::mbar_arrive(&p.full[r.s]);
+                    }
+                }
+                if (!ok) {
+                    *p.err = 1;
+                    break;
+                }
+                __syncwarp();
+            }
+        }
+        finish_copies(p, r);
+    } else if (warp == COPY_B) {
+        const bool one = elect();
+        Ring<C> r;
+        bool ok = true;
+        for (long long t = blockIdx.x / 2; ok && t < tiles; t += pairs) {
+            const Tile d = tile_at(t);
+            const int k = d.k0 + p.rank * (d.cols / 2);
+            for (int c = 0; c < d.nb; ++c, r.next()) {
+                if (!(ok = __all_sync(~0u, stage_free(p, r)))) break;
+                if (one && !ragged(d.rows - c * BK)) {
+                    const uint32_t bs = tc::smem_u32(p.sm) + r.s * C::STAGE + A_BYTES, bar = p.full0 + r.s * 8;
+                    tma2_load_2d(bs, &tx, k, d.r0 + c * BK, bar);
+                    tma2_load_2d(bs + BOX_MN, &tx, k + 64, d.r0 + c * BK, bar);
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == PRODUCTS) {
+        if (p.rank == 0) {
+            const bool one = elect();
+            const uint64_t a0 = sdesc<true>(tc::smem_u32(p.sm)), b0 = sdesc<true>(tc::smem_u32(p.sm) + A_BYTES);
+            Ring<C> r;
+            int j = 0;   // accumulators over all tiles
+            for (long long t = blockIdx.x / 2; t < tiles && !*p.err; t += pairs) {
+                const Tile d = tile_at(t);
+                const uint32_t id = idesc_f16(2 * FT, d.cols, a.bf16, true, true);
+                for (int c0 = 0; c0 < d.nb; c0 += DRAIN<OUT>, ++j) {
+                    const int b = j & 1, c1 = min(c0 + DRAIN<OUT>, d.nb);
+                    const uint32_t acc = p.tmem + b * NT;
+                    if (j >= 2 && !tc::mbar_wait(&p.tempty[b], (uint32_t)((j / 2 - 1) & 1))) *p.err = 1;
+                    tc::fence_after_sync();
+                    for (int c = c0; c < c1; ++c) {
+                        if (*p.err || !tc::mbar_wait(&p.full[r.s], r.phase)) {
+                            *p.err = 1;
+                            break;
+                        }
+                        tc::fence_after_sync();
+                        const int left = d.rows - c * BK;
+                        if (one) {
+#pragma unroll
+                            for (int q = 0; q < BK / 16; ++q)
+                                if (q * 16 < left)
+                                    mma2_f16(acc, a0 + ((r.s * C::STAGE + q * kstep<true>()) >> 4), b0 + ((r.s * C::STAGE + q * kstep<true>()) >> 4),
+                                             id, c > c0 || q > 0);
+                            commit2(&p.empty[r.s]);
+                        }
+                        r.next();
+                    }
+                    if (one) commit2(&p.tfull[b]);
+                }
+            }
+        }
+    } else {
+        constexpr int COLS = 128 / sizeof(OUT);
+        const int q = warp & 3, half = warp >> 2;
+        const bool one = elect();
+        char* const stage = p.sm + C::STAGING + warp * 4096;
+        int j = 0;
+        bool ok = true;
+        for (long long t = blockIdx.x / 2; ok && t < tiles; t += pairs) {
+            const Tile d = tile_at(t);
+            float sum[NT / 2];
+#pragma unroll
+            for (int c = 0; c < NT / 2; ++c) sum[c] = 0.f;
+            for (int c = 0; c < d.nb; c += DRAIN<OUT>, ++j) {
+                const int b = j & 1;
+                ok = !*p.err && tc::mbar_wait(&p.tfull[b], (uint32_t)((j / 2) & 1));
+                if (!__all_sync(~0u, ok)) {
+                    *p.err = 1;
+                    ok = false;
+                    break;
+                }
+                tc::fence_after_sync();
+                const uint32_t at = p.tmem + b * NT + half * (NT / 2) + ((uint32_t)(q * 32) << 16);
+#pragma unroll
+                for (int c0 = 0; c0 < NT / 2; c0 += 16) {
+                    if (half * (NT / 2) + c0 < d.cols) {
+                        float v[16];
+                        tc::tmem_ld16(at + c0, v);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) sum[c0 + x] += v[x];
+                    }
+                }
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) arrive_cluster(p.tempty0 + b * 8);
+            }
+            if (!ok) break;
+            // 32 rows x 128 bytes at a time through shared memory (in the swizzled layout, so that the lanes' rows meet no
+            // bank twice), then one TMA store: lanes that write their own rows to memory touch 32 lines per instruction,
+            // which took longer than the products (16 experts of 2048x5120 in fp32: 328 us so)
+            const int n = d.n0 + p.rank * FT + q * 32, k = d.k0 + half * (NT / 2);
+            const uint32_t mine = tc::smem_u32(stage) + lane * 128;
+#pragma unroll
+            for (int c = 0; c < NT / 2; c += COLS) {
+                if (n < a.N && k + c < a.K) {
+                    if (one) bulk_wait_read();
+                    __syncwarp();
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        const uint32_t at = mine + ((x ^ (lane & 7)) << 4);
+                        if constexpr (sizeof(OUT) == 4) {
+                            const float* v = sum + c + 4 * x;
+                            st_shared16(at, __float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+                        } else {
+                            const float* v = sum + c + 8 * x;
+                            st_shared16(at, pack16(v[0], v[1], a.bf16), pack16(v[2], v[3], a.bf16), pack16(v[4], v[5], a.bf16),
+                                        pack16(v[6], v[7], a.bf16));
+                        }
+                    }
+                    if (TMA_OUT) {
+                        tc::fence_async_smem();
+                        __syncwarp();
+                        if (one) tma_store_3d(&tdw, k + c, n, d.e, tc::smem_u32(stage));
+                    } else {
+                        __syncwarp();
+                        store_rows(stage, static_cast<OUT*>(a.dw) + ((long long)d.e * a.N + n) * a.K + k + c, a.K,
+                                   min(32, a.N - n), min(COLS, a.K - k - c));
+                    }
+                }
+            }
+        }
+        if (one) bulk_wait();   // the last results have left shared memory before it goes
+    }
+    tear_down<C>(p, a.status);
+}
+
+}  // namespace
+
+cudaError_t launch_mm_wgrad(const MmOperand& dy, const MmOperand& x, const MmWgradArgs& a, cudaStream_t st) {
+    const int size = a.out32 ? 4 : 2;
+    const bool rows16 = reinterpret_cast<uintptr_t>(a.dw) % 16 == 0 && (long long)a.K * size % 16 == 0;
+    alignas(64) CUtensorMap tdy, tx, tdw{};
+    cudaError_t e = encode_mm(&tdy, dy, a.type(), 64, BK);
+    if (e == cudaSuccess) e = encode_mm(&tx, x, a.type(), 64, BK);
+    if (e == cudaSuccess && rows16)
+        e = encode_mm(&tdw, MmOperand{a.dw, a.K, a.N, a.K, a.E, (long long)a.N * a.K, false}, a.out32 ? DT_F32 : a.type(),
+                      128 / size, 32);
+    int nsm = 0;
+    if (e == cudaSuccess) e = sm_count(&nsm);
+    if (e != cudaSuccess) return e;
+    const long long tiles = (long long)a.E * ((a.N + 2 * FT - 1) / (2 * FT)) * ((a.K + NT - 1) / NT);
+    const int pairs = (int)(tiles < nsm / 2 ? tiles : nsm / 2);
+    if (rows16)
+        return a.out32 ? launch_pairs<C, k_mm_wgrad<float, true>>(pairs, a.E, st, tdy, tx, tdw, a)
+                       : launch_pairs<C, k_mm_wgrad<uint16_t, true>>(pairs, a.E, st, tdy, tx, tdw, a);
+    return a.out32 ? launch_pairs<C, k_mm_wgrad<float, false>>(pairs, a.E, st, tdy, tx, tdw, a)
+                   : launch_pairs<C, k_mm_wgrad<uint16_t, false>>(pairs, a.E, st, tdy, tx, tdw, a);
+}
+
+}  // namespace spq

@@ -180,7 +180,8 @@ struct MmArgs {
     int E, T, N, K;       // experts, rows, features, contracted elements
     uint16_t* y;          // [T, N], ld ldy
     long long ldy;
-    int ntn;              // feature tiles of 128
+    int ntn;              // feature tiles of 256
+    float* part;          // partial sums of split tiles (null: no tile is split)
     bool bf16;            // bf16, else fp16
     DType type() const { return bf16 ? DT_BF16 : DT_F16; }
     bool zero_tail;       // zero the rows behind the last expert (else they are left as they are)
@@ -207,10 +208,17 @@ public:
 // tensor map of tiles of box_cols x box_rows (128 bytes wide) in the 128-byte-swizzled layout; elements outside read as
 // zeros and are not written
 cudaError_t encode_mm(CUtensorMap* m, const MmOperand& o, DType type, int box_cols, int box_rows);
-// y[t] = w[e(t)] x[t] for few rows per expert: row tiles of tn (16, 32 or 64)
-cudaError_t launch_mm_narrow(const MmOperand& x, const MmOperand& w, const MmArgs& a, int tn, cudaStream_t st);
-// the same for many rows per expert: tiles of 256 features x up to 256 rows on pairs of SMs (a.ntn is set there)
-cudaError_t launch_mm_wide(const MmOperand& x, const MmOperand& w, const MmArgs& a, cudaStream_t st);
+// how launch_mm takes a call's sizes on a device of nsm SMs
+struct MmPlan {
+    int nt;            // rows of a tile: 32, 64, 128 or 256
+    bool split;        // the contracted dimension is split over the pairs
+    int pairs;         // of SMs
+    long long tiles;   // the most that the offsets could give
+    size_t ws;         // bytes of workspace (0 without the split)
+};
+MmPlan mm_plan(int T, int E, int N, int K, int nsm);
+// y[t] = w[e(t)] x[t] (a.part: the plan's workspace, null without the split)
+cudaError_t launch_mm(const MmOperand& x, const MmOperand& w, const MmArgs& a, const MmPlan& p, cudaStream_t st);
 struct MmWgradArgs {
     const int* offsets;
     int E, T, N, K;

@@ -132,43 +132,59 @@ __device__ __forceinline__ void stmatrix4t(uint32_t addr, uint32_t a, uint32_t b
                  : "memory");
 }
 constexpr int Y_PITCH = 80;            // bytes from one staged row of y to the next: 32 features and 16 bytes against conflicts
-constexpr int Y_STAGE = 32 * Y_PITCH;  // per warp
+constexpr int Y_STAGE = 2 * 32 * Y_PITCH;   // per warp: two blocks of 32 rows in turn
 
-// This warp's 32 features x 32 rows of y: TMEM at `taddr` (this warp's lanes, the first column) through `stage` to y + r *
-// ldy, rows r < rows and features f < features.  v16: every row of y and the first feature are on 16 bytes.
-__device__ __forceinline__ void store_y32(uint32_t taddr, uint32_t stage, uint16_t* y, long long ldy, int rows, int features,
-                                          bool bf16, bool v16) {
-    const int lane = threadIdx.x & 31;
-    __syncwarp();   // the previous block has been read
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        float v[16];
-        tmem_ld_frag(taddr + ((uint32_t)(16 * h) << 16), v);
-        tc::tmem_wait_ld();
-        const uint32_t at = stage + ((lane >> 4) * 8 + (lane & 7)) * Y_PITCH + h * 32 + ((lane >> 3) & 1) * 16;
-#pragma unroll
-        for (int i = 0; i < 4; i += 2)
-            stmatrix4t(at + i * 8 * Y_PITCH, pack16(v[4 * i], v[4 * i + 1], bf16), pack16(v[4 * i + 2], v[4 * i + 3], bf16),
-                       pack16(v[4 * i + 4], v[4 * i + 5], bf16), pack16(v[4 * i + 6], v[4 * i + 7], bf16));
+// This warp's 32 features of a tile's rows c0, c0 + step, ... (blocks of 32, below cols): TMEM at `taddr` (this warp's lanes,
+// the tile's first column) through `stage` to y + r * ldy, rows r < rows and features f < features.  v16: every row of y and
+// the first feature are on 16 bytes.  The next block's accumulators are read while this one is stored.
+__device__ __forceinline__ void store_y(uint32_t taddr, uint32_t stage, uint16_t* y, long long ldy, int c0, int step, int cols,
+                                        int rows, int features, bool bf16, bool v16) {
+    const int lane = threadIdx.x & 31, f = (lane & 3) * 8;
+    const uint32_t at = ((lane >> 4) * 8 + (lane & 7)) * Y_PITCH + ((lane >> 3) & 1) * 16;
+    float v[2][16];
+    if (c0 < cols) {
+        tmem_ld_frag(taddr + c0, v[0]);
+        tmem_ld_frag(taddr + c0 + (16u << 16), v[1]);
     }
-    __syncwarp();
-    const int f = (lane & 3) * 8;
+    uint32_t other = stage + 32 * Y_PITCH;
+    for (int c = c0; c < cols; c += step) {
+        tc::tmem_wait_ld();
+        uint32_t w[2][8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = i * 8 + (lane >> 2);
-        uint32_t w[4];
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                     : "r"(stage + r * Y_PITCH + f * 2));
-        if (r >= rows) continue;
-        uint16_t* const o = y + r * ldy + f;
-        if (v16 && f + 8 <= features) {
-            *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int x = 0; x < 8; ++x)
-                if (f + x < features) o[x] = (uint16_t)(w[x >> 1] >> (16 * (x & 1)));
+            for (int i = 0; i < 8; ++i) w[h][i] = pack16(v[h][2 * i], v[h][2 * i + 1], bf16);
+        if (c + step < cols) {
+            tmem_ld_frag(taddr + c + step, v[0]);
+            tmem_ld_frag(taddr + c + step + (16u << 16), v[1]);
         }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            stmatrix4t(stage + at + h * 32, w[h][0], w[h][1], w[h][2], w[h][3]);
+            stmatrix4t(stage + at + h * 32 + 16 * Y_PITCH, w[h][4], w[h][5], w[h][6], w[h][7]);
+        }
+        __syncwarp();   // (the buffer's last readers passed the block in between)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 2);
+            uint32_t u[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3])
+                         : "r"(stage + r * Y_PITCH + f * 2)
+                         : "memory");
+            if (c + r >= rows) continue;
+            uint16_t* const o = y + (long long)(c + r) * ldy + f;
+            if (v16 && f + 8 <= features) {
+                *reinterpret_cast<uint4*>(o) = make_uint4(u[0], u[1], u[2], u[3]);
+            } else {
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    if (f + x < features) o[x] = (uint16_t)(u[x >> 1] >> (16 * (x & 1)));
+            }
+        }
+        const uint32_t next = other;
+        other = stage;
+        stage = next;
     }
 }
 

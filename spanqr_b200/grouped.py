@@ -9,6 +9,8 @@ x is [T, K] with the rows of expert e at offsets[e - 1] .. offsets[e] (offsets: 
 the rows per expert), w is [E, N, K], bf16 or fp16.  Everything runs on libspanqr's kernels on the current stream of x's
 device; the offsets are only read on the device, so nothing synchronises with the host.
 """
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -16,6 +18,20 @@ from . import _lib
 from .grads import DTYPES
 
 MAX_EXPERTS = 1024
+
+
+@functools.lru_cache(maxsize=4096)
+def _ws_bytes(fn, *sizes):
+    n = _lib.ctypes.c_size_t(0)
+    _lib.check(getattr(_lib.lib(), fn)(*sizes, _lib.ctypes.byref(n)), f"{fn}{sizes}")
+    return n.value
+
+
+def _workspace(fn, x, *sizes):
+    """a workspace for one call (None where it needs none), and its size: from torch's allocator each time, so that calls
+    on different streams and captured graphs never share one"""
+    n = _ws_bytes(fn, *sizes)
+    return (x.new_empty(n, dtype=torch.uint8), n) if n else (None, 0)
 
 
 def _up8(n):
@@ -110,9 +126,11 @@ def _mm(x, w, offsets, out=None):
         return y
     x, ldx = _rows(x)
     w, ldw, plane, transposed = _weights(w)
+    ws, n = _workspace("spanqr_mm_grouped_workspace_bytes", x, T, E, N, K)
     _lib.launch(x.get_device(), _lib.lib().spanqr_mm_grouped, lambda: f"mm_grouped({T}x{K}, {E} experts of {N}x{K})",
                 x.data_ptr(), ldx, w.data_ptr(), ldw, plane, transposed, offsets.data_ptr(), y.data_ptr(),
-                y.stride(0) if T > 1 else N, DTYPES[x.dtype], T, E, N, K, out is None)
+                y.stride(0) if T > 1 else N, DTYPES[x.dtype], T, E, N, K, out is None,
+                None if ws is None else ws.data_ptr(), n)
     return y
 
 

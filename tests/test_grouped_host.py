@@ -82,7 +82,7 @@ def test_overlap():
 
 
 def mm(x=A, ldx=64, w=A, ldw=64, sw=64 * 128, tr=0, off=A, y=A, ldy=128, type=BF16, T=16, E=2, N=128, K=64):
-    return _lib.lib().spanqr_mm_grouped(x, ldx, w, ldw, sw, tr, off, y, ldy, type, T, E, N, K, 1, None)
+    return _lib.lib().spanqr_mm_grouped(x, ldx, w, ldw, sw, tr, off, y, ldy, type, T, E, N, K, 1, None, 0, None)
 
 
 def wgrad(dy=A, lddy=128, x=A, ldx=64, off=A, dw=A, type=BF16, out=0, T=16, E=2, N=128, K=64):
