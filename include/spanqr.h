@@ -280,6 +280,9 @@ int spanqr_grad_clip(const void* const* in, const int* in_type, void* const* out
  *   `type`; zeros for an expert without rows.  Sums of 256 rows are taken by the tensor cores, their sums in fp32.
  * Both are deterministic.  Their workspaces (the _workspace_bytes of the same sizes, often 0, then ws may be NULL; 256-byte
  * aligned) need no initialisation; calls in flight at the same time need different ones.
+ * spanqr_mm_pad_rows: an operand that lies otherwise, copied to where these read it: planes x rows rows of `cols` 16-bit
+ *   elements (planes plane_stride and rows ld elements apart, >= 0, at any address) to consecutive rows of ldd elements (a
+ *   multiple of 8, >= cols; dst 16-byte aligned, not overlapping src).  What lies behind a row's cols is unspecified.
  * spanqr_mm_read_status: the word in which these kernels report, on the current device, a bounded device wait that ran
  *   out (0: none since the last read; else SPANQR_ERR_DEVICE, and results since then must not be used).  Clears it and
  *   synchronises `stream`.
@@ -288,8 +291,12 @@ int spanqr_mm_grouped_workspace_bytes(int T, int E, int N, int K, size_t* bytes)
 int spanqr_mm_grouped(const void* x, long long ldx, const void* w, long long ldw, long long stride_w, int w_transposed,
                       const int* offsets, void* y, long long ldy, int type, int T, int E, int N, int K, int zero_tail,
                       void* ws, size_t ws_bytes, spanqr_stream_t stream);
+int spanqr_mm_grouped_wgrad_workspace_bytes(int T, int E, int N, int K, size_t* bytes);
 int spanqr_mm_grouped_wgrad(const void* dy, long long lddy, const void* x, long long ldx, const int* offsets, void* dw,
-                            int type, int out_type, int T, int E, int N, int K, spanqr_stream_t stream);
+                            int type, int out_type, int T, int E, int N, int K, void* ws, size_t ws_bytes,
+                            spanqr_stream_t stream);
+int spanqr_mm_pad_rows(const void* src, long long plane_stride, long long ld, int planes, int rows, int cols, void* dst,
+                       int ldd, spanqr_stream_t stream);
 int spanqr_mm_read_status(spanqr_stream_t stream, int* device_status);
 
 #ifdef __cplusplus

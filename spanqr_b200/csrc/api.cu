@@ -32,10 +32,10 @@ int cuda_fail(cudaError_t e) {
 
 // ---- optional per-kernel timing (spanqr_timing_*) ----
 enum Kind { K_SETUP = 0, K_ABSMAX, K_GRAM, K_REDUCE, K_CHOL, K_TRSM_W, K_TRSM, K_NS, K_GRAM_ACC, K_COPY, K_BAND, K_PROJ, K_GRAD_SUMSQ, K_GRAD_SCALE,
-            K_MM, K_MM_WGRAD, K_COUNT };
+            K_MM, K_MM_WGRAD, K_PAD, K_COUNT };
 const char* const KIND_NAMES[K_COUNT] = {"k_setup", "k_absmax", "k_gram_tc", "k_gram_reduce", "k_chol", "k_trsm_w", "k_trsm",
                                          "k_ns_update", "k_gram_tc_acc", "k_scale_copy", "k_band_image", "k_project",
-                                         "k_grad_sumsq", "k_grad_scale", "k_mm", "k_mm_wgrad"};
+                                         "k_grad_sumsq", "k_grad_scale", "k_mm", "k_mm_wgrad", "k_pad_rows"};
 struct TimedLaunch {
     int kind;
     cudaEvent_t a, b;
@@ -1038,8 +1038,16 @@ int spanqr_mm_grouped(const void* x, long long ldx, const void* w, long long ldw
     return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
 }
 
+int spanqr_mm_grouped_wgrad_workspace_bytes(int T, int E, int N, int K, size_t* bytes) {
+    int rc = check_mm_sizes(T, E, N, K);
+    if (rc) return rc;
+    if (!bytes) return SPANQR_ERR_ARG;
+    *bytes = T > 0 ? mm_wgrad_plan(T, E, N, K, MAX_SMS).ws : 0;
+    return SPANQR_OK;
+}
+
 int spanqr_mm_grouped_wgrad(const void* dy, long long lddy, const void* x, long long ldx, const int* offsets, void* dw,
-                            int type, int out_type, int T, int E, int N, int K, spanqr_stream_t stream) {
+                            int type, int out_type, int T, int E, int N, int K, void* ws, size_t ws_bytes, spanqr_stream_t stream) {
     const int rc = check_mm(type, T, E, N, K, offsets);
     if (rc) return rc;
     const int os = type_bytes(out_type);
@@ -1051,9 +1059,27 @@ int spanqr_mm_grouped_wgrad(const void* dy, long long lddy, const void* x, long 
     }
     if (!mm_rows(dy, lddy, N) || !mm_rows(x, ldx, K)) return SPANQR_ERR_ARG;
     const MmOperand ody{dy, N, T, lddy, 0, 0, true}, ox{x, K, T, ldx, 0, 0, true};
-    const MmWgradArgs a{offsets, E, T, N, K, dw, type == SPANQR_BF16, out_type == SPANQR_F32, mm_status()};
+    int nsm = 0;
+    cudaError_t e = sm_count(&nsm);
+    if (e != cudaSuccess) return cuda_fail(e);
+    const MmWgradPlan plan = mm_wgrad_plan(T, E, N, K, nsm);
+    if (plan.ws && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0 || ws_bytes < plan.ws)) return SPANQR_ERR_WORKSPACE;
+    const MmWgradArgs a{offsets, E, T, N, K, dw, type == SPANQR_BF16, out_type == SPANQR_F32, 1, mm_status()};
     if (!a.status) return cuda_fail(cudaGetLastError());
-    const cudaError_t e = timed(K_MM_WGRAD, st, [&] { return launch_mm_wgrad(ody, ox, a, st); });
+    e = timed(K_MM_WGRAD, st, [&] { return launch_mm_wgrad(ody, ox, a, plan, static_cast<float*>(ws), st); },
+              plan.splits > 1 ? 2 : 1);
+    return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
+}
+
+int spanqr_mm_pad_rows(const void* src, long long plane_stride, long long ld, int planes, int rows, int cols, void* dst,
+                       int ldd, spanqr_stream_t stream) {
+    if (planes < 0 || planes > MM_MAX_E || rows < 0 || rows > MM_MAX_T || cols < 1 || cols > MM_MAX_DIM) return SPANQR_ERR_SHAPE;
+    if (planes == 0 || rows == 0) return SPANQR_OK;
+    if (!src || reinterpret_cast<uintptr_t>(src) % 2 || plane_stride < 0 || ld < 0 || !dst || !a16(dst) || ldd % 8 || ldd < cols)
+        return SPANQR_ERR_ARG;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const cudaError_t e =
+        timed(K_PAD, st, [&] { return launch_pad_rows(src, plane_stride, ld, planes, rows, cols, dst, ldd, st); });
     return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
 }
 

@@ -1,6 +1,7 @@
 // dw[e] = sum over expert e's rows of dy[t] x[t]^T (no reference counterpart): D = dy^T x in tiles of 256 features x 256
 // columns of x, on pairs of SMs (mm_pair.cuh).  Both operands are read as they lie, row by row (MN-major), in stages of 64
-// rows.
+// rows.  Where the tiles are fewer than the pairs, each expert's rows are cut into `splits` runs of whole stages with a
+// partial result each, and a second kernel adds those in order: the bits depend on the sizes alone.
 #include "mm_pair.cuh"
 
 namespace spq {
@@ -45,24 +46,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     k_mm_wgrad(const __grid_constant__ CUtensorMap tdy, const __grid_constant__ CUtensorMap tx,
                const __grid_constant__ CUtensorMap tdw, const MmWgradArgs a) {
     extern __shared__ char dyn[];
-    const Pair p = set_up<C>(dyn, a.offsets, a.E, a.T, 1 << 30);
+    if (a.splits > 1) launch_dependents();
+    const Pair p = set_up<C>(dyn, a.offsets, a.E, a.T, BK);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int ntn = (a.N + 2 * FT - 1) / (2 * FT), ntk = (a.K + NT - 1) / NT, per = ntn * ntk;
-    const long long tiles = (long long)a.E * per;
+    const long long tiles = (long long)a.E * a.splits * per;
     const int pairs = (int)gridDim.x / 2;
     struct Tile {
-        int e, n0, k0, cols, r0, rows, nb;   // cols: the tile's columns of x up to a multiple of 32; nb: stages of 64 rows
+        // plane: of the result, expert by expert and run by run; cols: the tile's columns of x up to a multiple of 32; rows
+        // r0 .. r0 + rows in nb stages
+        int plane, n0, k0, cols, r0, rows, nb;
     };
     auto tile_at = [&](long long i) {
         Tile t;
-        t.e = (int)(i / per);
-        const int l = (int)(i - (long long)t.e * per);
+        t.plane = (int)(i / per);
+        const int l = (int)(i - (long long)t.plane * per), e = t.plane / a.splits, run = t.plane - e * a.splits;
         t.n0 = l / ntk * 2 * FT;
         t.k0 = l % ntk * NT;
         t.cols = min(NT, up32(a.K - t.k0));
-        t.r0 = p.start[t.e];
-        t.rows = p.start[t.e + 1] - t.r0;
-        t.nb = (t.rows + BK - 1) / BK;
+        const int all = p.pre[e + 1] - p.pre[e], each = (all + a.splits - 1) / a.splits;   // stages of 64 rows
+        const int c0 = min(run * each, all);
+        t.nb = min(each, all - c0);
+        t.r0 = p.start[e] + c0 * BK;
+        t.rows = min(p.start[e + 1] - t.r0, t.nb * BK);
         return t;
     };
 
@@ -240,10 +246,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
                     if (TMA_OUT) {
                         tc::fence_async_smem();
                         __syncwarp();
-                        if (one) tma_store_3d(&tdw, k + c, n, d.e, tc::smem_u32(stage));
+                        if (one) tma_store_3d(&tdw, k + c, n, d.plane, tc::smem_u32(stage));
                     } else {
                         __syncwarp();
-                        store_rows(stage, static_cast<OUT*>(a.dw) + ((long long)d.e * a.N + n) * a.K + k + c, a.K,
+                        store_rows(stage, static_cast<OUT*>(a.dw) + ((long long)d.plane * a.N + n) * a.K + k + c, a.K,
                                    min(32, a.N - n), min(COLS, a.K - k - c));
                     }
                 }
@@ -254,27 +260,92 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tear_down<C>(p, a.status);
 }
 
+// the runs' partial results (rows of ldp floats, a multiple of 4), added in order: one thread, four columns of one row
+template <typename OUT>
+__global__ void __launch_bounds__(256) k_mm_wgrad_join(const MmWgradArgs a, const float* __restrict__ part, int ldp) {
+    const int quads = ldp / 4;
+    const long long plane = (long long)a.N * ldp, all = (long long)a.E * a.N * quads;
+    wait_primary();
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
+        const long long row = i / quads;   // of all experts
+        const int k = (int)(i - row * quads) * 4;
+        const long long e = row / a.N;
+        const float* p = part + e * a.splits * plane + (row - e * a.N) * ldp + k;
+        float4 s = *reinterpret_cast<const float4*>(p);
+#pragma unroll 4
+        for (int r = 1; r < a.splits; ++r) {
+            p += plane;
+            const float4 v = *reinterpret_cast<const float4*>(p);
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+        OUT* const o = static_cast<OUT*>(a.dw) + row * a.K + k;
+        const float v[4] = {s.x, s.y, s.z, s.w};
+        if (k + 4 <= a.K && reinterpret_cast<uintptr_t>(o) % (4 * sizeof(OUT)) == 0) {
+            if constexpr (sizeof(OUT) == 4) *reinterpret_cast<float4*>(o) = s;
+            else *reinterpret_cast<uint2*>(o) = make_uint2(pack16(s.x, s.y, a.bf16), pack16(s.z, s.w, a.bf16));
+        } else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                if (k + x < a.K) {
+                    if constexpr (sizeof(OUT) == 4) o[x] = v[x];
+                    else o[x] = to16(v[x], a.bf16);
+                }
+            }
+        }
+    }
+}
+
+constexpr int MIN_STAGES = 8;   // of a run
+
 }  // namespace
 
-cudaError_t launch_mm_wgrad(const MmOperand& dy, const MmOperand& x, const MmWgradArgs& a, cudaStream_t st) {
-    const int size = a.out32 ? 4 : 2;
-    const bool rows16 = reinterpret_cast<uintptr_t>(a.dw) % 16 == 0 && (long long)a.K * size % 16 == 0;
+MmWgradPlan mm_wgrad_plan(int T, int E, int N, int K, int nsm) {
+    MmWgradPlan p;
+    const long long tiles = (long long)E * ((N + 2 * FT - 1) / (2 * FT)) * ((K + NT - 1) / NT);
+    const long long stages = T / BK / E;   // of an average expert
+    long long s = nsm / 2 / tiles;
+    if (s > stages / MIN_STAGES) s = stages / MIN_STAGES;
+    // a stage takes about 0.3 us, the partial results and the second kernel about 4 us.  Measured (us, fp32 results): 2048
+    // rows, one expert of 768x512: 17.7 whole, 15.1 split four ways (24 of 32 stages saved); 4096 rows, 4 experts of 512x512:
+    // 15.8 whole, 17.4 split two ways (8 of 16); 32768 rows, one expert of 768x512: 162 whole, 35 split twelve ways
+    p.splits = s > 1 && stages * (s - 1) >= 16 * s ? (int)s : 1;
+    p.ldp = (K + 3) / 4 * 4;
+    p.tiles = tiles * p.splits;
+    p.ws = p.splits > 1 ? (size_t)E * p.splits * N * p.ldp * sizeof(float) : 0;
+    return p;
+}
+
+cudaError_t launch_mm_wgrad(const MmOperand& dy, const MmOperand& x, const MmWgradArgs& args, const MmWgradPlan& pl, float* ws,
+                            cudaStream_t st) {
+    MmWgradArgs a = args;
+    a.splits = pl.splits;
+    const bool split = pl.splits > 1;
+    if (split) a.dw = ws;   // the first kernel writes the partial results, in fp32
+    const bool out32 = a.out32 || split;
+    const int size = out32 ? 4 : 2, ld = split ? pl.ldp : a.K;
+    const bool rows16 = reinterpret_cast<uintptr_t>(a.dw) % 16 == 0 && (long long)ld * size % 16 == 0;
     alignas(64) CUtensorMap tdy, tx, tdw{};
     cudaError_t e = encode_mm(&tdy, dy, a.type(), 64, BK);
     if (e == cudaSuccess) e = encode_mm(&tx, x, a.type(), 64, BK);
     if (e == cudaSuccess && rows16)
-        e = encode_mm(&tdw, MmOperand{a.dw, a.K, a.N, a.K, a.E, (long long)a.N * a.K, false}, a.out32 ? DT_F32 : a.type(),
-                      128 / size, 32);
+        e = encode_mm(&tdw, MmOperand{a.dw, a.K, a.N, ld, a.E * a.splits, (long long)a.N * ld, false},
+                      out32 ? DT_F32 : a.type(), 128 / size, 32);
     int nsm = 0;
     if (e == cudaSuccess) e = sm_count(&nsm);
     if (e != cudaSuccess) return e;
-    const long long tiles = (long long)a.E * ((a.N + 2 * FT - 1) / (2 * FT)) * ((a.K + NT - 1) / NT);
-    const int pairs = (int)(tiles < nsm / 2 ? tiles : nsm / 2);
+    const int pairs = (int)(pl.tiles < nsm / 2 ? pl.tiles : nsm / 2);
     if (rows16)
-        return a.out32 ? launch_pairs<C, k_mm_wgrad<float, true>>(pairs, a.E, st, tdy, tx, tdw, a)
-                       : launch_pairs<C, k_mm_wgrad<uint16_t, true>>(pairs, a.E, st, tdy, tx, tdw, a);
-    return a.out32 ? launch_pairs<C, k_mm_wgrad<float, false>>(pairs, a.E, st, tdy, tx, tdw, a)
-                   : launch_pairs<C, k_mm_wgrad<uint16_t, false>>(pairs, a.E, st, tdy, tx, tdw, a);
+        e = out32 ? launch_pairs<C, k_mm_wgrad<float, true>>(pairs, a.E, st, tdy, tx, tdw, a)
+                  : launch_pairs<C, k_mm_wgrad<uint16_t, true>>(pairs, a.E, st, tdy, tx, tdw, a);
+    else
+        e = out32 ? launch_pairs<C, k_mm_wgrad<float, false>>(pairs, a.E, st, tdy, tx, tdw, a)
+                  : launch_pairs<C, k_mm_wgrad<uint16_t, false>>(pairs, a.E, st, tdy, tx, tdw, a);
+    if (e != cudaSuccess || !split) return e;
+    a.dw = args.dw;
+    const long long quads = (long long)a.E * a.N * (pl.ldp / 4), ctas = (quads + 255) / 256;
+    const dim3 grid((unsigned)(ctas < 8LL * nsm ? ctas : 8LL * nsm));
+    return a.out32 ? launch_join<k_mm_wgrad_join<float>>(grid, 256, 0, st, a, (const float*)ws, pl.ldp)
+                   : launch_join<k_mm_wgrad_join<uint16_t>>(grid, 256, 0, st, a, (const float*)ws, pl.ldp);
 }
 
 }  // namespace spq

@@ -224,10 +224,22 @@ struct MmWgradArgs {
     int E, T, N, K;
     void* dw;       // [E, N, K], fp32 (out32) or the operands' type
     bool bf16, out32;
+    int splits;     // runs of each expert's rows (set by launch_mm_wgrad)
     int* status;
     DType type() const { return bf16 ? DT_BF16 : DT_F16; }
 };
-// dw[e] = sum over e's rows of dy[t] x[t]^T
-cudaError_t launch_mm_wgrad(const MmOperand& dy, const MmOperand& x, const MmWgradArgs& a, cudaStream_t st);
+struct MmWgradPlan {
+    int splits;        // runs into which each expert's rows are cut
+    int ldp;           // row length of the runs' partial results
+    long long tiles;
+    size_t ws;         // bytes of workspace (0 without the split)
+};
+MmWgradPlan mm_wgrad_plan(int T, int E, int N, int K, int nsm);
+// dw[e] = sum over e's rows of dy[t] x[t]^T (ws: the plan's workspace)
+cudaError_t launch_mm_wgrad(const MmOperand& dy, const MmOperand& x, const MmWgradArgs& a, const MmWgradPlan& p, float* ws,
+                            cudaStream_t st);
+// 16-bit rows to rows of ldd elements (a multiple of 8) that start on 16 bytes
+cudaError_t launch_pad_rows(const void* src, long long plane_stride, long long ld, int planes, int rows, int cols, void* dst,
+                            int ldd, cudaStream_t st);
 
 }  // namespace spq

@@ -49,10 +49,16 @@ def _row_stride(ptr, rows, cols, ld, step):
 
 
 def _padded(t):
-    """a copy of t with its last dimension contiguous and every row on 16 bytes"""
-    buf = torch.empty((*t.shape[:-1], _up8(t.shape[-1])), dtype=t.dtype, device=t.device)
-    v = buf[..., :t.shape[-1]]
-    v.copy_(t)
+    """a copy of t (two or three dimensions) with its last dimension contiguous and every row on 16 bytes"""
+    cols, rows = t.shape[-1], t.shape[-2]
+    buf = t.new_empty((*t.shape[:-1], _up8(cols)))
+    v = buf[..., :cols]
+    if t.is_cuda and (t.stride(-1) == 1 or cols == 1):
+        planes, plane = (t.shape[0], t.stride(0)) if t.dim() == 3 else (1, 0)
+        _lib.launch(t.get_device(), _lib.lib().spanqr_mm_pad_rows, lambda: f"mm_pad_rows({planes}x{rows}x{cols})",
+                    t.data_ptr(), plane, t.stride(-2), planes, rows, cols, buf.data_ptr(), buf.shape[-1])
+    else:   # contiguous along another dimension, or along none
+        v.copy_(t)
     return v
 
 
@@ -78,6 +84,8 @@ def _weights(w):
                 return w, ld, _up8(need), transposed
             if se % 8 == 0 and se >= need:
                 return w, ld, se, transposed
+    if sn == 1 and sk != 1:   # stored [E, K, N]
+        return _padded(w.transpose(1, 2)).transpose(1, 2), _up8(N), K * _up8(N), True
     return _padded(w), _up8(K), N * _up8(K), False
 
 
@@ -140,15 +148,19 @@ def _wgrad(dy, x, offsets, dtype, out=None):
     dw = x.new_empty((E, N, K), dtype=dtype) if out is None else out
     dy, lddy = _rows(dy) if T else (dy, N)
     x, ldx = _rows(x) if T else (x, K)
+    ws, n = _workspace("spanqr_mm_grouped_wgrad_workspace_bytes", x, T, E, N, K)
     _lib.launch(x.get_device(), _lib.lib().spanqr_mm_grouped_wgrad,
                 lambda: f"mm_grouped_wgrad({T} rows, {E} experts of {N}x{K})", dy.data_ptr(), lddy, x.data_ptr(), ldx,
-                offsets.data_ptr(), dw.data_ptr(), DTYPES[x.dtype], DTYPES[dw.dtype], T, E, N, K)
+                offsets.data_ptr(), dw.data_ptr(), DTYPES[x.dtype], DTYPES[dw.dtype], T, E, N, K,
+                None if ws is None else ws.data_ptr(), n)
     return dw
 
 
 class _MmGrouped(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets):
+        # what had to be copied to be read is copied once for both passes
+        x, w = _rows(x)[0], _weights(w)[0]
         ctx.save_for_backward(x, w, offsets)
         return _mm(x, w, offsets)
 
@@ -156,6 +168,8 @@ class _MmGrouped(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
+        if dy.shape[0]:
+            dy = _rows(dy)[0]
         dx = _mm(dy, w.transpose(1, 2), offsets) if ctx.needs_input_grad[0] else None
         dw = _wgrad(dy, x, offsets, w.dtype) if ctx.needs_input_grad[1] else None
         return dx, dw, None
@@ -169,7 +183,7 @@ def mm_grouped(x, w, offsets, *, out=None):
     are summed in fp32 and rounded once.
 
     Operands whose rows do not start on 16 bytes (K not a multiple of 8, odd strides or addresses), or that are contiguous
-    along neither dimension, are copied first.  Ends that decrease or lie outside [0, T] are clamped to the nearest that
+    along neither dimension, are copied first (and kept so for the backward pass).  Ends that decrease or lie outside [0, T] are clamped to the nearest that
     do not, on the device.
 
     Differentiable once in x and w (without `out`): dx is this product with the transposed weights, dw is

@@ -203,6 +203,19 @@ def test_given_output_rows(T, ld, at):
     assert bool((buf[:, :at] == 9).all()) and bool((buf[:, at + N:] == 9).all())
 
 
+@pytest.mark.parametrize("planes,rows,cols,ld,plane,at", [
+    (1, 1, 1, 1, 1, 0), (1, 5, 7, 7, 35, 1), (3, 9, 61, 61, 9 * 61, 3), (2, 33, 64, 65, 33 * 65, 5), (4, 17, 100, 0, 7, 2),
+    (2, 1000, 777, 777, 1000 * 777, 7), (1, 3, 8, 8, 24, 8)])
+def test_padded_rows(planes, rows, cols, ld, plane, at):
+    """rows at every alignment, up to the last element of their allocation"""
+    n = at + (planes - 1) * plane + (rows - 1) * ld + cols
+    src = torch.arange(n, device="cuda", dtype=torch.int32).to(torch.int16).view(FP16)
+    t = src.as_strided((planes, rows, cols), (plane, ld, 1), at)
+    from spanqr_b200.grouped import _padded
+    v = _padded(t)
+    assert torch.equal(v.view(torch.int16), t.view(torch.int16)) and v.stride(1) % 8 == 0 and v.data_ptr() % 16 == 0
+
+
 def test_wgrad_into_given_output():
     dy, x = ints((200, 72), 1, BF16), ints((200, 136), 2, BF16)
     off = offsets([90, 110])

@@ -59,7 +59,7 @@ def test_row_operands(make, copied, ld):
     ((3, 64, 32), (2048, 1, 64), False, True),         # [E, K, N] seen as [E, N, K]
     ((3, 32, 61), (32 * 61, 61, 1), True, False),      # odd rows
     ((3, 61, 32), (61 * 32, 32, 1), False, False),     # odd N only
-    ((3, 61, 32), (61 * 32, 1, 61), True, False),      # odd rows of the transposed storage
+    ((3, 61, 32), (61 * 32, 1, 61), True, True),       # odd rows of the transposed storage
     ((3, 32, 64), (0, 64, 1), True, False),            # one matrix for all experts
     ((1, 32, 64), (5, 64, 1), False, False),           # a single expert's stride is free
     ((3, 32, 64), (2052, 64, 1), True, False),         # experts off 16 bytes
@@ -86,7 +86,7 @@ def mm(x=A, ldx=64, w=A, ldw=64, sw=64 * 128, tr=0, off=A, y=A, ldy=128, type=BF
 
 
 def wgrad(dy=A, lddy=128, x=A, ldx=64, off=A, dw=A, type=BF16, out=0, T=16, E=2, N=128, K=64):
-    return _lib.lib().spanqr_mm_grouped_wgrad(dy, lddy, x, ldx, off, dw, type, out, T, E, N, K, None)
+    return _lib.lib().spanqr_mm_grouped_wgrad(dy, lddy, x, ldx, off, dw, type, out, T, E, N, K, None, 0, None)
 
 
 def test_argument_checks_before_any_device_work():
@@ -100,5 +100,13 @@ def test_argument_checks_before_any_device_work():
     for bad in (dict(dy=None), dict(dy=A + 8), dict(lddy=120), dict(lddy=132), dict(x=None), dict(ldx=60), dict(off=None),
                 dict(dw=None), dict(dw=A + 2), dict(out=2, dw=A + 1), dict(out=1), dict(out=3), dict(type=0)):
         assert wgrad(**bad) == ARG, bad
+    pad = lambda src=A + 2, plane=999, ld=37, planes=2, rows=27, cols=37, dst=A, ldd=40: _lib.lib().spanqr_mm_pad_rows(  # noqa: E731
+        src, plane, ld, planes, rows, cols, dst, ldd, None)
+    for bad in (dict(planes=-1), dict(planes=1025), dict(rows=-1), dict(cols=0)):
+        assert pad(**bad) == SHAPE, bad
+    for bad in (dict(src=None), dict(src=A + 1), dict(plane=-1), dict(ld=-1), dict(dst=None), dict(dst=A + 8), dict(ldd=36),
+                dict(ldd=32)):
+        assert pad(**bad) == ARG, bad
+    assert pad(rows=0) == OK
     assert mm(T=0) == OK                 # nothing to do
     assert _lib.lib().spanqr_mm_read_status(None, None) == ARG
