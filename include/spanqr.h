@@ -270,33 +270,34 @@ int spanqr_grad_clip(const void* const* in, const int* in_type, void* const* out
  * orth take).  x [T, K] and dy, y [T, N] are row-major 16-bit matrices (type SPANQR_F16 or SPANQR_BF16, all alike) whose
  * rows are sorted by expert: expert e's rows are offsets[e - 1] .. offsets[e] (offsets: DEVICE array of E ends, read on
  * the device; ends that decrease or lie outside [0, T] are clamped to the nearest that do not).  1 <= E <= 1024,
- * 0 <= T <= 2^30, 1 <= N, K <= 2^24.  x, w and dy: 16-byte aligned, leading dimensions and expert strides multiples of 8.
+ * 0 <= T <= 2^30, 1 <= N, K <= 2^24.  Leading dimensions and expert strides are not negative.
  *
- * spanqr_mm_grouped: y[t] = w[e(t)] x[t], summed in fp32 and rounded once.  w holds E matrices, stride_w elements apart
- *   (without overlap): N x K with leading dimension ldw, or with w_transposed K x N, so that dx = the product of dy with
- *   the transposed weights is the same call.  y: any address and leading dimension >= N; it must overlap no input.  Rows
- *   from offsets[E - 1] on are zeroed (zero_tail != 0) or left as they are.
+ * spanqr_mm_grouped: y[t] = w[e(t)] x[t], summed in fp32 and rounded once.  w holds E matrices, stride_w elements apart: N x
+ *   K with leading dimension ldw, or with w_transposed K x N, so that dx = the product of dy with the transposed weights is
+ *   the same call.  y: any address and leading dimension >= N; it must overlap no input.  Rows from offsets[E - 1] on are
+ *   zeroed (zero_tail != 0) or left as they are.
  * spanqr_mm_grouped_wgrad: dw[e] = sum over e's rows of dy[t] x[t]^T, dw [E, N, K] contiguous, of out_type SPANQR_F32 or
- *   `type`; zeros for an expert without rows.  Sums of 256 rows are taken by the tensor cores, their sums in fp32.
- * Both are deterministic.  Their workspaces (the _workspace_bytes of the same sizes, often 0, then ws may be NULL; 256-byte
- * aligned) need no initialisation; calls in flight at the same time need different ones.
- * spanqr_mm_pad_rows: an operand that lies otherwise, copied to where these read it: planes x rows rows of `cols` 16-bit
- *   elements (planes plane_stride and rows ld elements apart, >= 0, at any address) to consecutive rows of ldd elements (a
- *   multiple of 8, >= cols; dst 16-byte aligned, not overlapping src).  What lies behind a row's cols is unspecified.
+ *   `type`; zeros for an expert without rows.  Summed by the tensor cores over 512 rows (fp32 results) or 2048, those sums
+ *   in fp32 to nearest.
+ * Operands are read where they lie if every row starts on 16 bytes and none overlap (a 16-byte aligned address, leading
+ *   dimension and, for E > 1, expert stride multiples of 8, leading dimension >= the row, expert stride >= the matrix); others are first
+ *   copied to the workspace.
+ * The workspaces, 256-byte aligned, need no initialisation; calls in flight at the same time need different ones.  Their
+ *   sizes (often 0, then ws may be NULL) come from the _workspace_bytes of the same sizes, where `copies` says which
+ *   operands have to be copied: 1 the first, 2 the second (plus 4 if the weights are transposed).
+ * Both are deterministic.
  * spanqr_mm_read_status: the word in which these kernels report, on the current device, a bounded device wait that ran
  *   out (0: none since the last read; else SPANQR_ERR_DEVICE, and results since then must not be used).  Clears it and
  *   synchronises `stream`.
  */
-int spanqr_mm_grouped_workspace_bytes(int T, int E, int N, int K, size_t* bytes);
+int spanqr_mm_grouped_workspace_bytes(int T, int E, int N, int K, int copies, size_t* bytes);
 int spanqr_mm_grouped(const void* x, long long ldx, const void* w, long long ldw, long long stride_w, int w_transposed,
                       const int* offsets, void* y, long long ldy, int type, int T, int E, int N, int K, int zero_tail,
                       void* ws, size_t ws_bytes, spanqr_stream_t stream);
-int spanqr_mm_grouped_wgrad_workspace_bytes(int T, int E, int N, int K, size_t* bytes);
+int spanqr_mm_grouped_wgrad_workspace_bytes(int T, int E, int N, int K, int copies, size_t* bytes);
 int spanqr_mm_grouped_wgrad(const void* dy, long long lddy, const void* x, long long ldx, const int* offsets, void* dw,
                             int type, int out_type, int T, int E, int N, int K, void* ws, size_t ws_bytes,
                             spanqr_stream_t stream);
-int spanqr_mm_pad_rows(const void* src, long long plane_stride, long long ld, int planes, int rows, int cols, void* dst,
-                       int ldd, spanqr_stream_t stream);
 int spanqr_mm_read_status(spanqr_stream_t stream, int* device_status);
 
 #ifdef __cplusplus

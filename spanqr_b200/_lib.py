@@ -48,11 +48,10 @@ SIGNATURES = {
     "spanqr_grad_workspace_bytes": (_I, [_I, ctypes.POINTER(_SZ)]),
     "spanqr_grad_norm": (_I, [_P, _P, _P, _I, _P, _P, _P, _SZ, _P]),
     "spanqr_grad_clip": (_I, [_P, _P, _P, _P, _P, _I, _D, _P, _P, _P, _SZ, _P]),
-    "spanqr_mm_grouped_workspace_bytes": (_I, [_I, _I, _I, _I, ctypes.POINTER(_SZ)]),
+    "spanqr_mm_grouped_workspace_bytes": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(_SZ)]),
     "spanqr_mm_grouped": (_I, [_P, _LL, _P, _LL, _LL, _I, _P, _P, _LL, _I, _I, _I, _I, _I, _I, _P, _SZ, _P]),
-    "spanqr_mm_grouped_wgrad_workspace_bytes": (_I, [_I, _I, _I, _I, ctypes.POINTER(_SZ)]),
+    "spanqr_mm_grouped_wgrad_workspace_bytes": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(_SZ)]),
     "spanqr_mm_grouped_wgrad": (_I, [_P, _LL, _P, _LL, _P, _P, _I, _I, _I, _I, _I, _I, _P, _SZ, _P]),
-    "spanqr_mm_pad_rows": (_I, [_P, _LL, _LL, _I, _I, _I, _P, _I, _P]),
     "spanqr_mm_read_status": (_I, [_P, ctypes.POINTER(_I)]),
 }
 

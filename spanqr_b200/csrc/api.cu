@@ -998,18 +998,54 @@ int check_mm(int type, int T, int E, int N, int K, const int* offsets) {
         return SPANQR_ERR_ARG;
     return SPANQR_OK;
 }
-// a row-major 16-bit operand that TMA can read: 16-byte aligned rows that do not overlap
-bool mm_rows(const void* p, long long ld, long long cols) { return p && a16(p) && ld >= cols && ld % 8 == 0 && ld < (1LL << 38); }
+// A 16-bit operand of rows in planes as the caller has it, and as TMA can read it: as it is, or copied to the workspace.
+struct Rows {
+    const void* p;
+    long long cols, rows, ld;
+    int planes;
+    long long plane;
+    bool mn;
+    bool valid() const {   // elements at their alignment, no negative steps
+        return p && reinterpret_cast<uintptr_t>(p) % 2 == 0 && ld >= 0 && plane >= 0 && ld < (1LL << 38) && plane < (1LL << 38);
+    }
+    bool readable() const {   // rows on 16 bytes that do not overlap
+        return a16(p) && (rows == 1 || (ld % 8 == 0 && ld >= cols)) &&
+               (planes <= 1 || (plane % 8 == 0 && plane >= (rows - 1) * ld + cols));
+    }
+};
+size_t copy_bytes(long long planes, long long rows, long long cols) {
+    return al256((size_t)planes * rows * ((cols + 7) / 8 * 8) * 2);
+}
+// the operand for the kernel; what has to be copied becomes a job and takes its place in the workspace at `at`
+MmOperand readable(const Rows& r, bool three, char*& at, PadJob* jobs, int& count) {
+    const long long cols8 = (r.cols + 7) / 8 * 8;
+    MmOperand o{r.p, r.cols, r.rows, r.rows > 1 ? r.ld : cols8, three ? r.planes : 0, r.plane, r.mn};
+    if (!r.readable()) {
+        jobs[count++] = PadJob{r.p, r.plane, r.ld, r.planes, (int)r.rows, (int)r.cols, at};
+        o.p = at;
+        o.ld = cols8;
+        o.plane = r.rows * cols8;
+        at += copy_bytes(r.planes, r.rows, r.cols);
+    } else if (r.planes <= 1) {
+        o.plane = r.rows * o.ld;
+    }
+    return o;
+}
+bool ws_ok(const void* ws, size_t have, size_t need) {
+    return need == 0 || (ws && (reinterpret_cast<uintptr_t>(ws) & 255u) == 0 && have >= need);
+}
 }  // namespace
 
 extern "C" {
 
-int spanqr_mm_grouped_workspace_bytes(int T, int E, int N, int K, size_t* bytes) {
-    int rc = check_mm_sizes(T, E, N, K);
+int spanqr_mm_grouped_workspace_bytes(int T, int E, int N, int K, int copies, size_t* bytes) {
+    const int rc = check_mm_sizes(T, E, N, K);
     if (rc) return rc;
-    if (!bytes) return SPANQR_ERR_ARG;
-    // the largest that a device of any number of SMs needs (a plan on more pairs splits no less)
-    *bytes = T > 0 ? mm_plan(T, E, N, K, MAX_SMS).ws : 0;
+    if (!bytes || copies < 0 || copies > 7) return SPANQR_ERR_ARG;
+    // the plan on the most SMs: one on fewer splits no more
+    *bytes = T > 0 ? al256(mm_plan(T, E, N, K, MAX_SMS).ws) + (copies & 1 ? copy_bytes(1, T, K) : 0) +
+                         (copies & 2 ? copies & 4 ? copy_bytes(E, K, N) : copy_bytes(E, N, K) : 0)
+                   : 0;
     return SPANQR_OK;
 }
 
@@ -1019,35 +1055,42 @@ int spanqr_mm_grouped(const void* x, long long ldx, const void* w, long long ldw
     const int rc = check_mm(type, T, E, N, K, offsets);
     if (rc) return rc;
     if (T == 0) return SPANQR_OK;
-    const long long wcols = w_transposed ? N : K, wrows = w_transposed ? K : N;
-    if (!mm_rows(x, ldx, K) || !mm_rows(w, ldw, wcols) || !y || reinterpret_cast<uintptr_t>(y) % 2 || ldy < N)
-        return SPANQR_ERR_ARG;
-    if (stride_w % 8 || (E > 1 && stride_w < (wrows - 1) * ldw + wcols) || stride_w >= (1LL << 38)) return SPANQR_ERR_ARG;
-    const MmOperand ox{x, K, T, ldx, 0, 0, false};
-    const MmOperand ow{w, wcols, wrows, ldw, E, E > 1 ? stride_w : wrows * ldw, w_transposed != 0};
+    const Rows rx{x, K, T, ldx, 1, 0, false};
+    const Rows rw{w, w_transposed ? N : K, w_transposed ? K : N, ldw, E, E > 1 ? stride_w : 0, w_transposed != 0};
+    if (!rx.valid() || !rw.valid() || !y || reinterpret_cast<uintptr_t>(y) % 2 || (T > 1 && ldy < N)) return SPANQR_ERR_ARG;
     int nsm = 0;
     cudaError_t e = sm_count(&nsm);
     if (e != cudaSuccess) return cuda_fail(e);
     const MmPlan plan = mm_plan(T, E, N, K, nsm);
-    if (plan.ws && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0 || ws_bytes < plan.ws)) return SPANQR_ERR_WORKSPACE;
-    const MmArgs a{offsets, E, T, N, K, static_cast<uint16_t*>(y), ldy, (N + 255) / 256, plan.ws ? static_cast<float*>(ws) : nullptr,
-                   type == SPANQR_BF16, zero_tail != 0, mm_status()};
+    const size_t need = al256(plan.ws) + (rx.readable() ? 0 : copy_bytes(1, T, K)) +
+                        (rw.readable() ? 0 : copy_bytes(E, rw.rows, rw.cols));
+    if (!ws_ok(ws, ws_bytes, need)) return SPANQR_ERR_WORKSPACE;
+    char* at = static_cast<char*>(ws) + al256(plan.ws);
+    PadJob jobs[2];
+    int njobs = 0;
+    const MmOperand ox = readable(rx, false, at, jobs, njobs), ow = readable(rw, true, at, jobs, njobs);
+    const MmArgs a{offsets, E, T, N, K, static_cast<uint16_t*>(y), T > 1 ? ldy : N, (N + 255) / 256,
+                   plan.ws ? static_cast<float*>(ws) : nullptr, type == SPANQR_BF16, zero_tail != 0, mm_status()};
     if (!a.status) return cuda_fail(cudaGetLastError());
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    e = timed(K_MM, st, [&] { return launch_mm(ox, ow, a, plan, st); }, plan.split ? 2 : 1);
+    if (njobs) e = timed(K_PAD, st, [&] { return launch_pad_rows(jobs, njobs, st); });
+    if (e == cudaSuccess) e = timed(K_MM, st, [&] { return launch_mm(ox, ow, a, plan, st); }, plan.split ? 2 : 1);
     return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
 }
 
-int spanqr_mm_grouped_wgrad_workspace_bytes(int T, int E, int N, int K, size_t* bytes) {
-    int rc = check_mm_sizes(T, E, N, K);
+int spanqr_mm_grouped_wgrad_workspace_bytes(int T, int E, int N, int K, int copies, size_t* bytes) {
+    const int rc = check_mm_sizes(T, E, N, K);
     if (rc) return rc;
-    if (!bytes) return SPANQR_ERR_ARG;
-    *bytes = T > 0 ? mm_wgrad_plan(T, E, N, K, MAX_SMS).ws : 0;
+    if (!bytes || copies < 0 || copies > 3) return SPANQR_ERR_ARG;
+    *bytes = T > 0 ? al256(mm_wgrad_plan(T, E, N, K, MAX_SMS).ws) + (copies & 1 ? copy_bytes(1, T, N) : 0) +
+                         (copies & 2 ? copy_bytes(1, T, K) : 0)
+                   : 0;
     return SPANQR_OK;
 }
 
 int spanqr_mm_grouped_wgrad(const void* dy, long long lddy, const void* x, long long ldx, const int* offsets, void* dw,
-                            int type, int out_type, int T, int E, int N, int K, void* ws, size_t ws_bytes, spanqr_stream_t stream) {
+                            int type, int out_type, int T, int E, int N, int K, void* ws, size_t ws_bytes,
+                            spanqr_stream_t stream) {
     const int rc = check_mm(type, T, E, N, K, offsets);
     if (rc) return rc;
     const int os = type_bytes(out_type);
@@ -1057,29 +1100,24 @@ int spanqr_mm_grouped_wgrad(const void* dy, long long lddy, const void* x, long 
         const cudaError_t e = cudaMemsetAsync(dw, 0, (size_t)E * N * K * os, st);
         return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
     }
-    if (!mm_rows(dy, lddy, N) || !mm_rows(x, ldx, K)) return SPANQR_ERR_ARG;
-    const MmOperand ody{dy, N, T, lddy, 0, 0, true}, ox{x, K, T, ldx, 0, 0, true};
+    const Rows rdy{dy, N, T, lddy, 1, 0, true}, rx{x, K, T, ldx, 1, 0, true};
+    if (!rdy.valid() || !rx.valid()) return SPANQR_ERR_ARG;
     int nsm = 0;
     cudaError_t e = sm_count(&nsm);
     if (e != cudaSuccess) return cuda_fail(e);
     const MmWgradPlan plan = mm_wgrad_plan(T, E, N, K, nsm);
-    if (plan.ws && (!ws || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0 || ws_bytes < plan.ws)) return SPANQR_ERR_WORKSPACE;
+    const size_t need = al256(plan.ws) + (rdy.readable() ? 0 : copy_bytes(1, T, N)) + (rx.readable() ? 0 : copy_bytes(1, T, K));
+    if (!ws_ok(ws, ws_bytes, need)) return SPANQR_ERR_WORKSPACE;
+    char* at = static_cast<char*>(ws) + al256(plan.ws);
+    PadJob jobs[2];
+    int njobs = 0;
+    const MmOperand ody = readable(rdy, false, at, jobs, njobs), ox = readable(rx, false, at, jobs, njobs);
     const MmWgradArgs a{offsets, E, T, N, K, dw, type == SPANQR_BF16, out_type == SPANQR_F32, 1, mm_status()};
     if (!a.status) return cuda_fail(cudaGetLastError());
-    e = timed(K_MM_WGRAD, st, [&] { return launch_mm_wgrad(ody, ox, a, plan, static_cast<float*>(ws), st); },
-              plan.splits > 1 ? 2 : 1);
-    return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
-}
-
-int spanqr_mm_pad_rows(const void* src, long long plane_stride, long long ld, int planes, int rows, int cols, void* dst,
-                       int ldd, spanqr_stream_t stream) {
-    if (planes < 0 || planes > MM_MAX_E || rows < 0 || rows > MM_MAX_T || cols < 1 || cols > MM_MAX_DIM) return SPANQR_ERR_SHAPE;
-    if (planes == 0 || rows == 0) return SPANQR_OK;
-    if (!src || reinterpret_cast<uintptr_t>(src) % 2 || plane_stride < 0 || ld < 0 || !dst || !a16(dst) || ldd % 8 || ldd < cols)
-        return SPANQR_ERR_ARG;
-    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    const cudaError_t e =
-        timed(K_PAD, st, [&] { return launch_pad_rows(src, plane_stride, ld, planes, rows, cols, dst, ldd, st); });
+    if (njobs) e = timed(K_PAD, st, [&] { return launch_pad_rows(jobs, njobs, st); });
+    if (e == cudaSuccess)
+        e = timed(K_MM_WGRAD, st, [&] { return launch_mm_wgrad(ody, ox, a, plan, static_cast<float*>(ws), st); },
+                  plan.splits > 1 ? 2 : 1);
     return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
 }
 

@@ -238,8 +238,14 @@ MmWgradPlan mm_wgrad_plan(int T, int E, int N, int K, int nsm);
 // dw[e] = sum over e's rows of dy[t] x[t]^T (ws: the plan's workspace)
 cudaError_t launch_mm_wgrad(const MmOperand& dy, const MmOperand& x, const MmWgradArgs& a, const MmWgradPlan& p, float* ws,
                             cudaStream_t st);
-// 16-bit rows to rows of ldd elements (a multiple of 8) that start on 16 bytes
-cudaError_t launch_pad_rows(const void* src, long long plane_stride, long long ld, int planes, int rows, int cols, void* dst,
-                            int ldd, cudaStream_t st);
+// planes x rows rows of cols 16-bit elements (planes `plane` and rows `ld` elements apart, any address) copied to consecutive
+// rows of cols elements rounded up to a multiple of 8, dst on 16 bytes; one or two such jobs in one launch
+struct PadJob {
+    const void* src;
+    long long plane, ld;
+    int planes, rows, cols;
+    void* dst;
+};
+cudaError_t launch_pad_rows(const PadJob* jobs, int count, cudaStream_t st);
 
 }  // namespace spq

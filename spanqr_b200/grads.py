@@ -21,6 +21,7 @@ from . import _lib
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _dtype, _shape = attrgetter("dtype"), attrgetter("shape")
 _contiguous = torch.Tensor.is_contiguous
+_PLAIN = {torch.Tensor, torch.nn.Parameter}
 _ptr, _numel, _device = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
 
 
@@ -39,9 +40,10 @@ def _check(tensors, name):
     if torch.is_tensor(tensors):
         raise TypeError(f"{name} must be a list of tensors (got one tensor)")
     ts = list(tensors)
-    if not all(map(torch.is_tensor, ts)):
+    if not set(map(type, ts)) <= _PLAIN and not all(map(torch.is_tensor, ts)):
         raise TypeError(f"{name} must hold tensors only")
-    kinds = set(map(_dtype, ts))
+    dtypes = list(map(_dtype, ts))
+    kinds = set(dtypes)
     if not kinds <= DTYPES.keys():
         raise TypeError(f"{name} must be fp32, fp16 or bf16 (got {', '.join(map(str, kinds - DTYPES.keys()))})")
     devs = set(map(_device, ts))
@@ -49,7 +51,7 @@ def _check(tensors, name):
         raise TypeError(f"{name} must be CUDA tensors")
     if len(devs) > 1:
         raise ValueError(f"{name} must be on one device (got cuda:{', cuda:'.join(map(str, sorted(devs)))})")
-    types = array("i", [DTYPES[kinds.pop()]]) * len(ts) if len(kinds) == 1 else array("i", map(DTYPES.get, map(_dtype, ts)))
+    types = array("i", [DTYPES[kinds.pop()]]) * len(ts) if len(kinds) == 1 else array("i", map(DTYPES.get, dtypes))
     return ts, types, devs.pop() if devs else None
 
 
@@ -160,7 +162,10 @@ def clip_grads(tensors, max_norm, *, out=None, group=None):
     sumsq = None if group is None else _group_sumsq(ins, types, dev, group)
     _run_clip(ins, types, res, out_types, dev, max_norm, sumsq, norm)
     if out is not None and res:
-        torch.autograd.graph.increment_version([o for o in res if not o.is_inference()])
+        try:
+            torch.autograd.graph.increment_version(res)
+        except RuntimeError:   # tensors of inference mode have no version
+            torch.autograd.graph.increment_version([o for o in res if not o.is_inference()])
     return res, norm
 
 

@@ -28,65 +28,41 @@ def _ws_bytes(fn, *sizes):
 
 
 def _workspace(fn, x, *sizes):
-    """a workspace for one call (None where it needs none), and its size: from torch's allocator each time, so that calls
-    on different streams and captured graphs never share one"""
+    """a workspace for one call (None where it needs none), its address and size: from torch's allocator each time, so that
+    calls on different streams and captured graphs never share one"""
     n = _ws_bytes(fn, *sizes)
-    return (x.new_empty(n, dtype=torch.uint8), n) if n else (None, 0)
-
-
-def _up8(n):
-    return -(-n // 8) * 8
-
-
-def _row_stride(ptr, rows, cols, ld, step):
-    """the row stride of an operand the copy engine can read (16-byte aligned rows of contiguous elements), or None: `rows`
-    rows `ld` elements apart, of `cols` elements `step` apart"""
-    if step != 1 and cols > 1 or ptr % 16:
-        return None
-    if rows == 1:
-        return _up8(cols)   # a single row's stride is free
-    return ld if ld % 8 == 0 and ld >= cols else None
-
-
-def _padded(t):
-    """a copy of t (two or three dimensions) with its last dimension contiguous and every row on 16 bytes"""
-    cols, rows = t.shape[-1], t.shape[-2]
-    buf = t.new_empty((*t.shape[:-1], _up8(cols)))
-    v = buf[..., :cols]
-    if t.is_cuda and (t.stride(-1) == 1 or cols == 1):
-        planes, plane = (t.shape[0], t.stride(0)) if t.dim() == 3 else (1, 0)
-        _lib.launch(t.get_device(), _lib.lib().spanqr_mm_pad_rows, lambda: f"mm_pad_rows({planes}x{rows}x{cols})",
-                    t.data_ptr(), plane, t.stride(-2), planes, rows, cols, buf.data_ptr(), buf.shape[-1])
-    else:   # contiguous along another dimension, or along none
-        v.copy_(t)
-    return v
+    if n == 0:
+        return None, None, 0
+    ws = x.new_empty(n, dtype=torch.uint8)
+    return ws, ws.data_ptr(), n
 
 
 def _rows(x):
-    """x [T, K] (or a padded copy) and its row stride"""
-    T, K = x.shape
-    ld = _row_stride(x.data_ptr(), T, K, *x.stride())
-    if ld is None:
-        x, ld = _padded(x), _up8(K)
-    return x, ld
+    """x [T, K] with contiguous rows, its address and row stride, and whether the library has to copy it to read it (rows
+    off 16 bytes or over one another)"""
+    ld, step = x.stride()
+    if step != 1 and x.shape[1] > 1 or ld < 0:
+        x = x.contiguous()
+        ld = x.stride(0)
+    ptr = x.data_ptr()
+    return x, ptr, ld, ptr % 16 != 0 or x.shape[0] > 1 and (ld % 8 != 0 or ld < x.shape[1])
 
 
 def _weights(w):
-    """w [E, N, K] (or a padded copy), its row stride, its expert stride and whether it is stored [E, K, N]"""
+    """w [E, N, K] with one of its last two dimensions contiguous, its address, row stride, expert stride, whether it is
+    stored [E, K, N], and whether the library has to copy it to read it"""
     E, N, K = w.shape
-    se, sn, sk = w.stride()
+    plane, sn, sk = w.stride()
+    if sk == 1 or K == 1:
+        rows, cols, ld, transposed = N, K, sn, False
+    elif sn == 1 or N == 1:
+        rows, cols, ld, transposed = K, N, sk, True
+    else:
+        return _weights(w.contiguous())
     ptr = w.data_ptr()
-    for transposed, rows, cols, ld, step in ((False, N, K, sn, sk), (True, K, N, sk, sn)):
-        ld = _row_stride(ptr, rows, cols, ld, step)
-        if ld is not None:
-            need = (rows - 1) * ld + cols
-            if E == 1:
-                return w, ld, _up8(need), transposed
-            if se % 8 == 0 and se >= need:
-                return w, ld, se, transposed
-    if sn == 1 and sk != 1:   # stored [E, K, N]
-        return _padded(w.transpose(1, 2)).transpose(1, 2), _up8(N), K * _up8(N), True
-    return _padded(w), _up8(K), N * _up8(K), False
+    copy = (ptr % 16 != 0 or rows > 1 and (ld % 8 != 0 or ld < cols) or
+            E > 1 and (plane % 8 != 0 or plane < (rows - 1) * ld + cols))
+    return w, ptr, ld, plane, transposed, copy
 
 
 def _span(t):
@@ -132,13 +108,12 @@ def _mm(x, w, offsets, out=None):
     y = x.new_empty((T, N)) if out is None else out
     if T == 0:
         return y
-    x, ldx = _rows(x)
-    w, ldw, plane, transposed = _weights(w)
-    ws, n = _workspace("spanqr_mm_grouped_workspace_bytes", x, T, E, N, K)
-    _lib.launch(x.get_device(), _lib.lib().spanqr_mm_grouped, lambda: f"mm_grouped({T}x{K}, {E} experts of {N}x{K})",
-                x.data_ptr(), ldx, w.data_ptr(), ldw, plane, transposed, offsets.data_ptr(), y.data_ptr(),
-                y.stride(0) if T > 1 else N, DTYPES[x.dtype], T, E, N, K, out is None,
-                None if ws is None else ws.data_ptr(), n)
+    x, px, ldx, copy_x = _rows(x)
+    w, pw, ldw, plane, transposed, copy_w = _weights(w)
+    ws, pws, n = _workspace("spanqr_mm_grouped_workspace_bytes", x, T, E, N, K, copy_x + 2 * copy_w + 4 * transposed)
+    _lib.launch(x.get_device(), _lib.lib().spanqr_mm_grouped, lambda: f"mm_grouped({T}x{K}, {E} experts of {N}x{K})", px, ldx,
+                pw, ldw, plane, transposed, offsets.data_ptr(), y.data_ptr(), y.stride(0), DTYPES[x.dtype], T, E, N, K,
+                out is None, pws, n)
     return y
 
 
@@ -146,21 +121,18 @@ def _wgrad(dy, x, offsets, dtype, out=None):
     T, N = dy.shape
     K, E = x.shape[1], offsets.shape[0]
     dw = x.new_empty((E, N, K), dtype=dtype) if out is None else out
-    dy, lddy = _rows(dy) if T else (dy, N)
-    x, ldx = _rows(x) if T else (x, K)
-    ws, n = _workspace("spanqr_mm_grouped_wgrad_workspace_bytes", x, T, E, N, K)
+    dy, pdy, lddy, copy_dy = _rows(dy)
+    x, px, ldx, copy_x = _rows(x)
+    ws, pws, n = _workspace("spanqr_mm_grouped_wgrad_workspace_bytes", x, T, E, N, K, copy_dy + 2 * copy_x)
     _lib.launch(x.get_device(), _lib.lib().spanqr_mm_grouped_wgrad,
-                lambda: f"mm_grouped_wgrad({T} rows, {E} experts of {N}x{K})", dy.data_ptr(), lddy, x.data_ptr(), ldx,
-                offsets.data_ptr(), dw.data_ptr(), DTYPES[x.dtype], DTYPES[dw.dtype], T, E, N, K,
-                None if ws is None else ws.data_ptr(), n)
+                lambda: f"mm_grouped_wgrad({T} rows, {E} experts of {N}x{K})", pdy, lddy, px, ldx, offsets.data_ptr(),
+                dw.data_ptr(), DTYPES[x.dtype], DTYPES[dw.dtype], T, E, N, K, pws, n)
     return dw
 
 
 class _MmGrouped(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets):
-        # what had to be copied to be read is copied once for both passes
-        x, w = _rows(x)[0], _weights(w)[0]
         ctx.save_for_backward(x, w, offsets)
         return _mm(x, w, offsets)
 
@@ -168,8 +140,6 @@ class _MmGrouped(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
-        if dy.shape[0]:
-            dy = _rows(dy)[0]
         dx = _mm(dy, w.transpose(1, 2), offsets) if ctx.needs_input_grad[0] else None
         dw = _wgrad(dy, x, offsets, w.dtype) if ctx.needs_input_grad[1] else None
         return dx, dw, None
@@ -183,7 +153,7 @@ def mm_grouped(x, w, offsets, *, out=None):
     are summed in fp32 and rounded once.
 
     Operands whose rows do not start on 16 bytes (K not a multiple of 8, odd strides or addresses), or that are contiguous
-    along neither dimension, are copied first (and kept so for the backward pass).  Ends that decrease or lie outside [0, T] are clamped to the nearest that
+    along neither dimension, are copied first, at each call.  Ends that decrease or lie outside [0, T] are clamped to the nearest that
     do not, on the device.
 
     Differentiable once in x and w (without `out`): dx is this product with the transposed weights, dw is

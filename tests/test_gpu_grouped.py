@@ -203,17 +203,23 @@ def test_given_output_rows(T, ld, at):
     assert bool((buf[:, :at] == 9).all()) and bool((buf[:, at + N:] == 9).all())
 
 
-@pytest.mark.parametrize("planes,rows,cols,ld,plane,at", [
-    (1, 1, 1, 1, 1, 0), (1, 5, 7, 7, 35, 1), (3, 9, 61, 61, 9 * 61, 3), (2, 33, 64, 65, 33 * 65, 5), (4, 17, 100, 0, 7, 2),
-    (2, 1000, 777, 777, 1000 * 777, 7), (1, 3, 8, 8, 24, 8)])
-def test_padded_rows(planes, rows, cols, ld, plane, at):
-    """rows at every alignment, up to the last element of their allocation"""
-    n = at + (planes - 1) * plane + (rows - 1) * ld + cols
-    src = torch.arange(n, device="cuda", dtype=torch.int32).to(torch.int16).view(FP16)
-    t = src.as_strided((planes, rows, cols), (plane, ld, 1), at)
-    from spanqr_b200.grouped import _padded
-    v = _padded(t)
-    assert torch.equal(v.view(torch.int16), t.view(torch.int16)) and v.stride(1) % 8 == 0 and v.data_ptr() % 16 == 0
+@pytest.mark.parametrize("at", [0, 1, 2, 3, 5, 7, 8])
+@pytest.mark.parametrize("K,extra", [(1, 0), (7, 0), (61, 0), (64, 1), (100, 3), (777, 0)])
+def test_operands_at_every_alignment(at, K, extra):
+    """x, w and dy up to the last element of their allocation, NaN between their rows"""
+    T, E, N = 37, 2, 19
+
+    def operand(planes, rows, cols, seed):
+        ld = cols + extra
+        flat = torch.full((at + (planes * rows - 1) * ld + cols,), float("nan"), dtype=FP16, device="cuda")
+        t = flat.as_strided((planes, rows, cols), (rows * ld, ld, 1), at)
+        t.copy_(ints((planes, rows, cols), seed, FP16))
+        return t
+    x, w, dy, wt = operand(1, T, K, 1)[0], operand(E, N, K, 2), operand(1, T, N, 3)[0], operand(E, K, N, 4).transpose(1, 2)
+    off = offsets([20, 17])
+    for v in (w, wt):
+        assert torch.equal(mm_grouped(x, v, off), exact_mm(x, v, off).to(FP16))
+    assert torch.equal(mm_grouped_wgrad(dy, x, off), exact_wgrad(dy, x, off).to(F32))
 
 
 def test_wgrad_into_given_output():

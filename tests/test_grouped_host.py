@@ -40,37 +40,35 @@ def test_offset_checks():
     assert g._check_offsets(o, x).is_contiguous()
 
 
-@pytest.mark.parametrize("make,copied,ld", [
-    (lambda: torch.zeros(5, 64), False, 64), (lambda: torch.zeros(5, 61), True, 64),
-    (lambda: torch.zeros(5, 128)[:, :61], False, 128), (lambda: torch.zeros(5, 128)[:, 1:62], True, 64),
-    (lambda: torch.zeros(64, 5).t(), True, 64), (lambda: torch.zeros(1, 64).expand(5, 64), True, 64),
-    (lambda: torch.zeros(5, 100)[:, :64], True, 64), (lambda: torch.zeros(9, 64)[::2], False, 128),
-    (lambda: torch.zeros(1, 61), False, 64), (lambda: torch.zeros(5, 1), True, 8)])
-def test_row_operands(make, copied, ld):
+@pytest.mark.parametrize("make,contiguous,copied", [
+    (lambda: torch.zeros(5, 64), False, False), (lambda: torch.zeros(5, 61), False, True),
+    (lambda: torch.zeros(5, 128)[:, :61], False, False), (lambda: torch.zeros(5, 128)[:, 1:62], False, True),
+    (lambda: torch.zeros(64, 5).t(), True, False), (lambda: torch.zeros(1, 64).expand(5, 64), False, True),
+    (lambda: torch.zeros(5, 100)[:, :64], False, True), (lambda: torch.zeros(9, 64)[::2], False, False),
+    (lambda: torch.zeros(1, 61), False, False), (lambda: torch.zeros(5, 1), False, True)])
+def test_row_operands(make, contiguous, copied):
+    """made contiguous where its rows are not; left to the library to copy where its rows are off 16 bytes or overlap"""
     base = make()
     x = torch.zeros(4096, dtype=torch.bfloat16).as_strided(base.shape, base.stride(), base.storage_offset())
-    y, got = g._rows(x)
-    assert (y.data_ptr() != x.data_ptr()) is copied and got == ld
-    assert got % 8 == 0 and y.data_ptr() % 16 == 0
+    y, ptr, ld, copy = g._rows(x)
+    assert (y is not x) is contiguous and ptr == y.data_ptr() and ld == y.stride(0) and copy is copied
 
 
-@pytest.mark.parametrize("shape,stride,copied,transposed", [
-    ((3, 32, 64), (2048, 64, 1), False, False),        # [E, N, K]
-    ((3, 64, 32), (2048, 1, 64), False, True),         # [E, K, N] seen as [E, N, K]
-    ((3, 32, 61), (32 * 61, 61, 1), True, False),      # odd rows
-    ((3, 61, 32), (61 * 32, 32, 1), False, False),     # odd N only
-    ((3, 61, 32), (61 * 32, 1, 61), True, True),       # odd rows of the transposed storage
-    ((3, 32, 64), (0, 64, 1), True, False),            # one matrix for all experts
-    ((1, 32, 64), (5, 64, 1), False, False),           # a single expert's stride is free
-    ((3, 32, 64), (2052, 64, 1), True, False),         # experts off 16 bytes
-    ((3, 32, 64), (4096, 128, 2), True, False)])       # contiguous along neither
-def test_weight_operands(shape, stride, copied, transposed):
+@pytest.mark.parametrize("shape,stride,contiguous,copied,transposed", [
+    ((3, 32, 64), (2048, 64, 1), False, False, False),        # [E, N, K]
+    ((3, 64, 32), (2048, 1, 64), False, False, True),         # [E, K, N] seen as [E, N, K]
+    ((3, 32, 61), (32 * 61, 61, 1), False, True, False),      # odd rows
+    ((3, 61, 32), (61 * 32, 32, 1), False, False, False),     # odd N only
+    ((3, 61, 32), (61 * 32, 1, 61), False, True, True),       # odd rows of the transposed storage
+    ((3, 32, 64), (0, 64, 1), False, True, False),            # one matrix for all experts
+    ((1, 32, 64), (5, 64, 1), False, False, False),           # a single expert's stride is free
+    ((3, 32, 64), (2052, 64, 1), False, True, False),         # experts off 16 bytes
+    ((3, 32, 64), (4096, 128, 2), True, False, False)])       # contiguous along neither
+def test_weight_operands(shape, stride, contiguous, copied, transposed):
     w = torch.zeros(1 << 15, dtype=torch.bfloat16).as_strided(shape, stride)
-    v, ld, plane, tr = g._weights(w)
-    assert (v.data_ptr() != w.data_ptr()) is copied and tr is transposed
-    E, N, K = shape
-    rows, cols = (K, N) if tr else (N, K)
-    assert ld % 8 == 0 and plane % 8 == 0 and ld >= cols and plane >= (rows - 1) * ld + cols
+    v, ptr, ld, plane, tr, copy = g._weights(w)
+    assert (v is not w) is contiguous and ptr == v.data_ptr() and plane == v.stride(0)
+    assert tr is transposed and copy is copied and ld == (v.stride(2) if tr else v.stride(1))
 
 
 def test_overlap():
@@ -93,20 +91,31 @@ def test_argument_checks_before_any_device_work():
     for bad in (dict(T=-1), dict(T=(1 << 30) + 1), dict(E=0), dict(E=1025), dict(N=0), dict(K=0), dict(K=(1 << 24) + 1)):
         assert mm(**bad) == SHAPE, bad
         assert wgrad(**bad) == SHAPE, bad
-    for bad in (dict(x=None), dict(x=A + 2), dict(ldx=63), dict(ldx=56), dict(ldx=68), dict(w=None), dict(w=A + 8),
-                dict(ldw=60), dict(ldw=56), dict(sw=64 * 127), dict(sw=64 * 128 + 4), dict(off=None), dict(off=A + 2),
-                dict(y=None), dict(y=A + 1), dict(ldy=127), dict(type=0), dict(type=3), dict(tr=1, ldw=120)):
+    for bad in (dict(x=None), dict(x=A + 1), dict(ldx=-64), dict(w=None), dict(w=A + 1), dict(ldw=-64), dict(sw=-8),
+                dict(off=None), dict(off=A + 2), dict(y=None), dict(y=A + 1), dict(ldy=127), dict(type=0), dict(type=3)):
         assert mm(**bad) == ARG, bad
-    for bad in (dict(dy=None), dict(dy=A + 8), dict(lddy=120), dict(lddy=132), dict(x=None), dict(ldx=60), dict(off=None),
-                dict(dw=None), dict(dw=A + 2), dict(out=2, dw=A + 1), dict(out=1), dict(out=3), dict(type=0)):
+    for bad in (dict(dy=None), dict(dy=A + 1), dict(lddy=-8), dict(x=None), dict(ldx=-8), dict(off=None), dict(dw=None),
+                dict(dw=A + 2), dict(out=2, dw=A + 1), dict(out=1), dict(out=3), dict(type=0)):
         assert wgrad(**bad) == ARG, bad
-    pad = lambda src=A + 2, plane=999, ld=37, planes=2, rows=27, cols=37, dst=A, ldd=40: _lib.lib().spanqr_mm_pad_rows(  # noqa: E731
-        src, plane, ld, planes, rows, cols, dst, ldd, None)
-    for bad in (dict(planes=-1), dict(planes=1025), dict(rows=-1), dict(cols=0)):
-        assert pad(**bad) == SHAPE, bad
-    for bad in (dict(src=None), dict(src=A + 1), dict(plane=-1), dict(ld=-1), dict(dst=None), dict(dst=A + 8), dict(ldd=36),
-                dict(ldd=32)):
-        assert pad(**bad) == ARG, bad
-    assert pad(rows=0) == OK
     assert mm(T=0) == OK                 # nothing to do
     assert _lib.lib().spanqr_mm_read_status(None, None) == ARG
+
+
+def test_workspace_bytes():
+    L, n = _lib.lib(), ctypes.c_size_t(0)
+
+    def size(fn, *a):
+        assert getattr(L, fn)(*a, ctypes.byref(n)) == OK, a
+        return n.value
+    mm_, wg = "spanqr_mm_grouped_workspace_bytes", "spanqr_mm_grouped_wgrad_workspace_bytes"
+    assert size(mm_, 4096, 8, 1024, 1024, 0) == 0 and size(mm_, 0, 8, 1024, 1024, 7) == 0
+    assert size(mm_, 64, 1, 768, 17408, 0) > 0                      # few tiles: partial sums
+    assert size(wg, 32768, 1, 768, 512, 0) > 0 and size(wg, 4096, 32, 768, 512, 0) == 0
+    one, two, tr = (size(mm_, 4096, 8, 1001, 1111, c) for c in (1, 2, 6))
+    assert one >= 4096 * 1112 * 2 and two >= 8 * 1001 * 1112 * 2 and tr >= 8 * 1111 * 1008 * 2
+    assert size(mm_, 4096, 8, 1001, 1111, 3) == one + two
+    assert size(wg, 4096, 32, 1001, 1111, 3) >= 4096 * (1008 + 1112) * 2
+    for fn, bad in ((mm_, 8), (mm_, -1), (wg, 4)):
+        assert getattr(L, fn)(16, 2, 64, 64, bad, ctypes.byref(n)) == ARG
+    assert L.spanqr_mm_grouped_workspace_bytes(16, 0, 64, 64, 0, ctypes.byref(n)) == SHAPE
+    assert L.spanqr_mm_grouped_workspace_bytes(16, 1, 64, 64, 0, None) == ARG
