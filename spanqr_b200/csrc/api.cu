@@ -934,7 +934,7 @@ int spanqr_grad_norm(const void* const* in, const int* in_type, const long long*
         e = timed(K_GRAD_SUMSQ, st, [&] { return launch_grad_sumsq(es.data(), (int)es.size(), part, &nparts, st); },
                   grad_launches((int)es.size()));
     if (e == cudaSuccess)
-        e = timed(K_GRAD_SUMSQ, st, [&] { return launch_grad_finish(part, nparts, sumsq, norm, st); });
+        e = timed(K_GRAD_SUMSQ, st, [&] { return launch_grad_finish(part, nparts, sumsq, norm, !es.empty(), st); });
     return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
 } catch (const std::bad_alloc&) {
     return SPANQR_ERR_ARG;
@@ -962,10 +962,10 @@ int spanqr_grad_clip(const void* const* in, const int* in_type, void* const* out
     const double* sums = sumsq ? sumsq : part;
     if (sumsq) nparts = 1;
     if (e == cudaSuccess && es.empty()) {
-        if (norm) e = timed(K_GRAD_SUMSQ, st, [&] { return launch_grad_finish(sums, nparts, nullptr, norm, st); });
+        if (norm) e = timed(K_GRAD_SUMSQ, st, [&] { return launch_grad_finish(sums, nparts, nullptr, norm, false, st); });
     } else if (e == cudaSuccess) {
         e = timed(K_GRAD_SCALE, st,
-                  [&] { return launch_grad_scale(es.data(), (int)es.size(), sums, nparts, max_norm, norm, st); }, launches);
+                  [&] { return launch_grad_scale(es.data(), (int)es.size(), sums, nparts, max_norm, norm, !sumsq, st); }, launches);
     }
     return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
 } catch (const std::bad_alloc&) {

@@ -27,6 +27,24 @@ constexpr int THREADS = 256;
 constexpr int UNROLL = 4;                              // 32-byte vectors in flight per thread
 constexpr int CHUNK = THREADS * UNROLL * 32;           // bytes of input per chunk (32 KB)
 
+// programmatic launch: the kernel that adds the slots starts while the last chunks are read, and waits for their end
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... P, typename... A>
+cudaError_t launch_behind(void (*kernel)(P...), int grid, cudaStream_t st, const A&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <int CAP>
 struct Table {
     GradEntry e[CAP];
@@ -173,6 +191,7 @@ template <int CAP>
 __global__ void __launch_bounds__(THREADS, GRAD_CTAS_PER_SM) k_grad_sumsq(const __grid_constant__ Table<CAP> t, double* __restrict__ part) {
     double acc = 0.0;
     const unsigned all = t.first[t.count];
+    launch_dependents();
     for (unsigned c = blockIdx.x; c < all; c += gridDim.x) {
         const int i = tensor_of(t, c);
         const GradEntry& e = t.e[i];
@@ -197,6 +216,7 @@ __global__ void __launch_bounds__(THREADS, GRAD_CTAS_PER_SM) k_grad_sumsq(const 
 __device__ double total(const double* __restrict__ part, int nparts) {
     __shared__ double red[THREADS / 32];
     double acc = 0.0;
+    wait_primary();   // the slots are written
     for (int i = threadIdx.x; i < nparts; i += THREADS) acc += part[i];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(~0u, acc, o);
@@ -332,9 +352,10 @@ cudaError_t sumsq_launch(const GradEntry* e, int count, int nsm, double* part, i
 
 template <int CAP>
 cudaError_t scale_launch(const GradEntry* e, int count, int nsm, const double* part, int nparts, double max_norm,
-                         float* norm, cudaStream_t st) {
+                         float* norm, bool behind, cudaStream_t st) {
     Table<CAP> t;
     const int grid = grid_for(fill(t, e, count), nsm);
+    if (behind) return launch_behind(k_grad_scale<CAP>, grid, st, t, part, nparts, max_norm, norm);
     k_grad_scale<CAP><<<grid, THREADS, 0, st>>>(t, part, nparts, max_norm, norm);
     return cudaGetLastError();
 }
@@ -353,20 +374,23 @@ cudaError_t launch_grad_sumsq(const GradEntry* e, int count, double* part, int* 
     return err;
 }
 
-cudaError_t launch_grad_finish(const double* part, int nparts, double* sumsq, float* norm, cudaStream_t st) {
+cudaError_t launch_grad_finish(const double* part, int nparts, double* sumsq, float* norm, bool behind, cudaStream_t st) {
+    if (behind) return launch_behind(k_grad_finish, 1, st, part, nparts, sumsq, norm);
     k_grad_finish<<<1, THREADS, 0, st>>>(part, nparts, sumsq, norm);
     return cudaGetLastError();
 }
 
 cudaError_t launch_grad_scale(const GradEntry* e, int count, const double* part, int nparts, double max_norm, float* norm,
-                              cudaStream_t st) {
+                              bool behind, cudaStream_t st) {
     int nsm = 0;
     cudaError_t err = sm_count(&nsm);
     if (err == cudaSuccess && count <= CAP_SMALL)
-        return scale_launch<CAP_SMALL>(e, count, nsm, part, nparts, max_norm, norm, st);
+        return scale_launch<CAP_SMALL>(e, count, nsm, part, nparts, max_norm, norm, behind, st);
+    if (err == cudaSuccess && count <= CAP_LARGE)
+        return scale_launch<CAP_LARGE>(e, count, nsm, part, nparts, max_norm, norm, behind, st);
     for (int i = (count - 1) / CAP_LARGE * CAP_LARGE; err == cudaSuccess && i >= 0; i -= CAP_LARGE)   // the last part first
         err = scale_launch<CAP_LARGE>(e + i, count - i < CAP_LARGE ? count - i : CAP_LARGE, nsm, part, nparts, max_norm,
-                                      i == 0 ? norm : nullptr, st);
+                                      i == 0 ? norm : nullptr, false, st);
     return err;
 }
 

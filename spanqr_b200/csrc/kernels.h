@@ -159,11 +159,12 @@ constexpr int GRAD_CTAS_PER_SM = 4;
 int grad_launches(int count);   // launches for a list of `count` tensors
 // CTA sums of squares into part[0 .. *nparts), at most grad_launches(count) * GRAD_CTAS_PER_SM per SM
 cudaError_t launch_grad_sumsq(const GradEntry* e, int count, double* part, int* nparts, cudaStream_t st);
-// *sumsq = the slots' sum, *norm = its square root (either may be null)
-cudaError_t launch_grad_finish(const double* part, int nparts, double* sumsq, float* norm, cudaStream_t st);
+// *sumsq = the slots' sum, *norm = its square root (either may be null); behind: launch_grad_sumsq was the stream's last
+// launch, and this one may start before its end
+cudaError_t launch_grad_finish(const double* part, int nparts, double* sumsq, float* norm, bool behind, cudaStream_t st);
 // out = in * min(1, max_norm / (n + 1e-6)) with n the root of the slots' sum, also to *norm when not null
 cudaError_t launch_grad_scale(const GradEntry* e, int count, const double* part, int nparts, double max_norm, float* norm,
-                              cudaStream_t st);
+                              bool behind, cudaStream_t st);
 
 // ---- products grouped by expert ----
 // An operand: `rows` rows of `cols` contiguous elements, `ld` elements apart, in `planes` planes `plane` elements apart (0
