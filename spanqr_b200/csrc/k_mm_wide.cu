@@ -159,8 +159,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const int q = warp & 3, half = warp >> 2;
         const uint32_t stage = tc::smem_u32(p.sm) + C::STAGING + warp * Y_STAGE;
         if (a.zero_tail) {   // rows behind the last expert
-            for (long long r = p.start[a.E] + (long long)blockIdx.x; r < a.T; r += gridDim.x)
-                for (int n = threadIdx.x; n < a.N; n += 256) a.y[r * a.ldy + n] = 0;
+            const int whole = v16 ? a.N / 8 * 8 : 0;
+            for (long long r = p.start[a.E] + (long long)blockIdx.x; r < a.T; r += gridDim.x) {
+                uint16_t* const y = a.y + r * a.ldy;
+                for (int n = threadIdx.x * 8; n < whole; n += 256 * 8) *reinterpret_cast<uint4*>(y + n) = make_uint4(0, 0, 0, 0);
+                for (int n = whole + threadIdx.x; n < a.N; n += 256) y[n] = 0;
+            }
         }
         for (int j = 0; parts.next(t); ++j) {
             const Tile d = tile_at<NT>(p.start, p.pre, a.E, ntn, t.tile);

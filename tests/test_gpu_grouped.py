@@ -96,6 +96,25 @@ def test_many_small_ragged_experts(T, E, N, K):
     assert torch.equal(mm_grouped(x, w, off), exact_mm(x, w, off).to(BF16))
 
 
+@pytest.mark.parametrize("T,E,N,K", [(64, 1, 768, 17408), (1, 1, 300, 9000), (33, 2, 100, 8192), (200, 3, 260, 5001),
+                                     (5, 1, 4096, 4096)])
+def test_few_tiles_split_over_the_contracted_dimension(T, E, N, K):
+    x, w = ints((T, K), T, BF16), ints((E, N, K), K, BF16)
+    off = offsets(spread(T, E))
+    want = exact_mm(x, w, off).to(BF16)
+    for _ in range(2):
+        assert torch.equal(mm_grouped(x, w, off), want)
+
+
+@pytest.mark.parametrize("T,E,N,K", [(20000, 1, 300, 77), (30000, 2, 256, 512), (9000, 3, 41, 260), (16385, 1, 768, 500)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_few_tiles_split_over_the_rows(T, E, N, K, dtype):
+    dy, x = ints((T, N), T, BF16), ints((T, K), K, BF16)
+    for counts in (spread(T, E), [T] + [0] * (E - 1)):
+        off = offsets(counts)
+        assert torch.equal(mm_grouped_wgrad(dy, x, off, dtype=dtype), exact_wgrad(dy, x, off).to(dtype))
+
+
 @pytest.mark.parametrize("T,E,N,K", [(24, 8, 512, 2048), (700, 16, 384, 1024), (3000, 4, 640, 4096), (5000, 3, 256, 17408)])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 def test_product_gaussian(T, E, N, K, dtype):
@@ -129,6 +148,15 @@ def test_uneven_experts(counts, scale):
     off = offsets(counts)
     assert torch.equal(mm_grouped(x, w, off), exact_mm(x, w, off).to(BF16))
     assert torch.equal(mm_grouped_wgrad(dy, x, off), exact_wgrad(dy, x, off).to(F32))
+
+
+@pytest.mark.parametrize("N", [136, 8, 2051])
+def test_padded_batch(N):
+    """a batch padded far behind its last row"""
+    x, w = ints((5000, 64), 1, BF16), ints((2, N, 64), 2, BF16)
+    off = torch.tensor([7, 100], dtype=torch.int32, device="cuda")
+    y = mm_grouped(x, w, off)
+    assert torch.equal(y, exact_mm(x, w, off).to(BF16))
 
 
 @pytest.mark.parametrize("T,end", [(50, 33), (50, 0), (700, 450), (700, 0)])
@@ -375,3 +403,48 @@ def test_optimizer_step_of_an_expert_layer():
         q, d = q.double(), d.double()
         assert float((q.t() @ q - torch.eye(K, device="cuda")).abs().max()) <= 3e-7
         assert float((d - q @ (q.t() @ d)).norm() / d.norm()) <= 1e-5
+
+
+def test_two_streams_at_once():
+    """calls in flight together on two streams, with workspaces (split products, copied operands): each its own"""
+    ws = [ints((1, 768, 8193), i, BF16) for i in range(2)]
+    xs = [ints((40, 8193), 5 + i, BF16) for i in range(2)]
+    big = [(ints((9000, 200), 7 + i, BF16), ints((9000, 131), 9 + i, BF16)) for i in range(2)]
+    off, boff = offsets([40]), offsets([9000])
+    want = [exact_mm(x, w, off).to(BF16) for x, w in zip(xs, ws)]
+    bwant = [exact_wgrad(d, x, boff).to(F32) for d, x in big]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((mm_grouped(xs[i], ws[i], off), mm_grouped_wgrad(*big[i], boff)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) and torch.equal(d, bwant[i]) for y, d in got[i])
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    """nothing a first call sets up is refused by a capture"""
+    import subprocess
+    import sys
+    code = """
+import torch
+from spanqr_b200 import clip_grads, grad_norm, mm_grouped, mm_grouped_wgrad
+x = torch.ones(40, 64, dtype=torch.bfloat16, device="cuda")
+w = torch.ones(2, 72, 64, dtype=torch.bfloat16, device="cuda")
+off = torch.tensor([15, 40], dtype=torch.int32, device="cuda")
+g = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(g):
+    y = mm_grouped(x, w, off)
+    dw = mm_grouped_wgrad(y, x, off)
+    (c,), n = clip_grads([dw], 1.0)
+    m = grad_norm([dw])
+g.replay()
+torch.cuda.synchronize()
+assert bool((y == 64).all()) and bool((dw[0] == 15 * 64).all()) and bool((dw[1] == 25 * 64).all())
+assert n.item() == m.item() > 1 and abs(c.norm().item() - 1) < 1e-5
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
