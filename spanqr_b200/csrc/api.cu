@@ -1016,12 +1016,12 @@ struct Rows {
 size_t copy_bytes(long long planes, long long rows, long long cols) {
     return al256((size_t)planes * rows * ((cols + 7) / 8 * 8) * 2);
 }
-// the operand for the kernel; what has to be copied becomes a job and takes its place in the workspace at `at`
-MmOperand readable(const Rows& r, bool three, char*& at, PadJob* jobs, int& count) {
+// the operand for the kernel (ends: of the experts, for one with a plane for each); what has to be copied becomes a job and takes its place in the workspace at `at`
+MmOperand readable(const Rows& r, const int* ends, char*& at, PadJob* jobs, int& count) {
     const long long cols8 = (r.cols + 7) / 8 * 8;
-    MmOperand o{r.p, r.cols, r.rows, r.rows > 1 ? r.ld : cols8, three ? r.planes : 0, r.plane, r.mn};
+    MmOperand o{r.p, r.cols, r.rows, r.rows > 1 ? r.ld : cols8, ends ? r.planes : 0, r.plane, r.mn};
     if (!r.readable()) {
-        jobs[count++] = PadJob{r.p, r.plane, r.ld, r.planes, (int)r.rows, (int)r.cols, at};
+        jobs[count++] = PadJob{r.p, r.plane, r.ld, r.planes, (int)r.rows, (int)r.cols, at, ends};
         o.p = at;
         o.ld = cols8;
         o.plane = r.rows * cols8;
@@ -1068,9 +1068,9 @@ int spanqr_mm_grouped(const void* x, long long ldx, const void* w, long long ldw
     char* at = static_cast<char*>(ws) + al256(plan.ws);
     PadJob jobs[2];
     int njobs = 0;
-    const MmOperand ox = readable(rx, false, at, jobs, njobs), ow = readable(rw, true, at, jobs, njobs);
+    const MmOperand ox = readable(rx, nullptr, at, jobs, njobs), ow = readable(rw, offsets, at, jobs, njobs);
     const MmArgs a{offsets, E, T, N, K, static_cast<uint16_t*>(y), T > 1 ? ldy : N, (N + 255) / 256,
-                   plan.ws ? static_cast<float*>(ws) : nullptr, type == SPANQR_BF16, zero_tail != 0, mm_status()};
+                   plan.ws ? static_cast<float*>(ws) : nullptr, type == SPANQR_BF16, zero_tail != 0, mm_status(), njobs > 0};
     if (!a.status) return cuda_fail(cudaGetLastError());
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (njobs) e = timed(K_PAD, st, [&] { return launch_pad_rows(jobs, njobs, st); });
@@ -1111,8 +1111,8 @@ int spanqr_mm_grouped_wgrad(const void* dy, long long lddy, const void* x, long 
     char* at = static_cast<char*>(ws) + al256(plan.ws);
     PadJob jobs[2];
     int njobs = 0;
-    const MmOperand ody = readable(rdy, false, at, jobs, njobs), ox = readable(rx, false, at, jobs, njobs);
-    const MmWgradArgs a{offsets, E, T, N, K, dw, type == SPANQR_BF16, out_type == SPANQR_F32, 1, mm_status()};
+    const MmOperand ody = readable(rdy, nullptr, at, jobs, njobs), ox = readable(rx, nullptr, at, jobs, njobs);
+    const MmWgradArgs a{offsets, E, T, N, K, dw, type == SPANQR_BF16, out_type == SPANQR_F32, 1, mm_status(), njobs > 0};
     if (!a.status) return cuda_fail(cudaGetLastError());
     if (njobs) e = timed(K_PAD, st, [&] { return launch_pad_rows(jobs, njobs, st); });
     if (e == cudaSuccess)

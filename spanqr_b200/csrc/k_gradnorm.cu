@@ -50,6 +50,7 @@ struct Table {
     GradEntry e[CAP];
     unsigned first[CAP + 1];   // first chunk of each tensor in this launch; first[count] = all chunks
     int count;
+    bool in_place;             // every output is its input
 };
 
 // the tensor that holds chunk c
@@ -303,12 +304,14 @@ __global__ void __launch_bounds__(THREADS, GRAD_CTAS_PER_SM) k_grad_scale(const 
     // or above fp32's largest value), else p = 1
     const bool sub = c < 0x1p-100;
     const Coef coef{(float)(c >= 1.0 ? 1.0 : sub ? c * 0x1p64 : c), sub ? 0x1p-64f : 1.0f};   // a NaN norm gives NaN
+    const bool unchanged = coef.c == 1.0f && coef.p == 1.0f;
+    if (unchanged && t.in_place) return;
     const unsigned all = t.first[t.count];
     for (unsigned k = blockIdx.x; k < all; k += gridDim.x) {
         const unsigned ch = all - 1 - k;
         const int i = tensor_of(t, ch);
         const GradEntry& e = t.e[i];
-        if (coef.c == 1.0f && coef.p == 1.0f && e.in == e.out) continue;
+        if (unchanged && e.in == e.out) continue;
         const unsigned local = ch - t.first[i];
         if (e.in_type == DT_F32) chunk_scale<DT_F32, DT_F32>(e, local, coef);
         else if (e.in_type == DT_F16 && e.out_type == DT_F16) chunk_scale<DT_F16, DT_F16>(e, local, coef);
@@ -324,7 +327,9 @@ constexpr int CAP_SMALL = 64, CAP_LARGE = 900;
 template <int CAP>
 unsigned fill(Table<CAP>& t, const GradEntry* e, int count) {
     unsigned c = 0;
+    t.in_place = true;
     for (int i = 0; i < count; ++i) {
+        t.in_place = t.in_place && e[i].in == e[i].out;
         t.e[i] = e[i];
         t.first[i] = c;
         const uintptr_t b = reinterpret_cast<uintptr_t>(e[i].in);

@@ -19,16 +19,22 @@ __device__ __forceinline__ void st_shared16(uint32_t at, uint32_t a, uint32_t b,
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// a warp's staged results to rows of dw that do not start on 16 bytes
+// a warp's staged results to rows of dw that do not start on 16 bytes: a lane is a column (two of 16 bits)
 template <typename OUT>
 __device__ __forceinline__ void store_rows(const char* stage, OUT* row, int ld, int rows, int cols) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll 1
-    for (int x = 0; x < rows; ++x, row += ld)
-#pragma unroll 1
-        for (int y = threadIdx.x & 31; y < cols; y += 32) {
-            const int at = y * (int)sizeof(OUT);
-            row[y] = *reinterpret_cast<const OUT*>(stage + x * 128 + (((at >> 4) ^ (x & 7)) << 4) + (at & 15));
+    for (int x = 0; x < rows; x += 8) {
+#pragma unroll
+        for (int z = 0; z < 8; ++z) {
+#pragma unroll
+            for (int y = lane; y < 128 / (int)sizeof(OUT); y += 32) {
+                const int at = y * (int)sizeof(OUT), r = x + z;   // (r & 7 == z)
+                const OUT v = *reinterpret_cast<const OUT*>(stage + r * 128 + (((at >> 4) ^ z) << 4) + (at & 15));
+                if (r < rows && y < cols) row[(long long)r * ld + y] = v;
+            }
         }
+    }
     __syncwarp();
 }
 
@@ -335,17 +341,17 @@ cudaError_t launch_mm_wgrad(const MmOperand& dy, const MmOperand& x, const MmWgr
     if (e != cudaSuccess) return e;
     const int pairs = (int)(pl.tiles < nsm / 2 ? pl.tiles : nsm / 2);
     if (rows16)
-        e = out32 ? launch_pairs<C, k_mm_wgrad<float, true>>(pairs, a.E, st, tdy, tx, tdw, a)
-                  : launch_pairs<C, k_mm_wgrad<uint16_t, true>>(pairs, a.E, st, tdy, tx, tdw, a);
+        e = out32 ? launch_pairs<C, k_mm_wgrad<float, true>>(pairs, a.E, a.behind, st, tdy, tx, tdw, a)
+                  : launch_pairs<C, k_mm_wgrad<uint16_t, true>>(pairs, a.E, a.behind, st, tdy, tx, tdw, a);
     else
-        e = out32 ? launch_pairs<C, k_mm_wgrad<float, false>>(pairs, a.E, st, tdy, tx, tdw, a)
-                  : launch_pairs<C, k_mm_wgrad<uint16_t, false>>(pairs, a.E, st, tdy, tx, tdw, a);
+        e = out32 ? launch_pairs<C, k_mm_wgrad<float, false>>(pairs, a.E, a.behind, st, tdy, tx, tdw, a)
+                  : launch_pairs<C, k_mm_wgrad<uint16_t, false>>(pairs, a.E, a.behind, st, tdy, tx, tdw, a);
     if (e != cudaSuccess || !split) return e;
     a.dw = args.dw;
     const long long quads = (long long)a.E * a.N * (pl.ldp / 4), ctas = (quads + 255) / 256;
     const dim3 grid((unsigned)(ctas < 8LL * nsm ? ctas : 8LL * nsm));
-    return a.out32 ? launch_join<k_mm_wgrad_join<float>>(grid, 256, 0, st, a, (const float*)ws, pl.ldp)
-                   : launch_join<k_mm_wgrad_join<uint16_t>>(grid, 256, 0, st, a, (const float*)ws, pl.ldp);
+    return a.out32 ? launch_behind(k_mm_wgrad_join<float>, grid, 256, 0, st, a, (const float*)ws, pl.ldp)
+                   : launch_behind(k_mm_wgrad_join<uint16_t>, grid, 256, 0, st, a, (const float*)ws, pl.ldp);
 }
 
 }  // namespace spq

@@ -243,10 +243,10 @@ cudaError_t run(const MmOperand& x, const MmOperand& w, const MmArgs& a, const M
     cudaError_t e = encode_mm(&tx, x, a.type(), BK, NT / 2);
     if (e == cudaSuccess) e = w.mn ? encode_mm(&tw, w, a.type(), 64, BK) : encode_mm(&tw, w, a.type(), BK, FT);
     if (e == cudaSuccess)
-        e = w.mn ? launch_pairs<C, k_mm_wide<true, NT>>(pl.pairs, a.E, st, tw, tx, a)
-                 : launch_pairs<C, k_mm_wide<false, NT>>(pl.pairs, a.E, st, tw, tx, a);
+        e = w.mn ? launch_pairs<C, k_mm_wide<true, NT>>(pl.pairs, a.E, a.behind, st, tw, tx, a)
+                 : launch_pairs<C, k_mm_wide<false, NT>>(pl.pairs, a.E, a.behind, st, tw, tx, a);
     if constexpr (CAN_SPLIT<NT>) {
-        if (e == cudaSuccess && pl.split) e = launch_join<k_mm_join<NT>>(dim3(pl.pairs - 1, NT / 2), 256, a.E, st, a, pl.pairs);
+        if (e == cudaSuccess && pl.split) e = launch_behind(k_mm_join<NT>, dim3(pl.pairs - 1, NT / 2), 256, 2 * (a.E + 1) * (int)sizeof(int), st, a, pl.pairs);
     }
     return e;
 }

@@ -187,6 +187,7 @@ struct MmArgs {
     DType type() const { return bf16 ? DT_BF16 : DT_F16; }
     bool zero_tail;       // zero the rows behind the last expert (else they are left as they are)
     int* status;          // a bounded wait that runs out ORs MM_TIMEOUT
+    bool behind;          // launch_pad_rows was the stream's last launch
 };
 constexpr int MM_TIMEOUT = 0x100;
 constexpr int MM_MAX_E = 1024;
@@ -227,6 +228,7 @@ struct MmWgradArgs {
     bool bf16, out32;
     int splits;     // runs of each expert's rows (set by launch_mm_wgrad)
     int* status;
+    bool behind;    // as above
     DType type() const { return bf16 ? DT_BF16 : DT_F16; }
 };
 struct MmWgradPlan {
@@ -246,6 +248,7 @@ struct PadJob {
     long long plane, ld;
     int planes, rows, cols;
     void* dst;
+    const int* ends;   // null, or the experts' ends (device): planes of experts without rows are not copied
 };
 cudaError_t launch_pad_rows(const PadJob* jobs, int count, cudaStream_t st);
 

@@ -98,6 +98,11 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
+// programmatic launch: the next kernel's CTAs may start (they wait for this grid's end before they touch its results);
+// the wait is over at once in a kernel that was launched otherwise
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---- 16-bit results ----
 __device__ __forceinline__ uint16_t to16(float x, bool bf16) {
     return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));
@@ -164,22 +169,31 @@ __device__ __forceinline__ void store_y(uint32_t taddr, uint32_t stage, uint16_t
             stmatrix4t(stage + at + h * 32 + 16 * Y_PITCH, w[h][4], w[h][5], w[h][6], w[h][7]);
         }
         __syncwarp();   // (the buffer's last readers passed the block in between)
+        if (v16) {   // 16 bytes a lane, 64 of each of 8 rows at a time
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + (lane >> 2);
-            uint32_t u[4];
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3])
-                         : "r"(stage + r * Y_PITCH + f * 2)
-                         : "memory");
-            if (c + r >= rows) continue;
-            uint16_t* const o = y + (long long)(c + r) * ldy + f;
-            if (v16 && f + 8 <= features) {
-                *reinterpret_cast<uint4*>(o) = make_uint4(u[0], u[1], u[2], u[3]);
-            } else {
+            for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + (lane >> 2);
+                uint32_t u[4];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3])
+                             : "r"(stage + r * Y_PITCH + f * 2)
+                             : "memory");
+                if (c + r >= rows) continue;
+                uint16_t* const o = y + (long long)(c + r) * ldy + f;
+                if (f + 8 <= features) {
+                    *reinterpret_cast<uint4*>(o) = make_uint4(u[0], u[1], u[2], u[3]);
+                } else {
 #pragma unroll
-                for (int x = 0; x < 8; ++x)
-                    if (f + x < features) o[x] = (uint16_t)(u[x >> 1] >> (16 * (x & 1)));
+                    for (int x = 0; x < 8; ++x)
+                        if (f + x < features) o[x] = (uint16_t)(u[x >> 1] >> (16 * (x & 1)));
+                }
+            }
+        } else {     // rows at any address: a lane is a feature
+            const int last = min(32, rows - c);
+            for (int r = 0; r < last; ++r) {
+                uint16_t u;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(stage + r * Y_PITCH + lane * 2) : "memory");
+                if (lane < features) y[(long long)(c + r) * ldy + lane] = u;
             }
         }
         const uint32_t next = other;

@@ -161,6 +161,7 @@ __device__ __forceinline__ Pair set_up(char* dyn, const int* offsets, int E, int
     p.full0 = mapa(tc::smem_u32(p.full), 0);
     p.tempty0 = mapa(tc::smem_u32(p.tempty), 0);
     p.zeroed0 = mapa(tc::smem_u32(p.zeroed), 0);
+    wait_primary();   // (the offsets, read above, are no copy's result)
     return p;
 }
 
@@ -221,26 +222,13 @@ __host__ __device__ __forceinline__ long long run_begin(long long total, int run
     return i < runs ? total * i / runs : total;
 }
 
-// programmatic launch: the next kernel's CTAs may start (they wait for this grid's end before they read its results)
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-// a pair kernel's launch
-template <typename C, auto kernel, typename... A>
-cudaError_t launch_pairs(int pairs, int E, cudaStream_t st, const A&... args) {
-    static SmemOnce once;   // of this kernel
-    const cudaError_t e = once.allow(reinterpret_cast<const void*>(kernel), C::FIXED + 2 * (MM_MAX_E + 1) * (int)sizeof(int));
-    if (e != cudaSuccess) return e;
-    kernel<<<2 * pairs, THREADS, C::FIXED + 2 * (E + 1) * (int)sizeof(int), st>>>(args...);
-    return cudaGetLastError();
-}
-// the second kernel's launch, right behind the first
-template <auto kernel, typename... A>
-cudaError_t launch_join(dim3 grid, int threads, int E, cudaStream_t st, const A&... args) {
+// a launch that may begin before the stream's last kernel has ended (programmatic launch)
+template <typename... P, typename... A>
+cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st, const A&... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = 2 * (E + 1) * sizeof(int);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -248,6 +236,18 @@ cudaError_t launch_join(dim3 grid, int threads, int E, cudaStream_t st, const A&
     cfg.attrs = at;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// a pair kernel's launch (behind: the copies of its operands precede it)
+template <typename C, auto kernel, typename... A>
+cudaError_t launch_pairs(int pairs, int E, bool behind, cudaStream_t st, const A&... args) {
+    static SmemOnce once;   // of this kernel
+    const cudaError_t e = once.allow(reinterpret_cast<const void*>(kernel), C::FIXED + 2 * (MM_MAX_E + 1) * (int)sizeof(int));
+    if (e != cudaSuccess) return e;
+    const int smem = C::FIXED + 2 * (E + 1) * (int)sizeof(int);
+    if (behind) return launch_behind(kernel, dim3(2 * pairs), THREADS, smem, st, args...);
+    kernel<<<2 * pairs, THREADS, smem, st>>>(args...);
+    return cudaGetLastError();
 }
 
 }  // namespace mm
