@@ -26,6 +26,8 @@
  *   spanqr_gram_mode_f32     the same, and kcholqr.py:106 Y.T @ Y (each Gram of the orth sequence on its own)
  *   spanqr_chol_f32          candidates/kchol.py:35-44 chol32(G, tau) (kernel candidates/cuk/chol.cu:273-276)
  *   spanqr_trsm_f32          candidates/tri.py:406-412 trsm_f(X, L, Li, s, Z, eps)
+ *   spanqr_grad_*, spanqr_mm_grouped*  no reference counterpart: the steps before orth in an optimizer (the rules above on
+ *                            types and alignment do not apply to them; their own stand at their declarations)
  */
 #ifndef SPANQR_H
 #define SPANQR_H
