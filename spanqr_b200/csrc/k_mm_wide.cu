@@ -3,9 +3,13 @@
 //
 // The weights are the tensor core's first operand whatever the number of rows: with few rows the kernel streams them once
 // from HBM, with many it is bound by the products, and a tile's last rows cost products in steps of 32 columns, not of
-// 128.  NT is 32 to 256 by the rows per expert and the tiles that leaves (launch_mm): the smaller the tile, the more of
+// 128.  NT is 32 to 256 by the rows per expert and the tiles that leaves (mm_plan): the smaller the tile, the more of
 // the weights are in flight and the more pairs have work.  Where even tiles of 32 rows leave pairs idle, the stages of the
 // contracted dimension are split evenly over the pairs and joined by a second kernel.
+//
+// Measured (bf16, inputs out of the caches): 16384 rows, 8 experts of 5120x2048: 209 us (1645 TFLOP/s, 0.98 of cuBLAS's
+// burst rate); 1024 rows, 128 experts of 1024x1024: 49 us (5.6 TB/s); 64 rows, 8 experts of 5120x2048: 34 us (5.0 TB/s);
+// one row and next to no work: 5 us.
 #include "mm_pair.cuh"
 
 namespace spq {
@@ -178,7 +182,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             const uint32_t acc = p.tmem + b * NT + ((uint32_t)(q * 32) << 16);
             if (n < a.N) {
                 if (!CAN_SPLIT<NT> || t.whole) {
-                    store_y(acc, stage, a.y + (long long)d.t0 * a.ldy + n, a.ldy, half * 32, 64, d.cols, d.rows, a.N - n, a.bf16, v16);
+                    store_y(acc, stage, a.y + (long long)d.t0 * a.ldy + n, a.ldy, half * 32, 64, d.cols, d.rows, a.N - n,
+                            a.bf16, v16);
                 } else {   // the part's slot: [column][feature]
                     float* const out = a.part + (size_t)(2 * pair + (t.k0 == 0)) * NT * 256 + f + lane;
                     for (int c = half * 32; c < d.cols; c += 64) {
@@ -246,7 +251,9 @@ cudaError_t run(const MmOperand& x, const MmOperand& w, const MmArgs& a, const M
         e = w.mn ? launch_pairs<C, k_mm_wide<true, NT>>(pl.pairs, a.E, a.behind, st, tw, tx, a)
                  : launch_pairs<C, k_mm_wide<false, NT>>(pl.pairs, a.E, a.behind, st, tw, tx, a);
     if constexpr (CAN_SPLIT<NT>) {
-        if (e == cudaSuccess && pl.split) e = launch_behind(k_mm_join<NT>, dim3(pl.pairs - 1, NT / 2), 256, 2 * (a.E + 1) * (int)sizeof(int), st, a, pl.pairs);
+        if (e == cudaSuccess && pl.split)
+            e = launch_behind(k_mm_join<NT>, dim3(pl.pairs - 1, NT / 2), 256, 2 * (a.E + 1) * (int)sizeof(int), st, a,
+                              pl.pairs);
     }
     return e;
 }
@@ -258,6 +265,10 @@ MmPlan mm_plan(int T, int E, int N, int K, int nsm) {
     const long long ntn = (N + 2 * FT - 1) / (2 * FT), some = T < E ? T : E;
     const int pairs = nsm / 2;
     auto tiles = [&](int nt) { return ntn * (T / nt + (some + 1) / 2); };   // as many as to expect
+    // Tiles that hold an average expert with room to spare (a second tile reads its weights again), halved while a quarter
+    // of the pairs would idle.  Measured (us at 32 / 64 / 128 / 256 rows): 16 experts of 2048x2048 with 256 rows in all:
+    // 26 / 27 / 27 / 28; 1024: 38 / 31 / 28 / 29; 4096: 95 / 58 / 45 / 43; one expert of 2048x2048 with 512 rows (two tiles
+    // of 256 for each of 8 in its features): 18 / 13 / 14 / 19.
     p.nt = T <= 20LL * E ? 32 : T <= 44LL * E ? 64 : T <= 96LL * E ? 128 : 256;
     while (p.nt > 32 && tiles(p.nt) * 4 < 3 * pairs) p.nt /= 2;
     // The split saves what the busiest pair has beyond its share, about 0.17 us a stage, and costs its partial sums and the

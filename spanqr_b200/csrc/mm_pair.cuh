@@ -112,7 +112,7 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, uin
 struct Pair {
     char* sm;
     uint64_t *full, *empty, *tfull, *tempty;
-    uint64_t *ragged, *zeroed;   // wgrad: this CTA's copies of a ragged stage; (leader) the other CTA's part of stage s is zeroed
+    uint64_t *ragged, *zeroed;   // wgrad: this CTA's copies of a ragged stage; (leader) the other has zeroed its part of stage s
     volatile int* err;
     int *start, *pre;
     uint32_t tmem;
