@@ -62,18 +62,23 @@ def _at(a):
 _WS_BYTES = {}
 
 
-def _workspace(dev, count):
+def _norm_like(ts, dev):
+    """where the norm goes"""
+    return ts[0].new_empty((), dtype=torch.float32) if ts else torch.empty((), dtype=torch.float32, device=dev)
+
+
+def _workspace(like, count):
     bytes_ = _WS_BYTES.get(count)
     if bytes_ is None:
         n = _lib.ctypes.c_size_t(0)
         _lib.check(_lib.lib().spanqr_grad_workspace_bytes(count, _lib.ctypes.byref(n)), f"grad_workspace_bytes({count})")
         bytes_ = _WS_BYTES[count] = n.value
-    return torch.empty(bytes_, dtype=torch.uint8, device=dev)
+    return like.new_empty(bytes_, dtype=torch.uint8)
 
 
 def _run_norm(ts, types, dev, sumsq, norm):
     """the norm's kernels for contiguous tensors ts; sumsq and norm are tensors or None"""
-    ws = _workspace(dev, len(ts))
+    ws = _workspace(sumsq if norm is None else norm, len(ts))
     ptrs, sizes = array("Q", map(_ptr, ts)), array("q", map(_numel, ts))
     _lib.launch(dev, _lib.lib().spanqr_grad_norm, lambda: f"grad_norm({len(ts)} tensors)", _at(ptrs), _at(types),
                 _at(sizes), len(ts), None if sumsq is None else sumsq.data_ptr(), None if norm is None else norm.data_ptr(),
@@ -81,7 +86,7 @@ def _run_norm(ts, types, dev, sumsq, norm):
 
 
 def _run_clip(ins, in_types, outs, out_types, dev, max_norm, sumsq, norm):
-    ws = _workspace(dev, len(ins))
+    ws = _workspace(norm, len(ins))
     pi, po, sizes = array("Q", map(_ptr, ins)), array("Q", map(_ptr, outs)), array("q", map(_numel, ins))
     try:
         _lib.launch(dev, _lib.lib().spanqr_grad_clip, lambda: f"clip_grads({len(ins)} tensors)", _at(pi), _at(in_types),
@@ -114,7 +119,7 @@ def grad_norm(tensors, *, group=None):
         dev = torch.cuda.current_device()
     if not all(map(_contiguous, ts)):
         ts = [t if _dense(t) else t.contiguous() for t in ts]
-    norm = torch.empty((), dtype=torch.float32, device=dev)
+    norm = _norm_like(ts, dev)
     if group is None:
         _run_norm(ts, types, dev, None, norm)
     else:   # an empty list's clipping gives the sum's square root
@@ -158,7 +163,7 @@ def clip_grads(tensors, max_norm, *, out=None, group=None):
             ins = [_like_output(i, t, o) for i, (t, o) in enumerate(zip(ts, res))]
     if dev is None:
         dev = torch.cuda.current_device()
-    norm = torch.empty((), dtype=torch.float32, device=dev)
+    norm = _norm_like(ts, dev)
     sumsq = None if group is None else _group_sumsq(ins, types, dev, group)
     _run_clip(ins, types, res, out_types, dev, max_norm, sumsq, norm)
     if out is not None and res:

@@ -85,14 +85,16 @@ def _check_rows(x, name):
         raise ValueError(f"{name} must be a 2-D tensor")
     if x.dtype not in (torch.bfloat16, torch.float16) or not x.is_cuda:
         raise TypeError(f"{name} must be a bf16 or fp16 CUDA tensor (got {x.dtype} on {x.device})")
-    if x.shape[1] < 1:
+    rows, cols = x.shape
+    if cols < 1:
         raise ValueError(f"{name} has no columns")
+    return rows, cols
 
 
 def _check_offsets(offsets, x, E=None):
     if not torch.is_tensor(offsets) or offsets.dim() != 1:
         raise ValueError("offsets must be a 1-D tensor: the end of each expert's rows")
-    if offsets.dtype != torch.int32 or offsets.device != x.device:
+    if offsets.dtype != torch.int32 or offsets.get_device() != x.get_device():
         raise TypeError(f"offsets must be int32 on {x.device} (got {offsets.dtype} on {offsets.device})")
     n = offsets.shape[0]
     if E is not None and n != E:
@@ -102,14 +104,13 @@ def _check_offsets(offsets, x, E=None):
     return offsets if offsets.stride(0) == 1 or n == 1 else offsets.contiguous()
 
 
-def _mm(x, w, offsets, out=None):
-    T, K = x.shape
-    E, N, _ = w.shape
+def _product(rows, weights, offsets, T, E, N, K, out=None):
+    """y [T, N] of operands as _rows and _weights give them, the weights [E, N, K]"""
+    x, px, ldx, copy_x = rows
+    w, pw, ldw, plane, transposed, copy_w = weights
     y = x.new_empty((T, N)) if out is None else out
     if T == 0:
         return y
-    x, px, ldx, copy_x = _rows(x)
-    w, pw, ldw, plane, transposed, copy_w = _weights(w)
     ws, pws, n = _workspace("spanqr_mm_grouped_workspace_bytes", x, T, E, N, K, copy_x + 2 * copy_w + 4 * transposed)
     _lib.launch(x.get_device(), _lib.lib().spanqr_mm_grouped, lambda: f"mm_grouped({T}x{K}, {E} experts of {N}x{K})", px, ldx,
                 pw, ldw, plane, transposed, offsets.data_ptr(), y.data_ptr(), y.stride(0), DTYPES[x.dtype], T, E, N, K,
@@ -117,12 +118,11 @@ def _mm(x, w, offsets, out=None):
     return y
 
 
-def _wgrad(dy, x, offsets, dtype, out=None):
-    T, N = dy.shape
-    K, E = x.shape[1], offsets.shape[0]
+def _wgrad(rows_dy, rows_x, offsets, T, E, N, K, dtype, out=None):
+    """dw [E, N, K] of operands as _rows gives them"""
+    dy, pdy, lddy, copy_dy = rows_dy
+    x, px, ldx, copy_x = rows_x
     dw = x.new_empty((E, N, K), dtype=dtype) if out is None else out
-    dy, pdy, lddy, copy_dy = _rows(dy)
-    x, px, ldx, copy_x = _rows(x)
     ws, pws, n = _workspace("spanqr_mm_grouped_wgrad_workspace_bytes", x, T, E, N, K, copy_dy + 2 * copy_x)
     _lib.launch(x.get_device(), _lib.lib().spanqr_mm_grouped_wgrad,
                 lambda: f"mm_grouped_wgrad({T} rows, {E} experts of {N}x{K})", pdy, lddy, px, ldx, offsets.data_ptr(),
@@ -130,19 +130,34 @@ def _wgrad(dy, x, offsets, dtype, out=None):
     return dw
 
 
+def _backward(ctx, dy):
+    x, w, offsets = ctx.saved_tensors
+    T, N = dy.shape
+    E, _, K = w.shape
+    rows_dy, dx, dw = _rows(dy), None, None
+    if ctx.needs_input_grad[0]:
+        v, ptr, ld, plane, transposed, copy = _weights(w)
+        dx = _product(rows_dy, (v, ptr, ld, plane, not transposed, copy), offsets, T, E, K, N)
+    if ctx.needs_input_grad[1]:
+        dw = _wgrad(rows_dy, _rows(x), offsets, T, E, N, K, w.dtype)
+    return dx, dw, None
+
+
+_backward_once = once_differentiable(_backward)
+
+
 class _MmGrouped(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets):
         ctx.save_for_backward(x, w, offsets)
-        return _mm(x, w, offsets)
+        T, K = x.shape
+        E, N, _ = w.shape
+        return _product(_rows(x), _weights(w), offsets, T, E, N, K)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, w, offsets = ctx.saved_tensors
-        dx = _mm(dy, w.transpose(1, 2), offsets) if ctx.needs_input_grad[0] else None
-        dw = _wgrad(dy, x, offsets, w.dtype) if ctx.needs_input_grad[1] else None
-        return dx, dw, None
+        # (under create_graph the gradients say that they cannot be differentiated again)
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
 
 
 def mm_grouped(x, w, offsets, *, out=None):
@@ -153,32 +168,33 @@ def mm_grouped(x, w, offsets, *, out=None):
     are summed in fp32 and rounded once.
 
     Operands whose rows do not start on 16 bytes (K not a multiple of 8, odd strides or addresses), or that are contiguous
-    along neither dimension, are copied first, at each call.  Ends that decrease or lie outside [0, T] are clamped to the nearest that
-    do not, on the device.
+    along neither dimension, are copied first, at each call.  Ends that decrease or lie outside [0, T] are clamped to
+    the nearest that do not, on the device.
 
     Differentiable once in x and w (without `out`): dx is this product with the transposed weights, dw is
     mm_grouped_wgrad in w's type; rows behind the last expert get a zero gradient and give none."""
-    _check_rows(x, "x")
-    if not torch.is_tensor(w) or w.dim() != 3 or w.shape[2] != x.shape[1]:
-        raise ValueError(f"w must be a 3-D tensor [E, N, {x.shape[1]}]")
-    if w.dtype != x.dtype or w.device != x.device:
+    T, K = _check_rows(x, "x")
+    if not torch.is_tensor(w) or w.dim() != 3 or w.shape[2] != K:
+        raise ValueError(f"w must be a 3-D tensor [E, N, {K}]")
+    if w.dtype != x.dtype or w.get_device() != x.get_device():
         raise TypeError(f"w must be {x.dtype} on {x.device}, as x (got {w.dtype} on {w.device})")
-    if w.shape[1] < 1:
+    E, N, _ = w.shape
+    if N < 1:
         raise ValueError("w has no rows")
-    offsets = _check_offsets(offsets, x, w.shape[0])
+    offsets = _check_offsets(offsets, x, E)
     grad = torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
     if out is None:
-        return _MmGrouped.apply(x, w, offsets) if grad else _mm(x, w, offsets)
+        return _MmGrouped.apply(x, w, offsets) if grad else _product(_rows(x), _weights(w), offsets, T, E, N, K)
     if grad:
         raise RuntimeError("mm_grouped with out= is not differentiable: leave out away, or use torch.no_grad()")
-    if not torch.is_tensor(out) or out.shape != (x.shape[0], w.shape[1]):
-        raise ValueError(f"out must have shape {(x.shape[0], w.shape[1])}")
+    if not torch.is_tensor(out) or out.shape != (T, N):
+        raise ValueError(f"out must have shape {(T, N)}")
     if out.dtype != x.dtype or out.device != x.device:
         raise TypeError(f"out must be {x.dtype} on {x.device} (got {out.dtype} on {out.device})")
-    if out.shape[1] > 1 and out.stride(1) != 1 or out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+    if N > 1 and out.stride(1) != 1 or T > 1 and out.stride(0) < N:
         raise ValueError("out must have contiguous rows that do not overlap")
     _no_overlap(out, x=x, w=w, offsets=offsets)
-    _mm(x, w, offsets, out)
+    _product(_rows(x), _weights(w), offsets, T, E, N, K, out)
     if not out.is_inference():
         torch.autograd.graph.increment_version(out)
     return out
@@ -188,29 +204,30 @@ def mm_grouped_wgrad(dy, x, offsets, *, out=None, dtype=None):
     """dw [E, N, K] with dw[e] = sum over expert e's rows t of dy[t] x[t]^T: the weight gradient of mm_grouped.  dy [T, N]
     and x [T, K] of one type (bf16 or fp16), offsets int32 [E] as there; an expert without rows gets zeros, and rows from
     offsets[-1] on count nowhere.  dtype is fp32 (the default: what clip_grads and orth_batched take) or the inputs' type;
-    `out`, a contiguous [E, N, K] tensor of either type that overlaps neither input, is overwritten.  Summed in fp32 (sums
-    of 256 rows by the tensor cores, those rounded to nearest) and rounded once.  Not differentiable."""
-    _check_rows(dy, "dy")
-    _check_rows(x, "x")
-    if dy.shape[0] != x.shape[0]:
-        raise ValueError(f"dy and x must have as many rows (got {dy.shape[0]} and {x.shape[0]})")
-    if dy.dtype != x.dtype or dy.device != x.device:
+    `out`, a contiguous [E, N, K] tensor of either type that overlaps neither input, is overwritten.  Summed in fp32 (over
+    512 rows, or 2048 for 16-bit results, by the tensor cores, those sums to nearest) and rounded once.  Not
+    differentiable."""
+    T, N = _check_rows(dy, "dy")
+    rows, K = _check_rows(x, "x")
+    if rows != T:
+        raise ValueError(f"dy and x must have as many rows (got {T} and {rows})")
+    if dy.dtype != x.dtype or dy.get_device() != x.get_device():
         raise TypeError(f"dy must be {x.dtype} on {x.device}, as x (got {dy.dtype} on {dy.device})")
     offsets = _check_offsets(offsets, x)
-    shape = (offsets.shape[0], dy.shape[1], x.shape[1])
+    E = offsets.shape[0]
     if out is None:
         dtype = torch.float32 if dtype is None else dtype
         if dtype not in (torch.float32, x.dtype):
             raise TypeError(f"dtype must be fp32 or {x.dtype} (got {dtype})")
-        return _wgrad(dy.detach(), x.detach(), offsets, dtype)
+        return _wgrad(_rows(dy), _rows(x), offsets, T, E, N, K, dtype)
     if dtype is not None:
         raise ValueError("give dtype or out, not both")
-    if not torch.is_tensor(out) or out.shape != shape or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous with shape {shape}")
+    if not torch.is_tensor(out) or out.shape != (E, N, K) or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous with shape {(E, N, K)}")
     if out.dtype not in (torch.float32, x.dtype) or out.device != x.device:
         raise TypeError(f"out must be fp32 or {x.dtype} on {x.device} (got {out.dtype} on {out.device})")
     _no_overlap(out, dy=dy, x=x, offsets=offsets)
-    _wgrad(dy.detach(), x.detach(), offsets, None, out)
+    _wgrad(_rows(dy), _rows(x), offsets, T, E, N, K, None, out)
     if not out.is_inference():
         torch.autograd.graph.increment_version(out)
     return out

@@ -132,6 +132,15 @@ def test_norm_of_many_equal_values_does_not_drift():
     check_norm(grad_norm([x]), want)
 
 
+def test_a_tensor_past_two_to_the_31_elements():
+    n = (1 << 31) + 12345
+    x = torch.zeros(n, dtype=BF16, device="cuda")
+    x[7], x[n - 1], x[1 << 31] = 3.0, 4.0, 12.0
+    assert grad_norm([x]).item() == 13.0
+    clip_grads([x], 6.5, out=[x])                        # 6.5 / (13 + 1e-6): half, to fp32's last bits
+    assert x[7].item() == 1.5 and x[n - 1].item() == 2.0 and x[1 << 31].item() == 6.0 and int((x != 0).sum()) == 3
+
+
 def test_zero_empty_and_unclipped():
     z = [torch.zeros(1000, device="cuda"), torch.zeros(0, device="cuda")]
     assert grad_norm(z).item() == 0.0 and grad_norm([]).item() == 0.0

@@ -405,6 +405,32 @@ def test_optimizer_step_of_an_expert_layer():
         assert float((d - q @ (q.t() @ d)).norm() / d.norm()) <= 1e-5
 
 
+def test_results_past_two_to_the_31_elements():
+    T, N, K = 1_100_003, 2048, 64
+    x, w = ints((T, K), 1, BF16), ints((2, N, K), 2, BF16)
+    off = torch.tensor([T - 300, T], dtype=torch.int32, device="cuda")
+    y = mm_grouped(x, w, off)
+    for rows, e in ((slice(0, 300), 0), (slice(T - 700, T - 300), 0), (slice(T - 300, T), 1)):
+        assert torch.equal(y[rows], (x[rows].double() @ w[e].double().t()).to(BF16))
+    del y
+    E, N, K = 1024, 2048, 1104                           # 2.3e9 results of 4 bytes
+    dy, x = ints((3000, N), 3, BF16), ints((3000, K), 4, BF16)
+    off = torch.zeros(E, dtype=torch.int32, device="cuda")
+    off[10:], off[E - 2:], off[E - 1] = 17, 1500, 3000
+    dw = mm_grouped_wgrad(dy, x, off)
+    for e, a, b in ((10, 0, 17), (E - 2, 17, 1500), (E - 1, 1500, 3000)):
+        assert torch.equal(dw[e], (dy[a:b].double().t() @ x[a:b].double()).float())
+    assert bool((dw[11:E - 2] == 0).all()) and bool((dw[:10] == 0).all())
+
+
+def test_offsets_inside_a_larger_tensor():
+    x, w = ints((50, 64), 1, BF16), ints((3, 72, 64), 2, BF16)
+    ends = torch.tensor([0, 20, 20, 50, 0], dtype=torch.int32, device="cuda")
+    want = exact_mm(x, w, ends[1:4]).to(BF16)
+    assert torch.equal(mm_grouped(x, w, ends[1:4]), want)
+    assert torch.equal(mm_grouped(x, w, ends[1:4].repeat_interleave(2)[::2]), want)
+
+
 def test_two_streams_at_once():
     """calls in flight together on two streams, with workspaces (split products, copied operands): each its own"""
     ws = [ints((1, 768, 8193), i, BF16) for i in range(2)]
