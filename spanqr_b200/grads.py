@@ -19,7 +19,7 @@ from . import _lib
 
 # SPANQR_F32, SPANQR_F16, SPANQR_BF16
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_dtype, _shape = attrgetter("dtype"), attrgetter("shape")
+_dtype, _same_size = attrgetter("dtype"), torch.Tensor.is_same_size
 _contiguous = torch.Tensor.is_contiguous
 _PLAIN = {torch.Tensor, torch.nn.Parameter}
 _ptr, _numel, _device = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
@@ -151,7 +151,7 @@ def clip_grads(tensors, max_norm, *, out=None, group=None):
             raise ValueError(f"out must hold {len(ts)} tensors (got {len(res)})")
         if odev != dev:
             raise ValueError(f"out must be on the tensors' device (got cuda:{odev} and cuda:{dev})")
-        if list(map(_shape, ts)) != list(map(_shape, res)):
+        if not all(map(_same_size, ts, res)):
             i = next(i for i, (t, o) in enumerate(zip(ts, res)) if t.shape != o.shape)
             raise ValueError(f"out[{i}] has shape {tuple(res[i].shape)}, its input {tuple(ts[i].shape)}")
         if out_types != types:

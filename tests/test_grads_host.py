@@ -99,3 +99,33 @@ def test_norm_argument_checks_before_any_device_work():
     assert L.spanqr_grad_norm(None, _at(k), _at(n), 1, None, BASE, BASE, 1 << 30, None) == ARG
     assert L.spanqr_grad_norm(_at(p), _at(k), _at(n), 1, BASE + 4, BASE, BASE, 1 << 30, None) == ARG  # fp64 off 8 bytes
     assert L.spanqr_grad_norm(_at(p), _at(k), _at(n), 1, None, BASE, BASE, 64, None) == WS
+
+
+@pytest.mark.parametrize("current,index", [(0, 0), (0, 3), (2, 1)])
+def test_a_launch_is_on_the_tensors_device_and_its_stream(monkeypatch, current, index):
+    """with the tensors' device current (entered only where it is not), on that device's current stream"""
+    state = {"current": current}
+
+    class Device:
+        def __init__(self, i):
+            self.i = i
+
+        def __enter__(self):
+            self.was, state["current"] = state["current"], self.i
+
+        def __exit__(self, *a):
+            state["current"] = self.was
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: state["current"])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    calls = []
+
+    def fn(*args):
+        calls.append((state["current"], args))
+        return args[0]
+    _lib.launch(index, fn, lambda: "never asked", 0, "x")
+    assert calls == [(index, (0, "x", 100 + index))] and state["current"] == current
+    with pytest.raises(_lib.SpanqrError, match="the call"):
+        _lib.launch(index, fn, lambda: "the call", 2)
+    assert state["current"] == current
