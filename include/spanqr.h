@@ -42,8 +42,10 @@ typedef struct CUstream_st* spanqr_stream_t; /* the same type as cudaStream_t */
 
 enum spanqr_status {
     SPANQR_OK = 0,
-    SPANQR_ERR_SHAPE = 1,     /* r not a multiple of 32, r > 512, K < r, batch < 1 (no Householder fallback)   */
-    SPANQR_ERR_ARG = 2,       /* null or misaligned pointer, leading dimension too small or not a multiple of 4 */
+    SPANQR_ERR_SHAPE = 1,     /* r not a multiple of 32, r > 512, K < r, batch < 1 (no Householder fallback);    */
+                              /* sizes of a grouped product out of range                                        */
+    SPANQR_ERR_ARG = 2,       /* null or misaligned pointer, leading dimension too small or not a multiple of 4, */
+                              /* unknown type, negative count or maximal norm                                   */
     SPANQR_ERR_WORKSPACE = 3, /* workspace too small or not 256-byte aligned                                    */
     SPANQR_ERR_CUDA = 4,      /* a CUDA runtime call or kernel launch failed                                    */
     SPANQR_ERR_DEVICE = 5,    /* the device status word reports a failure (spanqr_read_status)                  */
@@ -193,7 +195,7 @@ int spanqr_trsm_f32(const float* X, long long ldx, const float* Z, const float* 
 
 /*
  * Kernel timing (no reference counterpart; the reference stamps %globaltimer under CHOL_DEBUG, chol.cu:17-23).
- * mode 1: the orth entry points bracket every kernel they launch with CUDA events on the launching stream;
+ * mode 1: the entry points bracket every kernel they launch with CUDA events on the launching stream;
  * mode 2: they only count their launches (no events, nothing added to the streams); mode 0: off.
  * spanqr_timing_collect waits for the events, adds each kind's device time to ms[kind] and its kernel launches to
  * launches[kind] for kind < nkinds (k_ns_update counts its operand-image kernel too), and forgets them.  Kinds are numbered 0..spanqr_kernel_kinds()-1 (names from
@@ -282,8 +284,8 @@ int spanqr_grad_clip(const void* const* in, const int* in_type, void* const* out
  *   `type`; zeros for an expert without rows.  Summed by the tensor cores over 512 rows (fp32 results) or 2048, those sums
  *   in fp32 to nearest.
  * Operands are read where they lie if every row starts on 16 bytes and none overlap (a 16-byte aligned address, leading
- *   dimension and, for E > 1, expert stride multiples of 8, leading dimension >= the row, expert stride >= the matrix); others are first
- *   copied to the workspace.
+ *   dimension and, for E > 1, expert stride multiples of 8, leading dimension >= the row, expert stride >= the matrix);
+ *   others are first copied to the workspace.
  * The workspaces, 256-byte aligned, need no initialisation; calls in flight at the same time need different ones.  Their
  *   sizes (often 0, then ws may be NULL) come from the _workspace_bytes of the same sizes, where `copies` says which
  *   operands have to be copied: 1 the first, 2 the second (plus 4 if the weights are transposed).

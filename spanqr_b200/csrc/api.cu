@@ -214,8 +214,9 @@ int spanqr_version(void) { return 100; }
 const char* spanqr_strerror(int code) {
     switch (code) {
         case SPANQR_OK: return "ok";
-        case SPANQR_ERR_SHAPE: return "unsupported shape (r must be a multiple of 32 in [32, 512], K >= r, 1 <= batch <= 65535)";
-        case SPANQR_ERR_ARG: return "bad argument (null or not 16-byte aligned pointer, or bad leading dimension)";
+        case SPANQR_ERR_SHAPE: return "unsupported shape (orth: r must be a multiple of 32 in [32, 512], K >= r, 1 <= batch <= 65535; "
+                                      "grouped products: 1 to 1024 experts, at most 2^30 rows, 1 <= N, K <= 2^24)";
+        case SPANQR_ERR_ARG: return "bad argument (null or misaligned pointer, bad leading dimension, type or count)";
         case SPANQR_ERR_WORKSPACE: return "workspace too small or not 256-byte aligned";
         case SPANQR_ERR_CUDA: return "CUDA error";
         case SPANQR_ERR_DEVICE: return "device reported a failure";
@@ -965,7 +966,8 @@ int spanqr_grad_clip(const void* const* in, const int* in_type, void* const* out
         if (norm) e = timed(K_GRAD_SUMSQ, st, [&] { return launch_grad_finish(sums, nparts, nullptr, norm, false, st); });
     } else if (e == cudaSuccess) {
         e = timed(K_GRAD_SCALE, st,
-                  [&] { return launch_grad_scale(es.data(), (int)es.size(), sums, nparts, max_norm, norm, !sumsq, st); }, launches);
+                  [&] { return launch_grad_scale(es.data(), (int)es.size(), sums, nparts, max_norm, norm, !sumsq, st); },
+                  launches);
     }
     return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
 } catch (const std::bad_alloc&) {
@@ -1016,7 +1018,8 @@ struct Rows {
 size_t copy_bytes(long long planes, long long rows, long long cols) {
     return al256((size_t)planes * rows * ((cols + 7) / 8 * 8) * 2);
 }
-// the operand for the kernel (ends: of the experts, for one with a plane for each); what has to be copied becomes a job and takes its place in the workspace at `at`
+// the operand for the kernel (ends: of the experts, for one with a plane for each); what has to be copied becomes a job and
+// takes its place in the workspace at `at`
 MmOperand readable(const Rows& r, const int* ends, char*& at, PadJob* jobs, int& count) {
     const long long cols8 = (r.cols + 7) / 8 * 8;
     MmOperand o{r.p, r.cols, r.rows, r.rows > 1 ? r.ld : cols8, ends ? r.planes : 0, r.plane, r.mn};
