@@ -274,9 +274,10 @@ int spanqr_grad_clip(const void* const* in, const int* in_type, void* const* out
  * orth take).  x [T, K] and dy, y [T, N] are row-major 16-bit matrices (type SPANQR_F16 or SPANQR_BF16, all alike) whose
  * rows are sorted by expert: expert e's rows are offsets[e - 1] .. offsets[e] (offsets: DEVICE array of E ends, read on
  * the device; ends that decrease or lie outside [0, T] are clamped to the nearest that do not).  1 <= E <= 1024,
- * 0 <= T <= 2^30, 1 <= N, K <= 2^24.  Leading dimensions and expert strides are not negative.
+ * 0 <= T <= 2^30, 1 <= N, K <= 2^18 (weight gradients: 2^24).  Leading dimensions and expert strides are not negative.
  *
- * spanqr_mm_grouped: y[t] = w[e(t)] x[t], summed in fp32 and rounded once.  w holds E matrices, stride_w elements apart: N x
+ * spanqr_mm_grouped: y[t] = w[e(t)] x[t], summed in fp32 by the tensor cores (toward zero: about 1e-9 K of the result) and
+ *   rounded once.  w holds E matrices, stride_w elements apart: N x
  *   K with leading dimension ldw, or with w_transposed K x N, so that dx = the product of dy with the transposed weights is
  *   the same call.  y: any address and leading dimension >= N; it must overlap no input.  Rows from offsets[E - 1] on are
  *   zeroed (zero_tail != 0) or left as they are.

@@ -215,7 +215,7 @@ const char* spanqr_strerror(int code) {
     switch (code) {
         case SPANQR_OK: return "ok";
         case SPANQR_ERR_SHAPE: return "unsupported shape (orth: r must be a multiple of 32 in [32, 512], K >= r, 1 <= batch <= 65535; "
-                                      "grouped products: 1 to 1024 experts, at most 2^30 rows, 1 <= N, K <= 2^24)";
+                                      "grouped products: 1 to 1024 experts, at most 2^30 rows, 1 <= N, K <= 2^18 (weight gradients: 2^24))";
         case SPANQR_ERR_ARG: return "bad argument (null or misaligned pointer, bad leading dimension, type or count)";
         case SPANQR_ERR_WORKSPACE: return "workspace too small or not 256-byte aligned";
         case SPANQR_ERR_CUDA: return "CUDA error";
@@ -988,6 +988,9 @@ int* mm_status() {
 }
 
 constexpr int MM_MAX_T = 1 << 30, MM_MAX_DIM = 1 << 24;
+// The products' sums over the contracted dimension stay in the tensor core, which rounds toward zero: about 1e-9 of the
+// result per element.  At 2^18 that is 2.6e-4, as much as the rounding to fp16; both sides, because dx contracts N.
+constexpr int MM_MAX_CONTRACTED = 1 << 18;
 
 int check_mm_sizes(int T, int E, int N, int K) {
     const bool ok = T >= 0 && T <= MM_MAX_T && E >= 1 && E <= MM_MAX_E && N >= 1 && N <= MM_MAX_DIM && K >= 1 && K <= MM_MAX_DIM;
@@ -1044,6 +1047,7 @@ extern "C" {
 int spanqr_mm_grouped_workspace_bytes(int T, int E, int N, int K, int copies, size_t* bytes) {
     const int rc = check_mm_sizes(T, E, N, K);
     if (rc) return rc;
+    if (N > MM_MAX_CONTRACTED || K > MM_MAX_CONTRACTED) return SPANQR_ERR_SHAPE;
     if (!bytes || copies < 0 || copies > 7) return SPANQR_ERR_ARG;
     // the plan on the most SMs: one on fewer splits no more
     *bytes = T > 0 ? al256(mm_plan(T, E, N, K, MAX_SMS).ws) + (copies & 1 ? copy_bytes(1, T, K) : 0) +
@@ -1057,6 +1061,7 @@ int spanqr_mm_grouped(const void* x, long long ldx, const void* w, long long ldw
                       void* ws, size_t ws_bytes, spanqr_stream_t stream) {
     const int rc = check_mm(type, T, E, N, K, offsets);
     if (rc) return rc;
+    if (N > MM_MAX_CONTRACTED || K > MM_MAX_CONTRACTED) return SPANQR_ERR_SHAPE;
     if (T == 0) return SPANQR_OK;
     const Rows rx{x, K, T, ldx, 1, 0, false};
     const Rows rw{w, w_transposed ? N : K, w_transposed ? K : N, ldw, E, E > 1 ? stride_w : 0, w_transposed != 0};

@@ -46,10 +46,11 @@ __device__ __forceinline__ void store_rows(const char* stage, OUT* row, int ld, 
 __device__ __forceinline__ bool ragged(int left) { return left < BK && left % 16 != 0; }
 
 // The tensor core rounds toward zero each time it adds 16 products to its fp32 accumulator: over n additions of terms of
-// random sign the sum comes out about n * 3e-8 of itself too small.  So the accumulator is taken every DRAIN stages and
-// added to fp32 sums in registers, rounded to nearest, while the products go on in the other accumulator.  For fp32
-// results every 512 rows (measured 4e-7 off in all at 5000 rows, as a sum in fp32 is); for 16-bit results, whose own
-// rounding is 2^-9 or 2^-12, every 2048, which keeps the bias from growing with the length.  The reads of TMEM
+// random sign the sum comes out about n * 1.5e-8 of itself too small (measured on 4096x4096 results: 8.1e-7 at 1000 rows,
+// 4.6e-6 at 5000, 2.0e-5 at 20000, 1.0e-4 at 100000).  So the accumulator is taken every DRAIN stages and added to fp32 sums
+// in registers, rounded to nearest, while the products go on in the other accumulator: every 512 rows for fp32 results,
+// which are then 4.6e-7 to 5.4e-7 off in all at those lengths (sums of fp32 products in fp32: 2.5e-7 to 4.6e-6); every 2048
+// for 16-bit results, whose own rounding is 2^-9 or 2^-12, so that the bias does not grow with the length.  The reads of TMEM
 // take tensor-core time: 16384 rows, 8 experts of 5120x2048 in bf16, with one copy warp: 285 us drained every 256 rows, 258
 // every 512, 252 every 4096.
 template <typename OUT, bool TMA_OUT>

@@ -139,6 +139,28 @@ def test_wgrad_gaussian(T, E, N, K, dtype):
     assert bool(((mm_grouped_wgrad(dy, x, off).double() - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("T", [1000, 20000, 100000])
+def test_wgrad_does_not_drift_with_the_rows(T):
+    """sums of random sign: the tensor core's rounding toward zero stays that of 512 rows (32 additions of at most half a
+    unit of 2^-23 on average, 32 * 2^-24 = 1.9e-6 of the result at the most), the sums of those are to nearest"""
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x, dy = (torch.randn(T, n, device="cuda", generator=g).to(BF16) for n in (256, 512))
+    off = offsets([T // 3, T - T // 3])
+    want, got = exact_wgrad(dy, x, off), mm_grouped_wgrad(dy, x, off).double()
+    assert float((got - want).norm() / want.norm()) <= 2e-6
+    assert abs(float(((got - want) * want.sign()).sum() / want.abs().sum())) <= 2e-6
+
+
+def test_product_over_a_long_contracted_dimension():
+    g = torch.Generator(device="cuda").manual_seed(3)
+    K = 1 << 18
+    x, w = torch.randn(40, K, device="cuda", generator=g).to(BF16), torch.randn(1, 64, K, device="cuda", generator=g).to(BF16)
+    off = offsets([40])
+    want = exact_mm(x, w, off)
+    err = (mm_grouped(x, w, off).double() - want).norm() / want.norm()
+    assert float(err) <= 2.0 ** -8 + K / 16 * 2.0 ** -24          # half a step, and the additions toward zero
+
+
 @pytest.mark.parametrize("counts", [[0, 0, 40], [40, 0, 0], [0, 40, 0], [13, 14, 13], [0, 0, 0], [1, 0, 1]])
 @pytest.mark.parametrize("scale", [1, 20])
 def test_uneven_experts(counts, scale):

@@ -91,6 +91,8 @@ def test_argument_checks_before_any_device_work():
     for bad in (dict(T=-1), dict(T=(1 << 30) + 1), dict(E=0), dict(E=1025), dict(N=0), dict(K=0), dict(K=(1 << 24) + 1)):
         assert mm(**bad) == SHAPE, bad
         assert wgrad(**bad) == SHAPE, bad
+    for big in (dict(K=(1 << 18) + 1, ldx=1 << 19, ldw=1 << 19), dict(N=(1 << 18) + 1, ldy=1 << 19)):   # sums of products
+        assert mm(**big) == SHAPE, big
     for bad in (dict(x=None), dict(x=A + 1), dict(ldx=-64), dict(w=None), dict(w=A + 1), dict(ldw=-64), dict(sw=-8),
                 dict(off=None), dict(off=A + 2), dict(y=None), dict(y=A + 1), dict(ldy=127), dict(type=0), dict(type=3)):
         assert mm(**bad) == ARG, bad
