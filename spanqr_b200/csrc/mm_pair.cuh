@@ -242,12 +242,23 @@ cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, int threads, int smem
 template <typename C, auto kernel, typename... A>
 cudaError_t launch_pairs(int pairs, int E, bool behind, cudaStream_t st, const A&... args) {
     static SmemOnce once;   // of this kernel
-    const cudaError_t e = once.allow(reinterpret_cast<const void*>(kernel), C::FIXED + 2 * (MM_MAX_E + 1) * (int)sizeof(int));
+    const void* const fn = reinterpret_cast<const void*>(kernel);
+    const int most = C::FIXED + 2 * (MM_MAX_E + 1) * (int)sizeof(int), smem = C::FIXED + 2 * (E + 1) * (int)sizeof(int);
+    cudaError_t e = once.allow(fn, most);
     if (e != cudaSuccess) return e;
-    const int smem = C::FIXED + 2 * (E + 1) * (int)sizeof(int);
-    if (behind) return launch_behind(kernel, dim3(2 * pairs), THREADS, smem, st, args...);
-    kernel<<<2 * pairs, THREADS, smem, st>>>(args...);
-    return cudaGetLastError();
+    for (int attempt = 0;; ++attempt) {
+        if (behind) {
+            e = launch_behind(kernel, dim3(2 * pairs), THREADS, smem, st, args...);
+        } else {
+            kernel<<<2 * pairs, THREADS, smem, st>>>(args...);
+            e = cudaGetLastError();
+        }
+        // a device that was reset since has forgotten the limit
+        if (e != cudaErrorInvalidValue || attempt > 0) return e;
+        cudaGetLastError();
+        e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        if (e != cudaSuccess) return e;
+    }
 }
 
 }  // namespace mm
