@@ -358,6 +358,17 @@ def test_fp16_overflow_is_infinite():
     assert bool((mm_grouped_wgrad(x, -x, off) == -200.0 * 200.0 * 20).all())
 
 
+@pytest.mark.parametrize("dtype,tiny", [(FP16, 2.0 ** -24), (BF16, 2.0 ** -133)])
+def test_subnormal_values(dtype, tiny):
+    """whole multiples of the type's smallest value: exact sums, none of them flushed to zero"""
+    T, N, K = 70, 40, 64
+    x, w, dy = (ints((T, K), 1, F32) * tiny).to(dtype), ints((2, N, K), 2, dtype), ints((T, N), 3, dtype)
+    off = offsets([30, 40])
+    assert bool((x != 0).any())
+    assert torch.equal(mm_grouped(x, w, off), exact_mm(x, w, off).to(dtype))
+    assert torch.equal(mm_grouped_wgrad(dy, x, off), exact_wgrad(dy, x, off).to(F32))
+
+
 @pytest.mark.parametrize("T", [48, 2000])
 def test_streams_graphs_and_same_bits(T):
     E, N, K = 4, 264, 512
