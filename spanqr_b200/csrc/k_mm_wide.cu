@@ -271,11 +271,14 @@ MmPlan mm_plan(int T, int E, int N, int K, int nsm) {
     // of 256 for each of 8 in its features): 18 / 13 / 14 / 19.
     p.nt = T <= 20LL * E ? 32 : T <= 44LL * E ? 64 : T <= 96LL * E ? 128 : 256;
     while (p.nt > 32 && tiles(p.nt) * 4 < 3 * pairs) p.nt /= 2;
-    // The split saves what the busiest pair has beyond its share, about 0.17 us a stage, and costs its partial sums and the
-    // second kernel, about 7 us.  Measured (us, bf16): 64 rows, one expert of 768x17408 (6 tiles of 272 stages): 51 whole,
-    // 19 split; one row, 4096x4096 (16 of 64): 16.5 and 15.7; 16 rows, 16 experts of 1024x2048 (40 of 32): 13.9 and 18.9.
-    const long long kb = (K + BK - 1) / BK;
-    p.split = p.nt == 32 && kb * (pairs - tiles(32)) > 50 * pairs;
+    // Whole, a pair takes about 0.165 us for each of a tile's kb stages, the others idling.  Split, all pairs take 0.2 us a
+    // stage out of L2, and all the weights that are read for the first time come at HBM's rate (0.48 us a stage and pair);
+    // the partial sums and the second kernel cost 6.5 us.  Measured (us whole / split, bf16): 8 rows and one matrix of
+    // 256x8192 (one tile of 128 stages): 26 / 15; 256x4096: 16 / 11; 256x2048: 10 / 10; 2048x6144 (8 of 96): 21 / 16;
+    // 4096x4096 (16 of 64): 16 / 17; 6144x6144 (24 of 96): 21 / 23; 256 rows and 768x17408 (24 tiles of 272 stages over the
+    // weights of 3): 50 / 29; 16 rows, 16 experts of 1024x2048 (40 of 32): 14 / 19.
+    const long long kb = (K + BK - 1) / BK, first = ntn * some, all = tiles(32);
+    p.split = p.nt == 32 && kb * (10 * pairs - (12 * all > 30 * first ? 12 * all : 30 * first)) > 400LL * pairs;
     const long long most = ntn * (T / p.nt + some);
     p.tiles = most;
     p.pairs = p.split || most > pairs ? pairs : (int)most;
