@@ -138,6 +138,8 @@ def clip_grads(tensors, max_norm, *, out=None, group=None):
     infinite gradient gives the coefficient 0 (finite values become 0, infinite ones NaN) and a NaN makes every output
     NaN, so a step can be skipped by looking at the norm alone.  A finite norm above fp32's largest value reads as
     infinity, but the scaling uses its fp64 value.  Autograd does not see the scaling."""
+    if torch.is_tensor(max_norm):
+        raise TypeError("max_norm must be a number (reading a tensor would wait for the device)")
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must be a number >= 0 (got {max_norm})")

@@ -28,6 +28,8 @@ def test_refusals():
     for bad in (-1.0, float("nan")):
         with pytest.raises(ValueError, match="max_norm"):
             clip_grads([], bad)
+    with pytest.raises(TypeError, match="number"):
+        clip_grads([], torch.tensor(1.0))
 
 
 @pytest.mark.parametrize("make,want", [

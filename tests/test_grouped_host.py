@@ -77,6 +77,13 @@ def test_overlap():
     with pytest.raises(ValueError, match="overlaps x"):
         g._no_overlap(b[:33], x=b[32:])
     g._no_overlap(b[:0], x=b)
+    g._no_overlap(b[:, :40], x=b[:, 40:])                 # columns side by side in one buffer
+    g._no_overlap(b[:, 40:], x=b[3:, :40])
+    for out, x in ((b[:, :41], b[:, 40:]), (b[:, 40:], b[:, :41]), (b[:, 20:], b[:, :30]), (b, b[:, :1]), (b[:, 5:9], b)):
+        with pytest.raises(ValueError, match="overlaps x"):
+            g._no_overlap(out, x=x)
+    with pytest.raises(ValueError, match="overlaps x"):   # other strides: by their spans
+        g._no_overlap(b.view(-1)[:64 * 32].view(32, 64)[:, :8], x=b.view(-1)[8:8 + 32 * 32].view(32, 32)[:, :8])
 
 
 def mm(x=A, ldx=64, w=A, ldw=64, sw=64 * 128, tr=0, off=A, y=A, ldy=128, type=BF16, T=16, E=2, N=128, K=64):
