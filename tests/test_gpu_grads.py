@@ -249,8 +249,13 @@ def test_streams_and_captured_graphs():
 
 
 def test_under_a_process_group():
+    import socket
+
     import torch.distributed as dist
-    dist.init_process_group("nccl", init_method="tcp://127.0.0.1:29517", rank=0, world_size=1)
+    with socket.socket() as free:
+        free.bind(("127.0.0.1", 0))
+        port = free.getsockname()[1]
+    dist.init_process_group("nccl", init_method=f"tcp://127.0.0.1:{port}", rank=0, world_size=1)
     try:
         ts = mixed(7)
         want = norm64(ts)

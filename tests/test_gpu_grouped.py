@@ -6,6 +6,7 @@ step of its type, plus what the fp32 sums lose: the tensor core rounds toward ze
 most 2^-22 of S, the sum of the absolute terms, each time), and mm_grouped_wgrad adds its sums of 512 rows (32 such
 additions) to nearest."""
 import ctypes
+from pathlib import Path
 
 import pytest
 import torch
@@ -531,4 +532,4 @@ torch.cuda.synchronize()
 assert bool((y == 64).all()) and bool((dw[0] == 15 * 64).all()) and bool((dw[1] == 25 * 64).all())
 assert n.item() == m.item() > 1 and abs(c.norm().item() - 1) < 1e-5
 """
-    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=Path(__file__).resolve().parent.parent)
