@@ -87,7 +87,9 @@ def _run_norm(ts, types, dev, sumsq, norm):
 
 def _run_clip(ins, in_types, outs, out_types, dev, max_norm, sumsq, norm):
     ws = _workspace(norm, len(ins))
-    pi, po, sizes = array("Q", map(_ptr, ins)), array("Q", map(_ptr, outs)), array("q", map(_numel, ins))
+    sizes = array("q", map(_numel, ins))
+    ins = _signs(ins, outs, sizes)
+    pi, po = array("Q", map(_ptr, ins)), array("Q", map(_ptr, outs))
     try:
         _lib.launch(dev, _lib.lib().spanqr_grad_clip, lambda: f"clip_grads({len(ins)} tensors)", _at(pi), _at(in_types),
                     _at(po), _at(out_types), _at(sizes), len(ins), max_norm, None if sumsq is None else sumsq.data_ptr(),
@@ -96,6 +98,21 @@ def _run_clip(ins, in_types, outs, out_types, dev, max_norm, sumsq, norm):
         if e.code != 7:   # SPANQR_ERR_OVERLAP
             raise
         raise ValueError("clip_grads: an output overlaps another tensor of the call (one tensor listed twice?)") from None
+
+
+def _signs(ins, outs, sizes):
+    """ins, with a lazily negated one-element tensor resolved where its output is not one too (two such are scaled as
+    they lie).  `z.conj().imag` is such a view; of more elements it has gaps, so that it was copied and resolved already."""
+    if 1 not in sizes:
+        return ins
+    ins = list(ins)
+    for i in [i for i, n in enumerate(sizes) if n == 1]:
+        neg = outs[i].is_neg()
+        if ins[i].is_neg() != neg:
+            if neg:
+                raise ValueError(f"out[{i}] is a lazily negated view and its input is not: give a tensor of its own")
+            ins[i] = ins[i].resolve_neg()
+    return ins
 
 
 def _group_sumsq(ts, types, dev, group):

@@ -278,3 +278,25 @@ def test_clipped_gradients_go_to_orth():
         q, g = q.double(), g.double()
         assert float((q.t() @ q - torch.eye(128, device="cuda")).abs().max()) <= 3e-7
         assert float((g - q @ (q.t() @ g)).norm() / g.norm()) <= 1e-5
+
+
+def test_lazily_negated_tensors():
+    """the imaginary part of a conjugate (the gradient of b in complex(a, b).conj() is one) into new and given tensors, in
+    place, and refused as another tensor's output"""
+    z = torch.tensor([3.0 + 4.0j], device="cuda")
+    x, y = z.conj().imag, torch.zeros(1, device="cuda")
+    assert x.is_neg() and x.is_contiguous() and x.item() == -4.0
+    (a,), n = clip_grads([x], 8.0)
+    clip_grads([x], 8.0, out=[y])
+    assert a.item() == y.item() == -4.0 and n.item() == 4.0 and x.item() == -4.0
+    (a,), _ = clip_grads([x], 2.0)
+    check_clipped(a, x, coef64(4.0, 2.0))
+    with pytest.raises(ValueError, match="lazily negated"):
+        clip_grads([y], 1.0, out=[x])
+    want = x.clone()
+    clip_grads([x], 2.0, out=[x])
+    check_clipped(x, want, coef64(4.0, 2.0))
+    assert z.item().real == 3.0
+    v = torch.arange(1.0, 6.0, device="cuda").to(torch.cfloat).mul(1j).conj().imag      # with gaps
+    (c,), _ = clip_grads([v], 100.0)
+    assert c.tolist() == [-1.0, -2.0, -3.0, -4.0, -5.0]

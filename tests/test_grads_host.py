@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from spanqr_b200 import _lib, clip_grads, grad_norm
-from spanqr_b200.grads import _dense
+from spanqr_b200.grads import _dense, _signs
 
 OK, ARG, WS, OVERLAP = 0, 2, 3, 7
 BASE = 1 << 40          # device addresses that no call below dereferences: each fails its checks first
@@ -131,3 +131,16 @@ def test_a_launch_is_on_the_tensors_device_and_its_stream(monkeypatch, current, 
     with pytest.raises(_lib.SpanqrError, match="the call"):
         _lib.launch(index, fn, lambda: "the call", 2)
     assert state["current"] == current
+
+
+def test_lazily_negated_tensors_keep_their_sign():
+    """the imaginary part of a conjugate holds its values negated: one element of it has no gaps and passes as contiguous"""
+    z = torch.tensor([3.0 + 4.0j]).conj().imag
+    plain, two = torch.tensor([7.0]), torch.zeros(2)
+    assert z.is_neg() and z.is_contiguous() and z.item() == -4.0
+    ins = [two, z, plain]
+    got = _signs(ins, [torch.empty_like(t) for t in ins], array("q", [2, 1, 1]))
+    assert not got[1].is_neg() and got[1].item() == -4.0 and got[0] is two and got[2] is plain and ins[1] is z
+    assert _signs([z], [z], array("q", [1]))[0] is z             # in place: scaled as it lies
+    with pytest.raises(ValueError, match=r"out\[0\] is a lazily negated"):
+        _signs([plain], [z], array("q", [1]))
