@@ -40,6 +40,8 @@ def _workspace(fn, x, *sizes):
 def _rows(x):
     """x [T, K] with contiguous rows, its address and row stride, and whether the library has to copy it to read it (rows
     off 16 bytes or over one another)"""
+    if x.is_neg():   # (z.conj().imag: its memory holds the values negated)
+        x = x.resolve_neg()
     ld, step = x.stride()
     if step != 1 and x.shape[1] > 1 or ld < 0:
         x = x.contiguous()
@@ -51,6 +53,8 @@ def _rows(x):
 def _weights(w):
     """w [E, N, K] with one of its last two dimensions contiguous, its address, row stride, expert stride, whether it is
     stored [E, K, N], and whether the library has to copy it to read it"""
+    if w.is_neg():
+        w = w.resolve_neg()
     E, N, K = w.shape
     plane, sn, sk = w.stride()
     if sk == 1 or K == 1:
@@ -79,6 +83,13 @@ def _side_by_side(a, b):
     step = a.stride(0) * a.element_size()
     gap = (b.data_ptr() - a.data_ptr()) % step if step else 0   # from a row of a to the next start of one of b
     return a.shape[1] * a.element_size() <= gap and gap + b.shape[1] * b.element_size() <= step
+
+
+def _check_out(out, **others):
+    """refuses an output that cannot be written as it lies: negated lazily, or over one of the other tensors"""
+    if out.is_neg():
+        raise ValueError("out is a lazily negated view (out.resolve_neg() gives a tensor of its own)")
+    _no_overlap(out, **others)
 
 
 def _no_overlap(out, **others):
@@ -203,7 +214,7 @@ def mm_grouped(x, w, offsets, *, out=None):
         raise TypeError(f"out must be {x.dtype} on {x.device} (got {out.dtype} on {out.device})")
     if N > 1 and out.stride(1) != 1 or T > 1 and out.stride(0) < N:
         raise ValueError("out must have contiguous rows that do not overlap")
-    _no_overlap(out, x=x, w=w, offsets=offsets)
+    _check_out(out, x=x, w=w, offsets=offsets)
     _product(_rows(x), _weights(w), offsets, T, E, N, K, out)
     if not out.is_inference():
         torch.autograd.graph.increment_version(out)
@@ -236,7 +247,7 @@ def mm_grouped_wgrad(dy, x, offsets, *, out=None, dtype=None):
         raise ValueError(f"out must be contiguous with shape {(E, N, K)}")
     if out.dtype not in (torch.float32, x.dtype) or out.device != x.device:
         raise TypeError(f"out must be fp32 or {x.dtype} on {x.device} (got {out.dtype} on {out.device})")
-    _no_overlap(out, dy=dy, x=x, offsets=offsets)
+    _check_out(out, dy=dy, x=x, offsets=offsets)
     _wgrad(_rows(dy), _rows(x), offsets, T, E, N, K, None, out)
     if not out.is_inference():
         torch.autograd.graph.increment_version(out)

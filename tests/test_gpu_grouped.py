@@ -533,3 +533,22 @@ assert bool((y == 64).all()) and bool((dw[0] == 15 * 64).all()) and bool((dw[1] 
 assert n.item() == m.item() > 1 and abs(c.norm().item() - 1) < 1e-5
 """
     subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=Path(__file__).resolve().parent.parent)
+
+
+def test_lazily_negated_operands():
+    """fp16 imaginary parts of conjugates, whose memory holds the values negated: one column of them has usable strides"""
+    def negated(t):
+        z = torch.zeros(t.shape, dtype=torch.complex32, device="cuda")
+        z.imag.copy_(-t)
+        assert z.conj().imag.is_neg()
+        return z.conj().imag
+    off = offsets([20, 17])
+    for N, K in ((24, 1), (1, 24), (24, 40), (1, 1)):
+        x, w, dy = ints((37, K), 1, FP16), ints((2, N, K), 2, FP16), ints((37, N), 3, FP16)
+        want, dwant = exact_mm(x, w, off).to(FP16), exact_wgrad(dy, x, off).to(F32)
+        for a, b in ((negated(x), w), (x, negated(w)), (negated(x), negated(w))):
+            assert torch.equal(mm_grouped(a, b, off), want)
+        for a, b in ((negated(dy), x), (dy, negated(x))):
+            assert torch.equal(mm_grouped_wgrad(a, b, off), dwant)
+    with pytest.raises(ValueError, match="lazily negated"):
+        mm_grouped(x, w, off, out=negated(dy))

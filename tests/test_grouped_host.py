@@ -128,3 +128,25 @@ def test_workspace_bytes():
         assert getattr(L, fn)(16, 2, 64, 64, bad, ctypes.byref(n)) == ARG
     assert L.spanqr_mm_grouped_workspace_bytes(16, 0, 64, 64, 0, ctypes.byref(n)) == SHAPE
     assert L.spanqr_mm_grouped_workspace_bytes(16, 1, 64, 64, 0, None) == ARG
+
+
+def negated(*shape):
+    """fp16 values 1, 2, ... as the imaginary part of a conjugate: the memory holds their negatives, two elements apart"""
+    z = torch.zeros(shape, dtype=torch.complex32)
+    z.imag.copy_(-torch.arange(1.0, z.numel() + 1).view(shape))
+    return z.conj().imag
+
+
+def test_lazily_negated_operands_are_resolved():
+    """one column of such a view needs no copy for its strides"""
+    for make in (lambda: negated(5, 1), lambda: negated(1, 1), lambda: negated(5, 3)):
+        x = make()
+        assert x.is_neg()
+        y, ptr, _, _ = g._rows(x)
+        assert not y.is_neg() and ptr == y.data_ptr() and torch.equal(y.float(), torch.arange(1.0, x.numel() + 1).view(x.shape))
+    for shape in ((2, 3, 1), (2, 1, 3), (2, 3, 4), (1, 1, 1)):
+        w = negated(*shape)
+        v, ptr = g._weights(w)[:2]
+        assert not v.is_neg() and ptr == v.data_ptr() and torch.equal(v.float(), torch.arange(1.0, w.numel() + 1).view(shape))
+    with pytest.raises(ValueError, match="lazily negated"):
+        g._check_out(negated(5, 1), x=torch.zeros(5, 1))
