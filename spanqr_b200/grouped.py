@@ -12,6 +12,7 @@ device; the offsets are only read on the device, so nothing synchronises with th
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -150,6 +151,15 @@ def _wgrad(rows_dy, rows_x, offsets, T, E, N, K, dtype, out=None):
     return dw
 
 
+def _tracked(*tensors):
+    """whether autograd follows any of them: backward, or forward with a tangent (make_dual)"""
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors) or _dual(*tensors)
+
+
+def _dual(*tensors):
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _backward(ctx, dy):
     x, w, offsets = ctx.saved_tensors
     T, N = dy.shape
@@ -192,7 +202,7 @@ def mm_grouped(x, w, offsets, *, out=None):
     along neither dimension, are copied first, at each call.  Ends that decrease or lie outside [0, T] are clamped to
     the nearest that do not, on the device.
 
-    Differentiable once in x and w (without `out`): dx is this product with the transposed weights, dw is
+    Differentiable once in x and w, backward only (without `out`; forward-mode tangents are refused): dx is this product with the transposed weights, dw is
     mm_grouped_wgrad in w's type; rows behind the last expert get a zero gradient and give none."""
     T, K = _check_rows(x, "x")
     if not torch.is_tensor(w) or w.dim() != 3 or w.shape[2] != K:
@@ -203,8 +213,10 @@ def mm_grouped(x, w, offsets, *, out=None):
     if N < 1:
         raise ValueError("w has no rows")
     offsets = _check_offsets(offsets, x, E)
-    grad = torch.is_grad_enabled() and (x.requires_grad or w.requires_grad)
+    grad = _tracked(x, w)
     if out is None:
+        if grad and _dual(x, w):
+            raise RuntimeError("mm_grouped has no forward-mode derivative (forward AD): it is differentiable backward only")
         return _MmGrouped.apply(x, w, offsets) if grad else _product(_rows(x), _weights(w), offsets, T, E, N, K)
     if grad:
         raise RuntimeError("mm_grouped with out= is not differentiable: leave out away, or use torch.no_grad()")

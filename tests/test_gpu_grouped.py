@@ -552,3 +552,22 @@ def test_lazily_negated_operands():
             assert torch.equal(mm_grouped_wgrad(a, b, off), dwant)
     with pytest.raises(ValueError, match="lazily negated"):
         mm_grouped(x, w, off, out=negated(dy))
+
+
+def test_forward_mode_is_refused():
+    """a tangent is not dropped: every call with one raises"""
+    from torch.autograd import forward_ad
+    x, w, off = ints((40, 64), 1, BF16), ints((2, 72, 64), 2, BF16), offsets([15, 25])
+    want = exact_mm(x, w, off).to(BF16)
+    out = torch.full((40, 72), 3.0, dtype=BF16, device="cuda")
+    with forward_ad.dual_level():
+        xd, wd = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(w, torch.ones_like(w))
+        for a, b in ((xd, w), (x, wd), (xd, wd)):
+            with pytest.raises(RuntimeError, match="forward AD"):
+                mm_grouped(a, b, off)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward AD"):
+                mm_grouped(a, b, off)
+            with pytest.raises(RuntimeError, match="not differentiable"):
+                mm_grouped(a, b, off, out=out)
+        assert torch.equal(mm_grouped(x, w, off), want)      # nothing to follow
+    assert bool((out == 3).all())

@@ -150,3 +150,16 @@ def test_lazily_negated_operands_are_resolved():
         assert not v.is_neg() and ptr == v.data_ptr() and torch.equal(v.float(), torch.arange(1.0, w.numel() + 1).view(shape))
     with pytest.raises(ValueError, match="lazily negated"):
         g._check_out(negated(5, 1), x=torch.zeros(5, 1))
+
+
+def test_what_autograd_follows():
+    from torch.autograd import forward_ad
+    x, r = torch.zeros(3), torch.zeros(3, requires_grad=True)
+    assert not g._tracked(x, x) and g._tracked(x, r)
+    with torch.no_grad():
+        assert not g._tracked(x, r)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones(3))
+        assert g._tracked(d, x) and g._tracked(x, d) and not g._tracked(x, x)
+        with torch.no_grad():
+            assert g._tracked(x, d)                       # tangents pass through no_grad
