@@ -19,6 +19,7 @@ from . import _lib
 from .grads import DTYPES
 
 MAX_EXPERTS = 1024
+INT_MAX = 2 ** 31 - 1
 
 
 @functools.lru_cache(maxsize=4096)
@@ -101,12 +102,21 @@ def _no_overlap(out, **others):
             raise ValueError(f"out overlaps {name}")
 
 
+def _check_sizes(name, *sizes):
+    """the library's error for sizes beyond its int arguments, which would reach it cut to 32 bits (2^32 + 5 rows as 5); it
+    checks its own lower limits itself"""
+    if max(sizes) > INT_MAX:
+        raise _lib.SpanqrError(1, f"{name} {'x'.join(map(str, sizes))}")   # SPANQR_ERR_SHAPE
+
+
 def _check_rows(x, name):
     if not torch.is_tensor(x) or x.dim() != 2:
         raise ValueError(f"{name} must be a 2-D tensor")
+    rows, cols = x.shape
+    if rows > INT_MAX or cols > INT_MAX:
+        _check_sizes(name, rows, cols)
     if x.dtype not in (torch.bfloat16, torch.float16) or not x.is_cuda:
         raise TypeError(f"{name} must be a bf16 or fp16 CUDA tensor (got {x.dtype} on {x.device})")
-    rows, cols = x.shape
     if cols < 1:
         raise ValueError(f"{name} has no columns")
     return rows, cols
@@ -202,14 +212,17 @@ def mm_grouped(x, w, offsets, *, out=None):
     along neither dimension, are copied first, at each call.  Ends that decrease or lie outside [0, T] are clamped to
     the nearest that do not, on the device.
 
-    Differentiable once in x and w, backward only (without `out`; forward-mode tangents are refused): dx is this product with the transposed weights, dw is
-    mm_grouped_wgrad in w's type; rows behind the last expert get a zero gradient and give none."""
+    Differentiable once in x and w, backward only (without `out`; forward-mode tangents are refused): dx is this product with
+    the transposed weights, dw is mm_grouped_wgrad in w's type; rows behind the last expert get a zero gradient and give
+    none."""
     T, K = _check_rows(x, "x")
     if not torch.is_tensor(w) or w.dim() != 3 or w.shape[2] != K:
         raise ValueError(f"w must be a 3-D tensor [E, N, {K}]")
+    E, N, _ = w.shape
+    if N > INT_MAX:
+        _check_sizes("w", E, N, K)
     if w.dtype != x.dtype or w.get_device() != x.get_device():
         raise TypeError(f"w must be {x.dtype} on {x.device}, as x (got {w.dtype} on {w.device})")
-    E, N, _ = w.shape
     if N < 1:
         raise ValueError("w has no rows")
     offsets = _check_offsets(offsets, x, E)

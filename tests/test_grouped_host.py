@@ -163,3 +163,18 @@ def test_what_autograd_follows():
         assert g._tracked(d, x) and g._tracked(x, d) and not g._tracked(x, x)
         with torch.no_grad():
             assert g._tracked(x, d)                       # tangents pass through no_grad
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """an int argument of the library keeps the low 32 bits alone: 2^32 + 5 rows would be 5"""
+    assert _lib._I(2 ** 32 + 5).value == 5
+    one, off = torch.zeros(1, 1).bfloat16(), torch.zeros(1, dtype=torch.int32)
+    long, wide = one.expand(2 ** 32 + 5, 1), one.expand(1, 2 ** 32 + 5)
+    w = one[None]
+    for call in (lambda: mm_grouped(long, w, off), lambda: mm_grouped(wide, w, off), lambda: mm_grouped_wgrad(long, long, off),
+                 lambda: g._check_rows(wide, "x"), lambda: mm_grouped_wgrad(wide, one, off),
+                 lambda: g._check_sizes("w", 1, 2 ** 32 + 8, 1)):
+        with pytest.raises(_lib.SpanqrError, match="unsupported shape") as e:
+            call()
+        assert e.value.code == SHAPE
+    g._check_sizes("w", 1024, 2 ** 31 - 1, 1)
