@@ -88,7 +88,11 @@ def _side_by_side(a, b):
 
 
 def _check_out(out, **others):
-    """refuses an output that cannot be written as it lies: negated lazily, or over one of the other tensors"""
+    """refuses an output that cannot be written as it lies: one that autograd follows (its gradient would go to what it held
+    before), negated lazily, or over one of the other tensors"""
+    if _tracked(out):
+        raise RuntimeError("out requires a gradient, and its values would come from outside autograd: give out.detach(), or "
+                           "use torch.no_grad()")
     if out.is_neg():
         raise ValueError("out is a lazily negated view (out.resolve_neg() gives a tensor of its own)")
     _no_overlap(out, **others)
@@ -204,9 +208,9 @@ def mm_grouped(x, w, offsets, *, out=None):
     """y [T, N] with y[t] = w[e(t)] @ x[t] for the expert e(t) whose rows hold t: x [T, K] and w [E, N, K] of one type
     (bf16 or fp16), offsets int32 [E], the end of each expert's rows.  Experts may be empty; w may be stored [E, N, K] or
     [E, K, N] (pass its transposed view).  Rows from offsets[-1] on belong to no expert: they are zero in a new y and
-    left as they are in `out`, a [T, N] tensor of x's type with contiguous rows that overlaps neither input.  The products
-    are summed in fp32 by the tensor cores, which round toward zero (about 1e-9 K of the result), and rounded once; N and K
-    are at most 2^18.
+    left as they are in `out`, a [T, N] tensor of x's type with contiguous rows that overlaps neither input and needs no
+    gradient.  The products are summed in fp32 by the tensor cores, which round toward zero (about 1e-9 K of the result),
+    and rounded once; N and K are at most 2^18.
 
     Operands whose rows do not start on 16 bytes (K not a multiple of 8, odd strides or addresses), or that are contiguous
     along neither dimension, are copied first, at each call.  Ends that decrease or lie outside [0, T] are clamped to
@@ -250,9 +254,9 @@ def mm_grouped_wgrad(dy, x, offsets, *, out=None, dtype=None):
     """dw [E, N, K] with dw[e] = sum over expert e's rows t of dy[t] x[t]^T: the weight gradient of mm_grouped.  dy [T, N]
     and x [T, K] of one type (bf16 or fp16), offsets int32 [E] as there; an expert without rows gets zeros, and rows from
     offsets[-1] on count nowhere.  dtype is fp32 (the default: what clip_grads and orth_batched take) or the inputs' type;
-    `out`, a contiguous [E, N, K] tensor of either type that overlaps neither input, is overwritten.  Summed in fp32 (over
-    512 rows, or 2048 for 16-bit results, by the tensor cores, those sums to nearest) and rounded once.  Not
-    differentiable."""
+    `out`, a contiguous [E, N, K] tensor of either type that overlaps neither input and needs no gradient, is overwritten.
+    Summed in fp32 (over 512 rows, or 2048 for 16-bit results, by the tensor cores, those sums to nearest) and rounded
+    once.  Not differentiable."""
     T, N = _check_rows(dy, "dy")
     rows, K = _check_rows(x, "x")
     if rows != T:

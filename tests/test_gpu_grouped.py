@@ -571,3 +571,19 @@ def test_forward_mode_is_refused():
                 mm_grouped(a, b, off, out=out)
         assert torch.equal(mm_grouped(x, w, off), want)      # nothing to follow
     assert bool((out == 3).all())
+
+
+def test_outputs_that_autograd_follows_are_refused():
+    x, w, dy, off = ints((40, 64), 1, BF16), ints((2, 72, 64), 2, BF16), ints((40, 72), 3, BF16), offsets([15, 25])
+    leaf, dleaf = torch.ones(40, 72, dtype=BF16, device="cuda"), torch.ones(2, 72, 64, device="cuda")
+    leaf.requires_grad_(), dleaf.requires_grad_()
+    for out, dout in ((leaf, dleaf), (leaf * 2, dleaf * 2)):
+        held = out.detach().clone(), dout.detach().clone()
+        with pytest.raises(RuntimeError, match="out requires a gradient"):
+            mm_grouped(x, w, off, out=out)
+        with pytest.raises(RuntimeError, match="out requires a gradient"):
+            mm_grouped_wgrad(dy, x, off, out=dout)
+        assert torch.equal(out, held[0]) and torch.equal(dout, held[1])
+    with torch.no_grad():
+        mm_grouped(x, w, off, out=leaf), mm_grouped_wgrad(dy, x, off, out=dleaf)
+    assert torch.equal(leaf, exact_mm(x, w, off).to(BF16)) and torch.equal(dleaf, exact_wgrad(dy, x, off).to(F32))

@@ -178,3 +178,14 @@ def test_sizes_beyond_32_bits_are_refused():
             call()
         assert e.value.code == SHAPE
     g._check_sizes("w", 1024, 2 ** 31 - 1, 1)
+
+
+def test_an_output_that_autograd_follows_is_refused():
+    """written over, it would still hand its gradient to what it held before"""
+    leaf = torch.zeros(4, 8, requires_grad=True)
+    for out in (leaf, leaf * 2):
+        with pytest.raises(RuntimeError, match="out requires a gradient"):
+            g._check_out(out)
+        g._check_out(out.detach())
+        with torch.no_grad():
+            g._check_out(out)
