@@ -305,10 +305,11 @@ __global__ void __launch_bounds__(THREADS, GRAD_CTAS_PER_SM)
     const double n = sqrt(total(part, nparts));
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
     const double c = max_norm / (n + 1e-6);
-    // x * coef as (x * c32) * p: below fp32's normal range the coefficient keeps its bits in c32 = c * 2^64 (a norm near
-    // or above fp32's largest value), else p = 1
-    const bool sub = c < 0x1p-100;
-    const Coef coef{(float)(c >= 1.0 ? 1.0 : sub ? c * 0x1p64 : c), sub ? 0x1p-64f : 1.0f};   // a NaN norm gives NaN
+    // x * coef as (x * c32) * p, so that a coefficient below fp32's normal range (a norm near or above fp32's largest value,
+    // or a small max_norm) keeps its bits: c32 = c * 2^64 down to 2^-190, c * 2^149 below (and below 2^-278 every product
+    // rounds to zero), p the other power; else p = 1.  x * c32 stays in range, and normal where the result is not zero
+    const double up = c < 0x1p-190 ? 0x1p149 : c < 0x1p-100 ? 0x1p64 : 1.0;
+    const Coef coef{(float)(c >= 1.0 ? 1.0 : c * up), (float)(1.0 / up)};   // a NaN norm gives NaN
     const bool unchanged = coef.c == 1.0f && coef.p == 1.0f;
     if (unchanged && t.in_place) return;
     const unsigned all = t.first[t.count];

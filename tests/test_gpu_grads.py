@@ -300,3 +300,16 @@ def test_lazily_negated_tensors():
     v = torch.arange(1.0, 6.0, device="cuda").to(torch.cfloat).mul(1j).conj().imag      # with gaps
     (c,), _ = clip_grads([v], 100.0)
     assert c.tolist() == [-1.0, -2.0, -3.0, -4.0, -5.0]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("max_norm", [1e-12, 1e-18, 1e-19, 1e-20, 1e-25, 1e-31, 1e-38, 1e-41, 1e-44, 1e-60, 1e-300, 5e-324])
+@pytest.mark.parametrize("scale", [1.0, 1e30, 3e37])
+def test_small_maximal_norms(scale, max_norm, dtype):
+    """coefficients down to and past those whose products all round to zero (1e-60 / 6e39 is 2^-331)"""
+    ts = [rand((40001,), dtype, 3, scale), rand((70,), dtype, 4, scale)]
+    want = norm64(ts)
+    for out in (None, [torch.empty(t.shape, device="cuda") for t in ts]):
+        ys, _ = clip_grads(ts, max_norm, out=out)
+        for y, t in zip(ys, ts):
+            check_clipped(y, t, coef64(want, max_norm))
