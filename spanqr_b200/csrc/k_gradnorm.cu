@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(THREADS, GRAD_CTAS_PER_SM)
                  float* norm) {
     const double n = sqrt(total(part, nparts));
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
-    const double c = max_norm / (n + 1e-6);
+    const double c = n == INFINITY ? 0.0 : max_norm / (n + 1e-6);   // (zero for an infinite max_norm too)
     // x * coef as (x * c32) * p, so that a coefficient below fp32's normal range (a norm near or above fp32's largest value,
     // or a small max_norm) keeps its bits: c32 = c * 2^64 down to 2^-190, c * 2^149 below (and below 2^-278 every product
     // rounds to zero), p the other power; else p = 1.  x * c32 stays in range, and normal where the result is not zero

@@ -313,3 +313,17 @@ def test_small_maximal_norms(scale, max_norm, dtype):
         ys, _ = clip_grads(ts, max_norm, out=out)
         for y, t in zip(ys, ts):
             check_clipped(y, t, coef64(want, max_norm))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_infinite_gradient_and_infinite_maximal_norm(dtype):
+    """the coefficient of an infinite norm is 0 whatever max_norm is: inf / inf is not left to become NaN everywhere"""
+    x = rand((20000,), dtype, 2)
+    x[12345] = float("-inf")
+    for out in (None, [x.clone()]):
+        ins = [x] if out is None else out
+        (y,), n = clip_grads(ins, float("inf"), out=out)
+        assert n.item() == float("inf") and bool(y[12345].isnan()) and int((y == 0).sum()) == 19999
+    x[777] = float("nan")
+    (y,), n = clip_grads([x], float("inf"))
+    assert n.isnan().item() and bool(y.isnan().all())
