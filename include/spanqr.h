@@ -293,7 +293,9 @@ int spanqr_grad_clip(const void* const* in, const int* in_type, void* const* out
  * Both are deterministic.
  * spanqr_mm_read_status: the word in which these kernels report, on the current device, a bounded device wait that ran
  *   out (0: none since the last read; else SPANQR_ERR_DEVICE, and results since then must not be used).  Clears it and
- *   synchronises `stream`.
+ *   synchronises `stream`.  There is one word per device: it reports the calls of every stream, of those that have ended.
+ * spanqr_mm_selftest_timeout: one pair of CTAs of these kernels' set-up whose waits run out after limit_ns (1 .. 1e8)
+ *   nanoseconds unless `arrive` is non-zero; it reports in the same word, returns, and leaves the context usable.
  */
 int spanqr_mm_grouped_workspace_bytes(int T, int E, int N, int K, int copies, size_t* bytes);
 int spanqr_mm_grouped(const void* x, long long ldx, const void* w, long long ldw, long long stride_w, int w_transposed,
@@ -304,6 +306,7 @@ int spanqr_mm_grouped_wgrad(const void* dy, long long lddy, const void* x, long 
                             int type, int out_type, int T, int E, int N, int K, void* ws, size_t ws_bytes,
                             spanqr_stream_t stream);
 int spanqr_mm_read_status(spanqr_stream_t stream, int* device_status);
+int spanqr_mm_selftest_timeout(long long limit_ns, int arrive, spanqr_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -53,6 +53,7 @@ SIGNATURES = {
     "spanqr_mm_grouped_wgrad_workspace_bytes": (_I, [_I, _I, _I, _I, _I, ctypes.POINTER(_SZ)]),
     "spanqr_mm_grouped_wgrad": (_I, [_P, _LL, _P, _LL, _P, _P, _I, _I, _I, _I, _I, _I, _P, _SZ, _P]),
     "spanqr_mm_read_status": (_I, [_P, ctypes.POINTER(_I)]),
+    "spanqr_mm_selftest_timeout": (_I, [_LL, _I, _P]),
 }
 
 _lib = None

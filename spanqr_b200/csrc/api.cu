@@ -1129,6 +1129,15 @@ int spanqr_mm_grouped_wgrad(const void* dy, long long lddy, const void* x, long 
     return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
 }
 
+int spanqr_mm_selftest_timeout(long long limit_ns, int arrive, spanqr_stream_t stream) {
+    if (limit_ns <= 0 || limit_ns > 100000000LL) return SPANQR_ERR_ARG;
+    int* const status = mm_status();
+    if (!status) return cuda_fail(cudaGetLastError());
+    const cudaError_t e =
+        launch_mm_selftest(arrive != 0, (unsigned long long)limit_ns, status, reinterpret_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? SPANQR_OK : cuda_fail(e);
+}
+
 int spanqr_mm_read_status(spanqr_stream_t stream, int* device_status) {
     if (!device_status) return SPANQR_ERR_ARG;
     int* p = mm_status();

@@ -231,6 +231,8 @@ struct MmWgradArgs {
     bool behind;    // as above
     DType type() const { return bf16 ? DT_BF16 : DT_F16; }
 };
+// one pair whose waits run out after limit_ns (unless `arrive`) and which ORs MM_TIMEOUT into *status
+cudaError_t launch_mm_selftest(int arrive, unsigned long long limit_ns, int* status, cudaStream_t st);
 struct MmWgradPlan {
     int splits;        // runs into which each expert's rows are cut
     int ldp;           // row length of the runs' partial results

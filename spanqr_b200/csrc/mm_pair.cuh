@@ -91,8 +91,10 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+constexpr uint64_t WAIT_NS = 2000000000ull;   // the limit of every wait (only the self-test gives another)
+
 // the bounded wait on a barrier that the other CTA arrives on
-__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, uint64_t limit_ns = 2000000000ull) {
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, uint64_t limit_ns = WAIT_NS) {
     const uint64_t t0 = tc::globaltimer();
     for (;;) {
         uint32_t ok;
@@ -190,20 +192,20 @@ struct Ring {
 
 // the wait for the ring's stage to be free (a barrier's first wait, for the phase before its first, returns at once)
 template <typename C>
-__device__ __forceinline__ bool stage_free(const Pair& p, const Ring<C>& r) {
-    if (!*p.err && tc::mbar_wait(&p.empty[r.s], r.phase ^ 1)) return true;
+__device__ __forceinline__ bool stage_free(const Pair& p, const Ring<C>& r, uint64_t limit_ns = WAIT_NS) {
+    if (!*p.err && tc::mbar_wait(&p.empty[r.s], r.phase ^ 1, limit_ns)) return true;
     *p.err = 1;
     return false;
 }
 // the end of the copies: the products have released every stage (so no signal is on its way to a barrier of a CTA that
 // is gone), or, after a limit ran out, the leader has seen both CTAs' copies arrive
 template <typename C>
-__device__ __forceinline__ void finish_copies(const Pair& p, Ring<C> r) {
+__device__ __forceinline__ void finish_copies(const Pair& p, Ring<C> r, uint64_t limit_ns = WAIT_NS) {
     if (!*p.err) {
         for (int n = 0; n < C::STAGES; ++n, r.next())
-            if (!tc::mbar_wait(&p.empty[r.s], r.phase ^ 1)) *p.err = 1;
+            if (!tc::mbar_wait(&p.empty[r.s], r.phase ^ 1, limit_ns)) *p.err = 1;
     } else if (p.rank == 0) {
-        for (int s = 0; s < C::STAGES; ++s) tc::mbar_wait(&p.full[s], s < r.s ? r.phase : r.phase ^ 1);
+        for (int s = 0; s < C::STAGES; ++s) tc::mbar_wait(&p.full[s], s < r.s ? r.phase : r.phase ^ 1, limit_ns);
     }
 }
 

@@ -4,6 +4,7 @@ layers whose gradients clip_grads and orth_batched then take).
     from spanqr_b200 import mm_grouped, mm_grouped_wgrad
     y = mm_grouped(x, w, offsets)                 # y[t] = w[e(t)] @ x[t], differentiable in x and w
     dw = mm_grouped_wgrad(dy, x, offsets)         # dw[e] = sum over e's rows of dy[t] x[t]^T, fp32: orth's input type
+    mm_check()                                    # raises if a kernel of theirs gave up a wait (synchronises)
 
 x is [T, K] with the rows of expert e at offsets[e - 1] .. offsets[e] (offsets: int32 on the GPU, the cumulative sum of
 the rows per expert), w is [E, N, K], bf16 or fp16.  Everything runs on libspanqr's kernels on the current stream of x's
@@ -281,3 +282,23 @@ def mm_grouped_wgrad(dy, x, offsets, *, out=None, dtype=None):
     if not out.is_inference():
         torch.autograd.graph.increment_version(out)
     return out
+
+
+def mm_check(device=None):
+    """Raises SpanqrError if a kernel of mm_grouped or mm_grouped_wgrad gave up one of its device waits (2 s each) on this
+    device since the last check, whichever stream it ran on; its results, and any after it, must not be used.  The calls
+    themselves cannot say so without waiting: check where a program synchronises anyway, before it keeps what it computed
+    (a step's loss, a checkpoint).  Waits for the device's current stream: other streams' calls are reported once they have
+    ended.  Not inside a capture.  device: an index, a torch.device or its name; the current one by default."""
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError(f"device must be a CUDA device (got {device})")
+    index = torch.cuda.current_device() if device.index is None else device.index
+    with torch.cuda.device(index):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("mm_check waits for the stream, which a capture does not allow")
+        status = _lib.ctypes.c_int(0)
+        rc = _lib.lib().spanqr_mm_read_status(torch._C._cuda_getCurrentRawStream(index), _lib.ctypes.byref(status))
+    if rc:
+        raise _lib.SpanqrError(rc, f"mm_check(cuda:{index}): a product's wait ran out (status 0x{status.value:x})" if
+                               rc == 5 else f"mm_check(cuda:{index})")   # SPANQR_ERR_DEVICE

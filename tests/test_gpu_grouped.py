@@ -11,7 +11,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from spanqr_b200 import _lib, clip_grads, mm_grouped, mm_grouped_wgrad, orth_batched
+from spanqr_b200 import _lib, SpanqrError, clip_grads, mm_check, mm_grouped, mm_grouped_wgrad, orth_batched
 
 pytestmark = pytest.mark.gpu
 BF16, FP16, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -587,3 +587,26 @@ def test_outputs_that_autograd_follows_are_refused():
     with torch.no_grad():
         mm_grouped(x, w, off, out=leaf), mm_grouped_wgrad(dy, x, off, out=dleaf)
     assert torch.equal(leaf, exact_mm(x, w, off).to(BF16)) and torch.equal(dleaf, exact_wgrad(dy, x, off).to(F32))
+
+
+def test_waits_that_run_out_are_reported_and_leave_the_context_usable():
+    """one pair of CTAs whose roles wait for what does not come, each for at most a millisecond"""
+    L, st = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    x, w, dy, off = ints((300, 64), 1, BF16), ints((2, 72, 64), 2, BF16), ints((300, 72), 3, BF16), offsets([115, 185])
+    mm_check()
+    assert L.spanqr_mm_selftest_timeout(100_000_000, 1, st) == 0          # everything arrives
+    mm_check()
+    for device in (None, "cuda", torch.cuda.current_device()):
+        assert L.spanqr_mm_selftest_timeout(1_000_000, 0, st) == 0
+        with pytest.raises(SpanqrError, match="wait ran out .status 0x100"):
+            mm_check(device)
+        mm_check()                                                        # reported once
+        assert torch.equal(mm_grouped(x, w, off), exact_mm(x, w, off).to(BF16))
+        assert torch.equal(mm_grouped_wgrad(dy, x, off), exact_wgrad(dy, x, off).to(F32))
+    other = torch.cuda.Stream()
+    with torch.cuda.stream(other):
+        assert L.spanqr_mm_selftest_timeout(1_000_000, 0, other.cuda_stream) == 0
+    other.synchronize()
+    with pytest.raises(SpanqrError):                                      # a word for the device, not for the stream
+        mm_check()
+    mm_check()

@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from spanqr_b200 import _lib, mm_grouped, mm_grouped_wgrad
+from spanqr_b200 import _lib, mm_check, mm_grouped, mm_grouped_wgrad
 from spanqr_b200 import grouped as g
 
 OK, SHAPE, ARG = 0, 1, 2
@@ -189,3 +189,54 @@ def test_an_output_that_autograd_follows_is_refused():
         g._check_out(out.detach())
         with torch.no_grad():
             g._check_out(out)
+
+
+def test_selftest_argument_checks():
+    for limit in (0, -1, 10 ** 8 + 1):
+        assert _lib.lib().spanqr_mm_selftest_timeout(limit, 0, None) == ARG
+
+
+@pytest.mark.parametrize("device,index", [(None, 1), ("cuda", 1), ("cuda:3", 3), (2, 2), (torch.device("cuda", 0), 0)])
+def test_check_raises_what_the_device_reports(monkeypatch, device, index):
+    """of the device that is asked for, on its current stream; nothing when there is nothing to report"""
+    state = {"current": 1}
+
+    class Device:
+        def __init__(self, i):
+            self.i = i
+
+        def __enter__(self):
+            self.was, state["current"] = state["current"], self.i
+
+        def __exit__(self, *a):
+            state["current"] = self.was
+
+    class Library:
+        rc, word, seen = OK, 0, None
+
+        def spanqr_mm_read_status(self, stream, out):
+            Library.seen = state["current"], stream
+            out._obj.value = self.word
+            return self.rc
+
+        def spanqr_strerror(self, code):
+            return b"device reported a failure"
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: state["current"])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    monkeypatch.setattr(_lib, "lib", Library)
+    assert mm_check(device) is None
+    assert Library.seen == (index, 100 + index) and state["current"] == 1
+    Library.rc, Library.word = 5, 0x100
+    with pytest.raises(_lib.SpanqrError, match=f"cuda:{index}.*wait ran out .status 0x100.*reported a failure") as e:
+        mm_check(device)
+    assert e.value.code == 5 and state["current"] == 1
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="capture"):
+        mm_check(device)
+
+
+def test_check_refuses_other_devices():
+    with pytest.raises(ValueError, match="CUDA device"):
+        mm_check("cpu")
