@@ -167,9 +167,16 @@ __device__ __forceinline__ Pair set_up(char* dyn, const int* offsets, int E, int
     return p;
 }
 
-// no CTA of the pair leaves while the other may still signal its barriers or read its operands
+// No CTA of the pair leaves while the other may still signal its barriers or read its operands.  When all went well the roles
+// have seen every signal and copy by now.  After a wait that ran out they have not: the products' signals to both CTAs and
+// the second CTA's copies may be under way still.  Whoever finds the flag set stays for GRACE_NS, thousands of times what
+// either takes, so that all it issued has landed.
+constexpr uint64_t GRACE_NS = 10000000ull;
+
 template <typename C>
 __device__ __forceinline__ void tear_down(const Pair& p, int* status) {
+    if (*p.err)
+        for (const uint64_t t0 = tc::globaltimer(); tc::globaltimer() - t0 < GRACE_NS;) __nanosleep(1000);
     __syncwarp();
     tc::fence_before_sync();
     cluster_sync_all();

@@ -589,6 +589,21 @@ def test_outputs_that_autograd_follows_are_refused():
     assert torch.equal(leaf, exact_mm(x, w, off).to(BF16)) and torch.equal(dleaf, exact_wgrad(dy, x, off).to(F32))
 
 
+def test_a_pair_whose_waits_ran_out_stays_until_what_it_issued_has_landed():
+    """10 ms, where the waits alone take a few microseconds; nothing stays where all arrived"""
+    L, st = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    a, b, c = (torch.cuda.Event(enable_timing=True) for _ in range(3))
+    assert L.spanqr_mm_selftest_timeout(100_000_000, 1, st) == 0          # (loaded)
+    a.record()
+    assert L.spanqr_mm_selftest_timeout(1_000, 0, st) == 0
+    b.record()
+    assert L.spanqr_mm_selftest_timeout(100_000_000, 1, st) == 0
+    c.record()
+    with pytest.raises(SpanqrError):
+        mm_check()
+    assert 9.9 <= a.elapsed_time(b) < 100 and b.elapsed_time(c) < 5
+
+
 def test_waits_that_run_out_are_reported_and_leave_the_context_usable():
     """one pair of CTAs whose roles wait for what does not come, each for at most a millisecond"""
     L, st = _lib.lib(), torch.cuda.current_stream().cuda_stream
