@@ -293,7 +293,8 @@ int spanqr_grad_clip(const void* const* in, const int* in_type, void* const* out
  * Both are deterministic.
  * spanqr_mm_read_status: the word in which these kernels report, on the current device, a bounded device wait that ran
  *   out (0: none since the last read; else SPANQR_ERR_DEVICE, and results since then must not be used).  Clears it and
- *   synchronises `stream`.  There is one word per device: it reports the calls of every stream, of those that have ended.
+ *   synchronises `stream`.  There is one word per device, read and cleared in one step: it reports the calls
+ *   of every stream, and what a call that is still running reports later is left for the next read.
  * spanqr_mm_selftest_timeout: one pair of CTAs of these kernels' set-up whose waits run out after limit_ns (1 .. 1e8)
  *   nanoseconds unless `arrive` is non-zero; it reports in the same word, returns, and leaves the context usable.
  */

@@ -981,6 +981,11 @@ namespace {
 // the kernels report a bounded wait that ran out here: a word of the library's device image, so that no call has to
 // bring or clear a status word of its own
 __device__ int g_mm_status;
+// what a read takes out of it.  One exchange: a copy and a clearing one after the other lost what a kernel of another
+// stream reported between them
+__device__ int g_mm_taken;
+__global__ void k_mm_take_status() { g_mm_taken = atomicExch(&g_mm_status, 0); }
+std::mutex g_mm_take_mutex;   // (one result word per device)
 
 int* mm_status() {
     void* p = nullptr;
@@ -1140,12 +1145,16 @@ int spanqr_mm_selftest_timeout(long long limit_ns, int arrive, spanqr_stream_t s
 
 int spanqr_mm_read_status(spanqr_stream_t stream, int* device_status) {
     if (!device_status) return SPANQR_ERR_ARG;
-    int* p = mm_status();
-    if (!p) return cuda_fail(cudaGetLastError());
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     int h = 0;
-    cudaError_t e = cudaMemcpyAsync(&h, p, sizeof(int), cudaMemcpyDeviceToHost, st);
-    if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, sizeof(int), st);
+    const std::lock_guard<std::mutex> lock(g_mm_take_mutex);
+    void* taken = nullptr;
+    cudaError_t e = cudaGetSymbolAddress(&taken, g_mm_taken);
+    if (e == cudaSuccess) {
+        k_mm_take_status<<<1, 1, 0, st>>>();
+        e = cudaGetLastError();
+    }
+    if (e == cudaSuccess) e = cudaMemcpyAsync(&h, taken, sizeof(int), cudaMemcpyDeviceToHost, st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
     if (e != cudaSuccess) return cuda_fail(e);
     *device_status = h;

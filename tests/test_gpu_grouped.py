@@ -589,6 +589,21 @@ def test_outputs_that_autograd_follows_are_refused():
     assert torch.equal(leaf, exact_mm(x, w, off).to(BF16)) and torch.equal(dleaf, exact_wgrad(dy, x, off).to(F32))
 
 
+def test_no_report_is_lost_between_two_reads():
+    """a kernel of another stream reports while the word is read: one of the reads, or one after both, has it"""
+    L, status = _lib.lib(), ctypes.c_int(0)
+    mine, other = torch.cuda.current_stream().cuda_stream, torch.cuda.Stream()
+    read = lambda: L.spanqr_mm_read_status(mine, ctypes.byref(status))   # noqa: E731
+    assert read() == 0
+    for i in range(60):
+        assert L.spanqr_mm_selftest_timeout(1_000 + 200 * i, 0, other.cuda_stream) == 0
+        reports = 0
+        while not other.query():
+            reports += read() != 0
+        reports += read() != 0
+        assert reports == 1, i
+
+
 def test_a_pair_whose_waits_ran_out_stays_until_what_it_issued_has_landed():
     """10 ms, where the waits alone take a few microseconds; nothing stays where all arrived"""
     L, st = _lib.lib(), torch.cuda.current_stream().cuda_stream
