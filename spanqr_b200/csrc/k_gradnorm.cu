@@ -218,8 +218,9 @@ __global__ void __launch_bounds__(THREADS, GRAD_CTAS_PER_SM)
     }
 }
 
-// the slots' sum, the same bits in every CTA that takes it
-__device__ double total(const double* __restrict__ part, int nparts) {
+// the slots' sum, the same bits in every CTA that takes it.  (Not __restrict__, here and in the kernels that call this: a
+// kernel that starts before its predecessor's end must not read what that still writes as data that nobody changes.)
+__device__ double total(const double* part, int nparts) {
     __shared__ double red[THREADS / 32];
     double acc = 0.0;
     wait_primary();   // the slots are written
@@ -234,7 +235,7 @@ __device__ double total(const double* __restrict__ part, int nparts) {
     return s;
 }
 
-__global__ void __launch_bounds__(THREADS) k_grad_finish(const double* __restrict__ part, int nparts, double* sumsq_out,
+__global__ void __launch_bounds__(THREADS) k_grad_finish(const double* part, int nparts, double* sumsq_out,
                                                          float* norm) {
     const double s = total(part, nparts);
     if (threadIdx.x == 0) {
@@ -300,8 +301,7 @@ __device__ __forceinline__ void chunk_scale(const GradEntry& e, unsigned local, 
 // one leaves tensors clipped in place unread and unwritten.
 template <int CAP>
 __global__ void __launch_bounds__(THREADS, GRAD_CTAS_PER_SM)
-    k_grad_scale(const __grid_constant__ Table<CAP> t, const double* __restrict__ part, int nparts, double max_norm,
-                 float* norm) {
+    k_grad_scale(const __grid_constant__ Table<CAP> t, const double* part, int nparts, double max_norm, float* norm) {
     const double n = sqrt(total(part, nparts));
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n;
     const double c = n == INFINITY ? 0.0 : max_norm / (n + 1e-6);   // (zero for an infinite max_norm too)

@@ -273,9 +273,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     tear_down<C>(p, a.status);
 }
 
-// the runs' partial results (rows of ldp floats, a multiple of 4), added in order: one thread, four columns of one row
+// the runs' partial results (rows of ldp floats, a multiple of 4), added in order: one thread, four columns of one row.
+// (part is not __restrict__: the kernel before still writes it when this one starts.)
 template <typename OUT>
-__global__ void __launch_bounds__(256) k_mm_wgrad_join(const MmWgradArgs a, const float* __restrict__ part, int ldp) {
+__global__ void __launch_bounds__(256) k_mm_wgrad_join(const MmWgradArgs a, const float* part, int ldp) {
     const int quads = ldp / 4;
     const long long plane = (long long)a.N * ldp, all = (long long)a.E * a.N * quads;
     wait_primary();

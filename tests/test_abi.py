@@ -136,3 +136,19 @@ def test_peer_slab_argument_checks_before_any_device_work():
 def test_error_type_names_the_code():
     with pytest.raises(_lib.SpanqrError, match="unsupported shape"):
         _lib.check(SHAPE, "orth")
+
+
+def test_kernels_that_start_early_do_not_promise_unchanged_data():
+    """a kernel launched before its predecessor's end (it waits in wait_primary, itself or through a function) reads that
+    one's results: its pointers are not __restrict__, which promises that nobody writes them while it runs"""
+    seen = 0
+    for src in sorted((HDR.parent.parent / "spanqr_b200" / "csrc").glob("*.cu")):
+        text = re.sub(r"//[^\n]*|__launch_bounds__\([^)]*\)|__cluster_dims__\([^)]*\)", "", src.read_text())
+        waits = {"wait_primary", "set_up"}
+        for head, name, args, body in re.findall(
+                r"^((?:__device__|__global__)[^;{}()]*?)\b(\w+)\(([^;{}]*?)\)\s*\{\n(.*?)^\}", text, re.M | re.S):
+            if any(re.search(rf"\b{w}(<\w+>)?\(", body) for w in waits):
+                waits.add(name)
+                seen += "__global__" in head
+                assert "__restrict__" not in args, f"{src.name}: {name}"
+    assert seen >= 6
