@@ -115,11 +115,23 @@ def _signs(ins, outs, sizes):
     return ins
 
 
+def _refused(group):
+    """this rank's part in the all-reduce of a call that it is about to raise from: a NaN for its sum.  The other ranks do not
+    wait for it then, and see by their norm that something was wrong"""
+    if group is not None:
+        dev = torch.cuda.current_device() if torch.cuda.is_available() else "cpu"
+        dist.all_reduce(torch.full((), float("nan"), dtype=torch.float64, device=dev), group=group)
+
+
 def _group_sumsq(ts, types, dev, group):
     """the list's sum of squares (fp64), summed over the group's ranks"""
     with torch.cuda.device(dev):
-        sumsq = torch.empty((), dtype=torch.float64, device=dev)
-        _run_norm(ts, types, dev, sumsq, None)
+        try:
+            sumsq = torch.empty((), dtype=torch.float64, device=dev)
+            _run_norm(ts, types, dev, sumsq, None)
+        except Exception:
+            _refused(group)
+            raise
         dist.all_reduce(sumsq, group=group)
     return sumsq
 
@@ -128,10 +140,14 @@ def grad_norm(tensors, *, group=None):
     """The L2 norm over all elements of a list of fp32, fp16 or bf16 CUDA tensors on one device, as a 0-dim fp32 tensor.
     A tensor listed twice counts twice; an empty list gives 0.  With `group` (a torch.distributed process group whose
     ranks each hold their own part of the gradients) the norm is over all ranks' lists, through one 8-byte all-reduce
-    of the sum of squares; every rank of the group must call, with an empty list if it holds nothing.  Without it the
-    norm is of this process's list alone.  Deterministic; large and small values do not overflow or vanish in their
-    squares.  Not differentiable."""
-    ts, types, dev = _check(tensors, "tensors")
+    of the sum of squares; every rank of the group must call, with an empty list if it holds nothing (where one's list is
+    refused the others get NaN).  Without it the norm is of this process's list alone.  Deterministic; large and small
+    values do not overflow or vanish in their squares.  Not differentiable."""
+    try:
+        ts, types, dev = _check(tensors, "tensors")
+    except Exception:
+        _refused(group)
+        raise
     if dev is None:
         dev = torch.cuda.current_device()
     if not all(map(_contiguous, ts)):
@@ -145,16 +161,9 @@ def grad_norm(tensors, *, group=None):
     return norm
 
 
-def clip_grads(tensors, max_norm, *, out=None, group=None):
-    """(clipped, norm): every tensor scaled by min(1, max_norm / (norm + 1e-6)), norm the list's L2 norm before it (as
-    grad_norm gives it; `group` as there).  max_norm is a number >= 0.
-
-    `out`: None for new tensors of the inputs' types, or a list of tensors of the inputs' shapes, each of its input's
-    type or fp32 (so that bf16 gradients reach orth as fp32 in one pass).  An output may be its own input (in place),
-    but overlaps no other tensor of the call.  Outputs must be contiguous, or dense with their input's strides.  An
-    infinite gradient gives the coefficient 0 (finite values become 0, infinite ones NaN) and a NaN makes every output
-    NaN, so a step can be skipped by looking at the norm alone.  A finite norm above fp32's largest value reads as
-    infinity, but the scaling uses its fp64 value.  Autograd does not see the scaling."""
+def _clip_operands(tensors, max_norm, out):
+    """the checked operands of a clipping: max_norm, the inputs as the kernels read them, their types and device, the
+    outputs and their types, and where the norm goes"""
     if torch.is_tensor(max_norm):
         raise TypeError("max_norm must be a number (reading a tensor would wait for the device)")
     max_norm = float(max_norm)
@@ -182,7 +191,24 @@ def clip_grads(tensors, max_norm, *, out=None, group=None):
             ins = [_like_output(i, t, o) for i, (t, o) in enumerate(zip(ts, res))]
     if dev is None:
         dev = torch.cuda.current_device()
-    norm = _norm_like(ts, dev)
+    return max_norm, ins, types, dev, res, out_types, _norm_like(ts, dev)
+
+
+def clip_grads(tensors, max_norm, *, out=None, group=None):
+    """(clipped, norm): every tensor scaled by min(1, max_norm / (norm + 1e-6)), norm the list's L2 norm before it (as
+    grad_norm gives it; `group` as there).  max_norm is a number >= 0.
+
+    `out`: None for new tensors of the inputs' types, or a list of tensors of the inputs' shapes, each of its input's
+    type or fp32 (so that bf16 gradients reach orth as fp32 in one pass).  An output may be its own input (in place),
+    but overlaps no other tensor of the call.  Outputs must be contiguous, or dense with their input's strides.  An
+    infinite gradient gives the coefficient 0 (finite values become 0, infinite ones NaN) and a NaN makes every output
+    NaN, so a step can be skipped by looking at the norm alone.  A finite norm above fp32's largest value reads as
+    infinity, but the scaling uses its fp64 value.  Autograd does not see the scaling."""
+    try:
+        max_norm, ins, types, dev, res, out_types, norm = _clip_operands(tensors, max_norm, out)
+    except Exception:
+        _refused(group)
+        raise
     sumsq = None if group is None else _group_sumsq(ins, types, dev, group)
     _run_clip(ins, types, res, out_types, dev, max_norm, sumsq, norm)
     if out is not None and res:

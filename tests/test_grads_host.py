@@ -144,3 +144,86 @@ def test_lazily_negated_tensors_keep_their_sign():
     assert _signs([z], [z], array("q", [1]))[0] is z             # in place: scaled as it lies
     with pytest.raises(ValueError, match=r"out\[0\] is a lazily negated"):
         _signs([plain], [z], array("q", [1]))
+
+
+# ---- group=: gloo ranks on CPU, the library's two entry points replaced by the formulas over the same pointers ----
+
+def _fake_library(monkeypatch):
+    """grads on CPU tensors of fp32: what it hands to the library is read from and written to their memory"""
+    import contextlib
+
+    import numpy as np
+    from spanqr_b200 import grads
+    real = _lib.lib()
+
+    def view(address, ctype, n):
+        return np.frombuffer((ctype * n).from_address(address), dtype=ctype) if n else np.zeros(0)
+
+    def launch(index, fn, what, *args):
+        clip = fn == real.spanqr_grad_clip
+        ptrs, types, *rest = args
+        if clip:
+            outs, out_types, sizes, count, max_norm, sumsq, norm, ws, _ = rest
+        else:
+            sizes, count, sumsq, norm, ws, _ = rest
+        assert ws and (not count or set(view(types, ctypes.c_int32, count)) == {0})
+        ns = view(sizes, ctypes.c_longlong, count)
+        ins = [view(int(p), ctypes.c_float, int(n)) for p, n in zip(view(ptrs, ctypes.c_ulonglong, count), ns)]
+        total = sum(float((x.astype(np.float64) ** 2).sum()) for x in ins)
+        if clip:
+            if sumsq:
+                total = float(view(sumsq, ctypes.c_double, 1)[0])
+            c = min(1.0, max_norm / (total ** 0.5 + 1e-6)) if total == total else total
+            for x, p, n in zip(ins, view(outs, ctypes.c_ulonglong, count), ns):
+                view(int(p), ctypes.c_float, int(n))[:] = x * c
+        elif sumsq:
+            view(sumsq, ctypes.c_double, 1)[0] = total
+        if norm:
+            view(norm, ctypes.c_float, 1)[0] = total ** 0.5
+    monkeypatch.setattr(_lib, "launch", launch)
+    monkeypatch.setattr(grads, "_device", lambda t: torch.device("cpu"))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: torch.device("cpu"))
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+
+
+def _rank(rank, port, work):
+    from datetime import timedelta
+
+    import torch.distributed as dist
+    dist.init_process_group("gloo", init_method=f"tcp://127.0.0.1:{port}", rank=rank, world_size=3,
+                            timeout=timedelta(seconds=20))
+    try:
+        with pytest.MonkeyPatch.context() as m:
+            _fake_library(m)
+            work(rank, dist)
+    finally:
+        dist.destroy_process_group()
+
+
+def _ranks(work):
+    import socket
+
+    import torch.multiprocessing as mp
+    with socket.socket() as free:
+        free.bind(("127.0.0.1", 0))
+        port = free.getsockname()[1]
+    mp.spawn(_rank, args=(port, work), nprocs=3, join=True)
+
+
+def _refusals_of_one_rank(rank, dist):
+    world = dist.group.WORLD
+    good, bad = [torch.tensor([3.0, 4.0])], [torch.zeros(4, dtype=torch.float64)]
+    for call, error in ((lambda ts: grad_norm(ts, group=world), TypeError),
+                        (lambda ts: clip_grads(ts, 1.0, group=world)[1], TypeError),
+                        (lambda ts: clip_grads(ts, 1.0, out=good + bad if ts is bad else None, group=world)[1], TypeError),
+                        (lambda ts: clip_grads(good, -1.0 if ts is bad else 1.0, group=world)[1], ValueError)):
+        if rank == 1:
+            with pytest.raises(error):
+                call(bad)
+        else:
+            assert call(good).isnan().item()
+        assert abs(grad_norm(good, group=world).item() - 75 ** 0.5) < 1e-5       # the next call of all ranks is right
+
+
+def test_a_rank_whose_list_is_refused_leaves_no_other_waiting():
+    _ranks(_refusals_of_one_rank)
