@@ -327,3 +327,29 @@ def test_infinite_gradient_and_infinite_maximal_norm(dtype):
     x[777] = float("nan")
     (y,), n = clip_grads([x], float("inf"))
     assert n.isnan().item() and bool(y.isnan().all())
+
+
+def test_a_group_adds_the_sums_of_squares_in_fp64(monkeypatch):
+    """another rank's part, added where the all-reduce would: to the fp64 sum of squares on the tensors' device, once per call"""
+    import torch.distributed as dist
+    ts, other, group, seen = mixed(11), rand((5001,), F32, 12, 3.0), object(), []
+
+    def all_reduce(t, op=None, group=None):
+        assert t.dtype == torch.float64 and t.dim() == 0 and t.is_cuda
+        seen.append(group)
+        t += other.double().square().sum()
+    monkeypatch.setattr(dist, "all_reduce", all_reduce)
+    both, alone = norm64(ts + [other]), norm64([other])
+    check_norm(grad_norm(ts, group=group), both)
+    check_norm(grad_norm([], group=group), alone)
+    for out in (None, [torch.empty(t.shape, device="cuda") for t in ts]):
+        ys, n = clip_grads(ts, 1.0, out=out, group=group)
+        check_norm(n, both)
+        for y, x in zip(ys, ts):
+            check_clipped(y, x, coef64(both, 1.0))
+    _, n = clip_grads([], 1.0, group=group)
+    check_norm(n, alone)
+    assert seen == [group] * 5
+    with pytest.raises(TypeError):
+        grad_norm([other.double()], group=group)
+    assert len(seen) == 6                                 # a refused list takes part too

@@ -227,3 +227,27 @@ def _refusals_of_one_rank(rank, dist):
 
 def test_a_rank_whose_list_is_refused_leaves_no_other_waiting():
     _ranks(_refusals_of_one_rank)
+
+
+def _norms_of_all_ranks(rank, dist):
+    """rank 0 holds two tensors, rank 1 nothing, rank 2 one: 9 + 16 + 144 = 13 squared"""
+    world = dist.group.WORLD
+    part = [[torch.tensor([3.0]), torch.tensor([[0.0, 4.0]])], [], [torch.tensor([12.0])]][rank]
+    for _ in range(2):
+        assert grad_norm(part, group=world).item() == 13.0
+        own = sum(float((t ** 2).sum()) for t in part) ** 0.5
+        assert abs(grad_norm(part).item() - own) < 1e-6              # without the group: this process's own
+        ys, n = clip_grads(part, 6.5, group=world)
+        assert n.item() == 13.0 and len(ys) == len(part)
+        for y, t in zip(ys, part):
+            assert torch.allclose(y, t / 2, rtol=1e-6, atol=0)
+    pair = dist.new_group([0, 2])                                    # (every rank makes it)
+    if rank != 1:
+        assert grad_norm(part, group=pair).item() == 13.0
+        mine = [t.clone() for t in part]
+        _, n = clip_grads(mine, 1.3, out=mine, group=pair)
+        assert n.item() == 13.0 and all(torch.allclose(y, t / 10, rtol=1e-6, atol=0) for y, t in zip(mine, part))
+
+
+def test_norm_and_clipping_over_ranks():
+    _ranks(_norms_of_all_ranks)
