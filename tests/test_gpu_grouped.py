@@ -117,6 +117,22 @@ def test_few_tiles_split_over_the_rows(T, E, N, K, dtype):
         assert torch.equal(mm_grouped_wgrad(dy, x, off, dtype=dtype), exact_wgrad(dy, x, off).to(dtype))
 
 
+@pytest.mark.parametrize("N,K", [(2048, 2048), (2048, 1999), (2040, 2056)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_wgrad_in_16_bits_over_several_drains(N, K, dtype):
+    """experts of more rows than are summed in one accumulator (2048), too many tiles to split the rows: the accumulators are
+    taken in turn several times within a tile, at whole and ragged ends, and stored in both ways"""
+    counts = [7001, 2049, 0, 4101, 2048, 4096]
+    T, off = sum(counts), offsets(counts)
+    dy, x = ints((T, N), 1, dtype), ints((T, K), 2, dtype)
+    want = exact_wgrad(dy, x, off).to(dtype)
+    assert torch.equal(mm_grouped_wgrad(dy, x, off, dtype=dtype), want)
+    assert torch.equal(mm_grouped_wgrad(dy, x, off), exact_wgrad(dy, x, off).to(F32))
+    w = ints((len(counts), N, K), 3, dtype).requires_grad_()
+    dw, = torch.autograd.grad(mm_grouped(x, w, off), w, dy)
+    assert torch.equal(dw, want)
+
+
 @pytest.mark.parametrize("T,E,N,K", [(24, 8, 512, 2048), (700, 16, 384, 1024), (3000, 4, 640, 4096), (5000, 3, 256, 17408)])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 def test_product_gaussian(T, E, N, K, dtype):
