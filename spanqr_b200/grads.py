@@ -10,6 +10,7 @@ Both run on libspanqr's kernels on the current stream of the tensors' device, wi
 workspace comes from torch's allocator per call, so calls on different streams and captured graphs never share one.
 """
 from array import array
+from itertools import compress
 from operator import attrgetter
 
 import torch
@@ -21,6 +22,7 @@ from . import _lib
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _dtype, _same_size = attrgetter("dtype"), torch.Tensor.is_same_size
 _contiguous = torch.Tensor.is_contiguous
+_neg = torch.Tensor.is_neg
 _PLAIN = {torch.Tensor, torch.nn.Parameter}
 _ptr, _numel, _device = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device
 
@@ -87,9 +89,10 @@ def _run_norm(ts, types, dev, sumsq, norm):
 
 def _run_clip(ins, in_types, outs, out_types, dev, max_norm, sumsq, norm):
     ws = _workspace(norm, len(ins))
-    sizes = array("q", map(_numel, ins))
-    ins = _signs(ins, outs, sizes)
-    pi, po = array("Q", map(_ptr, ins)), array("Q", map(_ptr, outs))
+    sizes = list(map(_numel, ins))
+    if 1 in sizes:
+        ins = _signs(ins, outs, sizes)
+    pi, po, sizes = array("Q", map(_ptr, ins)), array("Q", map(_ptr, outs)), array("q", sizes)
     try:
         _lib.launch(dev, _lib.lib().spanqr_grad_clip, lambda: f"clip_grads({len(ins)} tensors)", _at(pi), _at(in_types),
                     _at(po), _at(out_types), _at(sizes), len(ins), max_norm, None if sumsq is None else sumsq.data_ptr(),
@@ -103,10 +106,11 @@ def _run_clip(ins, in_types, outs, out_types, dev, max_norm, sumsq, norm):
 def _signs(ins, outs, sizes):
     """ins, with a lazily negated one-element tensor resolved where its output is not one too (two such are scaled as
     they lie).  `z.conj().imag` is such a view; of more elements it has gaps, so that it was copied and resolved already."""
-    if 1 not in sizes:
+    ones = [n == 1 for n in sizes]
+    if not (any(map(_neg, compress(ins, ones))) or any(map(_neg, compress(outs, ones)))):
         return ins
     ins = list(ins)
-    for i in [i for i, n in enumerate(sizes) if n == 1]:
+    for i in compress(range(len(ins)), ones):
         neg = outs[i].is_neg()
         if ins[i].is_neg() != neg:
             if neg:

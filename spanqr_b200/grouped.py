@@ -91,7 +91,7 @@ def _side_by_side(a, b):
 def _check_out(out, **others):
     """refuses an output that cannot be written as it lies: one that autograd follows (its gradient would go to what it held
     before), negated lazily, or over one of the other tensors"""
-    if _tracked(out):
+    if _tracked(out, out):
         raise RuntimeError("out requires a gradient, and its values would come from outside autograd: give out.detach(), or "
                            "use torch.no_grad()")
     if out.is_neg():
@@ -166,13 +166,13 @@ def _wgrad(rows_dy, rows_x, offsets, T, E, N, K, dtype, out=None):
     return dw
 
 
-def _tracked(*tensors):
-    """whether autograd follows any of them: backward, or forward with a tangent (make_dual)"""
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors) or _dual(*tensors)
+def _tracked(x, w):
+    """whether autograd follows either of them: backward, or forward with a tangent (make_dual)"""
+    return torch.is_grad_enabled() and (x.requires_grad or w.requires_grad) or _dual(x, w)
 
 
-def _dual(*tensors):
-    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+def _dual(x, w):
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (x, w))
 
 
 def _backward(ctx, dy):
