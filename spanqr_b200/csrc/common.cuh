@@ -63,6 +63,27 @@ __device__ __forceinline__ void cluster_sync_all() {
 
 __host__ __device__ __forceinline__ int cdiv(int a, int b) { return (a + b - 1) / b; }
 
+// programmatic launch: the next kernel's CTAs may start (they wait for this grid's end before they touch its results);
+// the wait is over at once in a kernel that was launched otherwise
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// a launch that may begin before the stream's last kernel has ended (programmatic launch)
+template <typename... P, typename... A>
+cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st, const A&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Float-float accumulation (Knuth's two-sum; the square's rounding error from a fused multiply-add): a sum kept as
 // hi + lo in two fp32 registers, about 44 significant bits, at the full fp32 rate.  B200 converts fp32 to fp64 at
 // about a tenth of its fp64 add rate, so sums of fp32 terms that need more than fp32 accuracy are kept this way and

@@ -30,24 +30,6 @@ constexpr int THREADS = 256;
 constexpr int UNROLL = 4;                              // 32-byte vectors in flight per thread
 constexpr int CHUNK = THREADS * UNROLL * 32;           // bytes of input per chunk (32 KB)
 
-// programmatic launch: the kernel that adds the slots starts while the last chunks are read, and waits for their end
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-template <typename... P, typename... A>
-cudaError_t launch_behind(void (*kernel)(P...), int grid, cudaStream_t st, const A&... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(THREADS);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <int CAP>
 struct Table {
     GradEntry e[CAP];
@@ -197,7 +179,7 @@ __global__ void __launch_bounds__(THREADS, GRAD_CTAS_PER_SM)
     k_grad_sumsq(const __grid_constant__ Table<CAP> t, double* __restrict__ part) {
     double acc = 0.0;
     const unsigned all = t.first[t.count];
-    launch_dependents();
+    launch_dependents();   // the kernel that adds the slots starts while the last chunks are read
     for (unsigned c = blockIdx.x; c < all; c += gridDim.x) {
         const int i = tensor_of(t, c);
         const GradEntry& e = t.e[i];
@@ -366,7 +348,7 @@ cudaError_t scale_launch(const GradEntry* e, int count, int nsm, const double* p
                          float* norm, bool behind, cudaStream_t st) {
     Table<CAP> t;
     const int grid = grid_for(fill(t, e, count), nsm);
-    if (behind) return launch_behind(k_grad_scale<CAP>, grid, st, t, part, nparts, max_norm, norm);
+    if (behind) return launch_behind(k_grad_scale<CAP>, dim3(grid), THREADS, 0, st, t, part, nparts, max_norm, norm);
     k_grad_scale<CAP><<<grid, THREADS, 0, st>>>(t, part, nparts, max_norm, norm);
     return cudaGetLastError();
 }
@@ -386,7 +368,7 @@ cudaError_t launch_grad_sumsq(const GradEntry* e, int count, double* part, int* 
 }
 
 cudaError_t launch_grad_finish(const double* part, int nparts, double* sumsq, float* norm, bool behind, cudaStream_t st) {
-    if (behind) return launch_behind(k_grad_finish, 1, st, part, nparts, sumsq, norm);
+    if (behind) return launch_behind(k_grad_finish, dim3(1), THREADS, 0, st, part, nparts, sumsq, norm);
     k_grad_finish<<<1, THREADS, 0, st>>>(part, nparts, sumsq, norm);
     return cudaGetLastError();
 }

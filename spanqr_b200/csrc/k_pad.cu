@@ -3,12 +3,10 @@
 // four or five aligned 4-byte words of the source that hold them (rows of odd length start at every even address); a word
 // is read only if it holds an element of the row.  1537 rows and 24 experts of 1001x1111, 57 MB each way: 28 us, where a
 // copy of as much takes 27.
-#include "mm.cuh"
+#include "kernels.h"
 
 namespace spq {
 namespace {
-
-using mm::launch_dependents;
 
 // `lanes` threads (a power of two up to a warp) copy one row, then the one `groups` rows on: the plane is carried along,
 // because 64-bit divisions for every 16 bytes took longer than the copy

@@ -73,11 +73,6 @@ __device__ __forceinline__ uint32_t mapa(uint32_t saddr, uint32_t rank) {
     return r;
 }
 
-// programmatic launch: the next kernel's CTAs may start (they wait for this grid's end before they touch its results);
-// the wait is over at once in a kernel that was launched otherwise
-__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // ---- 16-bit results ----
 __device__ __forceinline__ uint16_t to16(float x, bool bf16) {
     return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(x)) : __half_as_ushort(__float2half_rn(x));

@@ -231,22 +231,6 @@ __host__ __device__ __forceinline__ long long run_begin(long long total, int run
     return i < runs ? total * i / runs : total;
 }
 
-// a launch that may begin before the stream's last kernel has ended (programmatic launch)
-template <typename... P, typename... A>
-cudaError_t launch_behind(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st, const A&... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 // a pair kernel's launch (behind: the copies of its operands precede it)
 template <typename C, auto kernel, typename... A>
 cudaError_t launch_pairs(int pairs, int E, bool behind, cudaStream_t st, const A&... args) {
