@@ -290,7 +290,7 @@ int spanqr_grad_clip(const void* const* in, const int* in_type, void* const* out
  * The workspaces, 256-byte aligned, need no initialisation; calls in flight at the same time need different ones.  Their
  *   sizes (often 0, then ws may be NULL) come from the _workspace_bytes of the same sizes, where `copies` says which
  *   operands have to be copied: 1 the first, 2 the second (plus 4 if the weights are transposed).
- * Both are deterministic.
+ * Both are deterministic: the same sizes and offsets give the same bits on the same kind of device.
  * spanqr_mm_read_status: the word in which these kernels report, on the current device, a bounded device wait that ran
  *   out (0: none since the last read; else SPANQR_ERR_DEVICE, and results since then must not be used).  Clears it and
  *   synchronises `stream`.  There is one word per device, read and cleared in one step: it reports the calls

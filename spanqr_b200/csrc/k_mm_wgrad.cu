@@ -1,10 +1,12 @@
 // dw[e] = sum over expert e's rows of dy[t] x[t]^T (no reference counterpart): D = dy^T x in tiles of 256 features x 256
 // columns of x, on pairs of SMs (mm_pair.cuh).  Both operands are read as they lie, row by row (MN-major), in stages of 64
 // rows.  Where the tiles are fewer than the pairs, each expert's rows are cut into `splits` runs of whole stages with a
-// partial result each, and a second kernel adds those in order: the bits depend on the sizes alone.
+// partial result each, and a second kernel adds those in order: the bits depend on the sizes, the offsets and the device's
+// number of SMs, from one call to the next they are the same.
 //
-// Measured (inputs out of the caches): 32768 rows, 8 experts of 5120x2048, fp32 results: 463 us (1485 TFLOP/s), bf16 results
-// 422 us (1629); 8191 rows, 32 experts of 768x512, fp32 results (50 MB, a fill of which takes 21 us): 32 us.
+// Measured (inputs out of the caches): 32768 rows, 8 experts of 5120x2048, rows split evenly, fp16 to fp32: 527 us (1304
+// TFLOP/s), to fp16 553 us; in a row, under the power limit, 556 and 544 us; 8191 rows, 32 experts of 768x512, bf16 to fp32
+// (50 MB, a fill of which takes 21 us): 40 us evenly, 44 us with 18 to 1505 rows each.
 #include "mm_pair.cuh"
 
 namespace spq {

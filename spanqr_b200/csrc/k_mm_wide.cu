@@ -7,9 +7,10 @@
 // the weights are in flight and the more pairs have work.  Where even tiles of 32 rows leave pairs idle, the stages of the
 // contracted dimension are split evenly over the pairs and joined by a second kernel.
 //
-// Measured (bf16, inputs out of the caches): 16384 rows, 8 experts of 5120x2048: 209 us (1645 TFLOP/s, 0.98 of cuBLAS's
-// burst rate); 1024 rows, 128 experts of 1024x1024: 49 us (5.6 TB/s); 64 rows, 8 experts of 5120x2048: 34 us (5.0 TB/s);
-// one row and next to no work: 5 us.
+// Measured (bf16, inputs out of the caches, rows split evenly): 16384 rows, 8 experts of 5120x2048: 222 us (1546 TFLOP/s;
+// cuBLAS with one matrix at this size, in the same run: 217 us); the same rows unevenly (997 to 4092 each): 268 us; 1024
+// rows, 128 experts of 1024x1024: 49 us (5.6 TB/s); 64 rows, 8 experts of 5120x2048: 35 us (4.8 TB/s); one row and next to
+// no work: 5 us.
 #include "mm_pair.cuh"
 
 namespace spq {
@@ -276,7 +277,8 @@ MmPlan mm_plan(int T, int E, int N, int K, int nsm) {
     // the partial sums and the second kernel cost 6.5 us.  Measured (us whole / split, bf16): 8 rows and one matrix of
     // 256x8192 (one tile of 128 stages): 26 / 15; 256x4096: 16 / 11; 256x2048: 10 / 10; 2048x6144 (8 of 96): 21 / 16;
     // 4096x4096 (16 of 64): 16 / 17; 6144x6144 (24 of 96): 21 / 23; 256 rows and 768x17408 (24 tiles of 272 stages over the
-    // weights of 3): 50 / 29; 16 rows, 16 experts of 1024x2048 (40 of 32): 14 / 19.
+    // weights of 3): 50 / 29; 16 rows over 16 experts of 1024x2048 (4 tiles of 32 for each expert that has rows, some ten of
+    // them): 14 / 19.
     const long long kb = (K + BK - 1) / BK, first = ntn * some, all = tiles(32);
     p.split = p.nt == 32 && kb * (10 * pairs - (12 * all > 30 * first ? 12 * all : 30 * first)) > 400LL * pairs;
     const long long most = ntn * (T / p.nt + some);

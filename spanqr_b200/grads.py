@@ -105,7 +105,9 @@ def _run_clip(ins, in_types, outs, out_types, dev, max_norm, sumsq, norm):
 
 def _signs(ins, outs, sizes):
     """ins, with a lazily negated one-element tensor resolved where its output is not one too (two such are scaled as
-    they lie).  `z.conj().imag` is such a view; of more elements it has gaps, so that it was copied and resolved already."""
+    they lie).  `z.conj().imag` is such a view; of more elements it has gaps, so that it was copied and resolved already.
+    Only as_strided makes longer ones without gaps, and a look at every tensor of a list of hundreds would cost a fifth of
+    the call."""
     ones = [n == 1 for n in sizes]
     if not (any(map(_neg, compress(ins, ones))) or any(map(_neg, compress(outs, ones)))):
         return ins
@@ -207,7 +209,9 @@ def clip_grads(tensors, max_norm, *, out=None, group=None):
     but overlaps no other tensor of the call.  Outputs must be contiguous, or dense with their input's strides.  An
     infinite gradient gives the coefficient 0 (finite values become 0, infinite ones NaN) and a NaN makes every output
     NaN, so a step can be skipped by looking at the norm alone.  A finite norm above fp32's largest value reads as
-    infinity, but the scaling uses its fp64 value.  Autograd does not see the scaling."""
+    infinity, but the scaling uses its fp64 value.  Autograd does not see the scaling.  Lazily negated inputs (z.conj().imag)
+    are resolved, and such outputs refused unless their input is one too; but what as_strided lays without gaps over one is
+    taken as its memory lies: call resolve_neg() first."""
     try:
         max_norm, ins, types, dev, res, out_types, norm = _clip_operands(tensors, max_norm, out)
     except Exception:
