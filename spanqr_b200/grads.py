@@ -37,8 +37,9 @@ def _dense(t):
     return True
 
 
-def _check(tensors, name):
-    """the list as a list, its types and its device's index (None when empty)"""
+def _check(tensors, name, like=None):
+    """the list as a list, its types, its device's index (None when empty) and its dtypes; like: types and dtypes of another
+    list, whose types are these where the dtypes are"""
     if torch.is_tensor(tensors):
         raise TypeError(f"{name} must be a list of tensors (got one tensor)")
     ts = list(tensors)
@@ -53,8 +54,11 @@ def _check(tensors, name):
         raise TypeError(f"{name} must be CUDA tensors")
     if len(devs) > 1:
         raise ValueError(f"{name} must be on one device (got cuda:{', cuda:'.join(map(str, sorted(devs)))})")
-    types = array("i", [DTYPES[kinds.pop()]]) * len(ts) if len(kinds) == 1 else array("i", map(DTYPES.get, dtypes))
-    return ts, types, devs.pop() if devs else None
+    if like is not None and dtypes == like[1]:
+        types = like[0]
+    else:
+        types = array("i", [DTYPES[kinds.pop()]]) * len(ts) if len(kinds) == 1 else array("i", map(DTYPES.get, dtypes))
+    return ts, types, devs.pop() if devs else None, dtypes
 
 
 def _at(a):
@@ -89,10 +93,7 @@ def _run_norm(ts, types, dev, sumsq, norm):
 
 def _run_clip(ins, in_types, outs, out_types, dev, max_norm, sumsq, norm):
     ws = _workspace(norm, len(ins))
-    sizes = list(map(_numel, ins))
-    if 1 in sizes:
-        ins = _signs(ins, outs, sizes)
-    pi, po, sizes = array("Q", map(_ptr, ins)), array("Q", map(_ptr, outs)), array("q", sizes)
+    pi, po, sizes = array("Q", map(_ptr, ins)), array("Q", map(_ptr, outs)), array("q", map(_numel, ins))
     try:
         _lib.launch(dev, _lib.lib().spanqr_grad_clip, lambda: f"clip_grads({len(ins)} tensors)", _at(pi), _at(in_types),
                     _at(po), _at(out_types), _at(sizes), len(ins), max_norm, None if sumsq is None else sumsq.data_ptr(),
@@ -103,21 +104,25 @@ def _run_clip(ins, in_types, outs, out_types, dev, max_norm, sumsq, norm):
         raise ValueError("clip_grads: an output overlaps another tensor of the call (one tensor listed twice?)") from None
 
 
-def _signs(ins, outs, sizes):
-    """ins, with a lazily negated one-element tensor resolved where its output is not one too (two such are scaled as
-    they lie).  `z.conj().imag` is such a view; of more elements it has gaps, so that it was copied and resolved already.
-    Only as_strided makes longer ones without gaps, and a look at every tensor of a list of hundreds would cost a fifth of
-    the call."""
-    ones = [n == 1 for n in sizes]
-    if not (any(map(_neg, compress(ins, ones))) or any(map(_neg, compress(outs, ones)))):
+def _any_negated(ts, types):
+    """whether a tensor's memory holds its values negated, as that of z.conj().imag does (no bf16 one can: there is no complex
+    type of such parts)"""
+    bf16 = types.count(2)   # SPANQR_BF16
+    if bf16 == 0:
+        return True in map(_neg, ts)
+    return bf16 < len(ts) and True in map(_neg, compress(ts, [t != 2 for t in types]))
+
+
+def _signs(ins, in_types, outs, out_types):
+    """ins, with those resolved that are negated lazily where their output is not (two such are scaled as they lie)"""
+    if not (_any_negated(ins, in_types) or _any_negated(outs, out_types)):
         return ins
     ins = list(ins)
-    for i in compress(range(len(ins)), ones):
-        neg = outs[i].is_neg()
-        if ins[i].is_neg() != neg:
-            if neg:
+    for i, (t, o) in enumerate(zip(ins, outs)):
+        if t.is_neg() != o.is_neg():
+            if o.is_neg():
                 raise ValueError(f"out[{i}] is a lazily negated view and its input is not: give a tensor of its own")
-            ins[i] = ins[i].resolve_neg()
+            ins[i] = t.resolve_neg()
     return ins
 
 
@@ -150,7 +155,7 @@ def grad_norm(tensors, *, group=None):
     refused the others get NaN).  Without it the norm is of this process's list alone.  Deterministic; large and small
     values do not overflow or vanish in their squares.  Not differentiable."""
     try:
-        ts, types, dev = _check(tensors, "tensors")
+        ts, types, dev, _ = _check(tensors, "tensors")
     except Exception:
         _refused(group)
         raise
@@ -175,12 +180,12 @@ def _clip_operands(tensors, max_norm, out):
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must be a number >= 0 (got {max_norm})")
-    ts, types, dev = _check(tensors, "tensors")
+    ts, types, dev, dtypes = _check(tensors, "tensors")
     if out is None:
         ins = ts if all(map(_contiguous, ts)) else [t.contiguous() for t in ts]
         res, out_types = [torch.empty_like(t, requires_grad=False) for t in ins], types
     else:
-        res, out_types, odev = _check(out, "out")
+        res, out_types, odev, _ = _check(out, "out", (types, dtypes))
         if len(res) != len(ts):
             raise ValueError(f"out must hold {len(ts)} tensors (got {len(res)})")
         if odev != dev:
@@ -188,13 +193,15 @@ def _clip_operands(tensors, max_norm, out):
         if not all(map(_same_size, ts, res)):
             i = next(i for i, (t, o) in enumerate(zip(ts, res)) if t.shape != o.shape)
             raise ValueError(f"out[{i}] has shape {tuple(res[i].shape)}, its input {tuple(ts[i].shape)}")
-        if out_types != types:
+        if out_types is not types:
             for i, (t, o) in enumerate(zip(ts, res)):
                 if o.dtype != t.dtype and o.dtype != torch.float32:
                     raise TypeError(f"out[{i}] must be {t.dtype} or fp32 (got {o.dtype})")
         ins = ts
         if not (all(map(_contiguous, ts)) and all(map(_contiguous, res))):
             ins = [_like_output(i, t, o) for i, (t, o) in enumerate(zip(ts, res))]
+    if out is not tensors:
+        ins = _signs(ins, types, res, out_types)
     if dev is None:
         dev = torch.cuda.current_device()
     return max_norm, ins, types, dev, res, out_types, _norm_like(ts, dev)
@@ -210,8 +217,7 @@ def clip_grads(tensors, max_norm, *, out=None, group=None):
     infinite gradient gives the coefficient 0 (finite values become 0, infinite ones NaN) and a NaN makes every output
     NaN, so a step can be skipped by looking at the norm alone.  A finite norm above fp32's largest value reads as
     infinity, but the scaling uses its fp64 value.  Autograd does not see the scaling.  Lazily negated inputs (z.conj().imag)
-    are resolved, and such outputs refused unless their input is one too; but what as_strided lays without gaps over one is
-    taken as its memory lies: call resolve_neg() first."""
+    are resolved, and such outputs refused unless their input is one too."""
     try:
         max_norm, ins, types, dev, res, out_types, norm = _clip_operands(tensors, max_norm, out)
     except Exception:

@@ -353,3 +353,25 @@ def test_a_group_adds_the_sums_of_squares_in_fp64(monkeypatch):
     with pytest.raises(TypeError):
         grad_norm([other.double()], group=group)
     assert len(seen) == 6                                 # a refused list takes part too
+
+
+def test_lazily_negated_tensors_of_any_length():
+    """as_strided lays a view without gaps over the memory of a conjugate's imaginary part"""
+    for dtype, part in ((torch.complex64, F32), (torch.complex32, F16)):
+        z = torch.zeros(3000, dtype=dtype, device="cuda")
+        z.imag.copy_(rand((3000,), part, 1)), z.real.copy_(rand((3000,), part, 2))
+        x = z.conj().imag.as_strided((5999,), (1,), 1)
+        assert x.dtype == part and x.is_neg() and x.is_contiguous()
+        c = coef64(norm64([x]), 2.0)
+        (y,), n = clip_grads([x], 2.0)
+        check_norm(n, norm64([x]))
+        check_clipped(y, x, c)
+        wide = [torch.empty(5999, device="cuda"), torch.empty(7, device="cuda")]
+        ones = torch.ones(7, device="cuda")
+        clip_grads([x, ones], 2.0, out=wide)
+        check_clipped(wide[0], x, coef64(norm64([x, ones]), 2.0))
+        want = x.clone()
+        clip_grads([x], 2.0, out=[x])
+        check_clipped(x, want, c)
+        with pytest.raises(ValueError, match="lazily negated"):
+            clip_grads([y], 1.0, out=[x])

@@ -138,12 +138,18 @@ def test_lazily_negated_tensors_keep_their_sign():
     z = torch.tensor([3.0 + 4.0j]).conj().imag
     plain, two = torch.tensor([7.0]), torch.zeros(2)
     assert z.is_neg() and z.is_contiguous() and z.item() == -4.0
-    ins = [two, z, plain]
-    got = _signs(ins, [torch.empty_like(t) for t in ins], array("q", [2, 1, 1]))
+    strided = torch.tensor([1.0 + 2.0j, 3.0 + 4.0j]).conj().imag.as_strided((3,), (1,), 1)    # without gaps, of any length
+    assert strided.is_neg() and strided.is_contiguous() and strided.tolist() == [-2.0, -3.0, -4.0]
+    ins, types = [two, z, plain, strided], array("i", [0] * 4)
+    got = _signs(ins, types, [torch.empty_like(t) for t in ins], types)
     assert not got[1].is_neg() and got[1].item() == -4.0 and got[0] is two and got[2] is plain and ins[1] is z
-    assert _signs([z], [z], array("q", [1]))[0] is z             # in place: scaled as it lies
+    assert not got[3].is_neg() and got[3].tolist() == [-2.0, -3.0, -4.0]
+    one = types[:1]
+    assert _signs([z], one, [z], one)[0] is z                    # two of them: scaled as they lie
     with pytest.raises(ValueError, match=r"out\[0\] is a lazily negated"):
-        _signs([plain], [z], array("q", [1]))
+        _signs([plain], one, [z], one)
+    with pytest.raises(ValueError, match=r"out\[1\] is a lazily negated"):
+        _signs([two.bfloat16(), two.bfloat16()], array("i", [2, 2]), [two, strided], types[:2])
 
 
 # ---- group=: gloo ranks on CPU, the library's two entry points replaced by the formulas over the same pointers ----
