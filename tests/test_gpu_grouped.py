@@ -606,7 +606,8 @@ def test_outputs_that_autograd_follows_are_refused():
 
 
 def test_no_report_is_lost_between_two_reads():
-    """a kernel of another stream reports while the word is read: one of the reads, or one after both, has it"""
+    """a kernel of another stream reports while the word is read: one of the reads, or one after both, has it (two, where one
+    comes between the pair's two CTAs)"""
     L, status = _lib.lib(), ctypes.c_int(0)
     mine, other = torch.cuda.current_stream().cuda_stream, torch.cuda.Stream()
     read = lambda: L.spanqr_mm_read_status(mine, ctypes.byref(status))   # noqa: E731
@@ -617,7 +618,7 @@ def test_no_report_is_lost_between_two_reads():
         while not other.query():
             reports += read() != 0
         reports += read() != 0
-        assert reports == 1, i
+        assert 1 <= reports <= 2, (i, reports)
 
 
 def test_a_pair_whose_waits_ran_out_stays_until_what_it_issued_has_landed():
